@@ -340,6 +340,19 @@ int b200_embed_norm(const long long* ids, const void* table, long long ldt, int 
 int b200_attn_paged(const void* q, long long ldq, void* out, long long ldo, int hq, int M, const int* positions,
                     const int* seq_ids, const int* seq_lens, const b200_paged_cache* cache, const b200_attn_spec* spec,
                     int* status, cudaStream_t stream);
+// (positions NULL: the last tokens of sequences of lengths seq_lens)
+// Attention of single rows over the pages that always count and those whose keys' bounds promise most (attn_sparse.cu): `top` pages per KV head, the
+// `first` pages and the `last` up to the row's own among them.  bounds [pages][kv_heads][2][dk] as b200_page_bounds leaves them.  splits: CTAs (a
+// cluster) per row and KV head.  chosen [M][kv_heads][top] or NULL: the pages read, ascending, -1 behind them.
+int b200_attn_paged_sparse(const void* q, long long ldq, void* out, long long ldo, int hq, int M, const int* positions, const int* seq_ids,
+                           const int* seq_lens, const b200_paged_cache* cache, const void* bounds, const b200_attn_spec* spec, int top, int first,
+                           int last, int splits, int* chosen, int* status, cudaStream_t stream);
+// Smallest and largest element per dimension over the keys of a page that a sequence has, for the pages of tokens starts[i] .. ends[i] of every
+// portion (at most max_tokens of them; seq_ids NULL: portion i is of sequence i).
+int b200_page_bounds(const b200_paged_cache* cache, const int* starts, const int* ends, const int* seq_ids, int portions, int max_tokens, void* bounds,
+                     int* status, cudaStream_t stream);
+// Records src[i] -> dst[i] of every array (record lengths in bytes, multiples of 16); page numbers on the host, no page both written and named again.
+int b200_copy_pages(void* const* arrays, const long long* records, int n_arrays, const int* src, const int* dst, int n, cudaStream_t stream);
 // Prefill portions on the tensor cores (bf16, dk and dv up to 128, page size 16): rows [cu[b], cu[b+1]) are consecutive
 // positions of one sequence whose keys up to there are in the cache already.
 int b200_attn_prefill_paged(const void* q, long long ldq, void* out, long long ldo, int hq, int M, int B, int max_len,

@@ -57,8 +57,8 @@ __global__ void __launch_bounds__(32 * APG_WARPS) attn_paged_kernel(const __grid
   const int dk = p.c.dk, dv = p.dv, ps = p.c.page_size, d0 = blockIdx.y * APG_MAX_DV, dn = min(dv - d0, APG_MAX_DV);
   const int seq = p.seq_ids ? p.seq_ids[tok] : tok;
   T* o = static_cast<T*>(p.out) + static_cast<size_t>(tok) * p.ldo + static_cast<size_t>(h) * dv + d0;
-  const int pos = p.positions[tok];
   const bool empty = p.seq_lens && p.seq_lens[tok] <= 0;            // decode over a slot without a sequence
+  const int pos = p.positions ? p.positions[tok] : empty ? 0 : p.seq_lens[tok] - 1;      // lengths alone: the last token
   const bool bad = pos < 0 || seq < 0 || seq >= p.c.num_seqs || pos / ps >= p.c.max_pages;
   if (bad || empty) {
     if (bad && threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, static_cast<int>(ST_BAD_ARGUMENT) | (14 << 8));
@@ -262,7 +262,7 @@ extern "C" int b200_attn_paged(const void* q, long long ldq, void* out, long lon
                                const int* seq_ids, const int* seq_lens, const b200_paged_cache* cache, const b200_attn_spec* spec,
                                int* status, cudaStream_t stream) {
   if (M <= 0) return 0;
-  if (!q || !out || !positions || !cache || !cache->data || !cache->page_table || !spec) return -1;
+  if (!q || !out || (!positions && !seq_lens) || !cache || !cache->data || !cache->page_table || !spec) return -1;
   if (hq <= 0 || cache->kv_heads <= 0 || hq % cache->kv_heads || cache->page_size <= 0 || cache->dk <= 0 || cache->dv <= 0) return -2;
   AttnPagedParams p = {};
   p.q = p.q2 = q; p.ldq = ldq; p.q_len = p.q_head = cache->dk; p.dv = cache->dv; p.out = out; p.ldo = ldo; p.hq = hq; p.M = M;

@@ -17,7 +17,7 @@ _KERNEL_NAMES = {
     1: "w8a8_gemm", 2: "w8a8_gemm_decode", 3: "attn_prefill", 4: "attn_decode_tma", 5: "attn_decode_tc", 6: "attn_decode_tcp", 7: "rope_kv_write",
     8: "attn_decode", 9: "bf16_gemm", 10: "bf16_gemm_decode", 11: "attn_prefill_paged", 12: "rotary_paged", 13: "attn_decode_paged", 14: "attn_paged",
     15: "latent_append", 16: "rotary_heads", 17: "latent_gather", 18: "attn_latent", 19: "attn_prefill_latent", 20: "w8a8_gemm_pair",
-    21: "bf16_gemm_pair", 22: "f32_gemm_tc", 23: "w8a8_gemm_experts",
+    21: "bf16_gemm_pair", 22: "f32_gemm_tc", 23: "w8a8_gemm_experts", 24: "page_bounds", 25: "attn_paged_sparse", 26: "attn_decode_shared",
 }
 
 

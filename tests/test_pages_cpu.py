@@ -1,0 +1,61 @@
+"""What copies of pages, their bounds and the attentions that select or share them refuse, before anything is launched."""
+import pytest
+import torch
+
+from mojo_linuxperiments_b200.ops import attention as A
+from mojo_linuxperiments_b200.ops import pages as PG
+from mojo_linuxperiments_b200.ops import shared as SH
+from mojo_linuxperiments_b200.ops import sparse as SP
+
+
+@pytest.mark.parametrize("src,dst,error", [([0], [1, 2], ValueError), ([0, 1], [2, 2], ValueError), ([0, 1], [1, 2], ValueError), ([3], [3], ValueError)])
+def test_copies_that_depend_on_their_order_are_refused(src, dst, error):
+    with pytest.raises(error):
+        PG.copy_pages(torch.zeros(4, 8), src, dst)
+
+
+def test_copies_of_nothing_and_of_tensors_elsewhere():
+    PG.copy_pages(torch.zeros(4, 8), [], [])
+    PG.copy_pages([], [1], [2])
+    with pytest.raises(ValueError):
+        PG.copy_pages(torch.zeros(4, 8), [0], [1])          # not on a GPU
+
+
+def _cache(dtype=torch.bfloat16, dk=32, dv=16):
+    return A.PagedKVCache(6, 2, 16, "cpu", dk=dk, dv=dv, dtype=dtype)
+
+
+def test_bounds_have_the_shape_and_type_of_the_keys():
+    c = _cache()
+    b = PG.bounds_for(c)
+    assert tuple(b.shape) == (6, 2, 2, 32) and b.dtype == torch.bfloat16
+    for bad in (b.float(), b[:5], b.transpose(2, 3), b[:, :1]):
+        with pytest.raises(ValueError):
+            PG.check_bounds(c, bad)
+
+
+def _sparse(**kw):
+    c = kw.pop("cache", _cache())
+    q, out = torch.zeros(3, 4 * c.dk, dtype=c.data.dtype), torch.zeros(3, 4 * c.dv, dtype=c.data.dtype)
+    args = dict(top=8, first=1, last=2)
+    args.update(kw)
+    scale, table = args.pop("scale", 0.1), args.pop("table", torch.zeros(3, 40, dtype=torch.int32))
+    return SP.attn_paged_sparse(q, 4, torch.zeros(3, dtype=torch.int32), None, c, table, args.pop("bounds", PG.bounds_for(c)), A.attn_spec(scale), out, **args)
+
+
+@pytest.mark.parametrize("kw", [dict(top=2), dict(last=0), dict(first=-1), dict(scale=0.0), dict(scale=-1.0), dict(table=torch.zeros(2, 40, dtype=torch.int32)),
+                                dict(cache=_cache(dk=520)), dict(cache=_cache(dv=0)), dict(bounds=torch.zeros(6, 2, 2, 32))])
+def test_selections_that_make_no_sense_are_refused(kw):
+    with pytest.raises(ValueError):
+        _sparse(**kw)
+
+
+@pytest.mark.parametrize("groups", [[([0, 0], 16)], [([0, 1], 16), ([1, 2], 32)], [([0, 4], 16)], [([0, -1], 16)], [([0, 1], 20)], [([0, 1], -16)]])
+def test_groups_that_make_no_sense_are_refused(groups):
+    with pytest.raises(ValueError):
+        SH.SharedPrefixes(4, "cpu").set(groups)
+
+
+@pytest.mark.parametrize("pairs,pages,want", [(8, 8192, 8), (64, 1000, 4), (512, 8192, 1), (512, 60000, 4), (2, 20, 1), (1, 40, 2)])
+def test_clusters_for_selections(pairs, pages, want):
+    assert SP.pick_sparse_splits(pairs, pages) == want
