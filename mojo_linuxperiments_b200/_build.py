@@ -38,7 +38,7 @@ KERNEL_LIB = "libb200_kernels.so"
 # such model from a fresh checkout compiles.
 KERNEL_VARIANTS = {"": [], "trace": ["-DB200RT_TRACE"], "debug": ["-DB200RT_DEBUG"], "dense": []}
 KERNEL_SUBSETS = {"dense": ("attn_decode_paged.cu", "attn_latent.cu", "attn_paged.cu", "attn_prefill_latent.cu",
-                            "attn_prefill_paged.cu", "attn_sparse.cu", "bf16_gemm.cu", "bf16_gemm_decode.cu", "bf16_gemm_pair.cu",
+                            "attn_prefill_paged.cu", "attn_shared.cu", "attn_sparse.cu", "bf16_gemm.cu", "bf16_gemm_decode.cu", "bf16_gemm_pair.cu",
                             "f32_gemm.cu", "f32_gemm_tc.cu", "latent.cu", "mingru.cu", "moe.cu", "moe_route.cu", "pages.cu", "rope_kv.cu", "rotary_paged.cu",
                             "stream_rows.cu", "tmap.cu", "trace.cu")}
 

@@ -1,0 +1,495 @@
+// Decode attention of sequences that share the pages of a prefix, on sm_100a tensor cores: the prefix is read once per group, not once per sequence.
+//
+//   o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m):  keys of the prefix and a sequence's own keys give (m, l, O) each, which are joined by
+//   m = max(m_1, m_2), l = sum l_i exp(m_i - m), O = sum O_i exp(m_i - m).
+//
+// Two launches.  The first takes the prefixes: the rows (member x query head) of a group are the M of tcgen05 MMAs over tiles of 128 keys, in pieces of
+// 128 rows and of some tiles, which leave (m, l, O) in fp32.  Which pieces there are is a list on the device, made when groups change, so that a captured call
+// follows them.  The second takes each sequence's own keys (decode_warp.cuh) while the first still runs, joins the pieces of the prefix, adds sink
+// and gate and writes the output; it waits for the first only there.
+#include "ptx.cuh"
+#include "api.h"
+#include "launch.cuh"
+#include "gemm_common.cuh"
+#include "decode_warp.cuh"
+
+namespace b200 {
+
+// ---- the plan: int32 on the device -------------------------------------------------------------------------------------------------
+// [0] pieces, then at SP_INFO four numbers per slot: first row of its partial results, rows between the parts of the prefix, parts, tokens;
+// then the pieces, eight numbers each; then the slots of the groups' members.
+constexpr int SP_INFO = 16, SP_PIECE = 8;
+struct SharedPiece { int member0, members, row0, rows, key0, key1, part, unused; };   // members: place in the list of slots, number of them in the group; rows within the group
+
+struct SharedParams {
+  const __nv_bfloat16* q; long long ldq;
+  __nv_bfloat16* out; long long ldo;
+  int hq, B;
+  const int* seq_lens;
+  const int* plan; int pieces_at, slots_at, max_pieces;
+  float* part; int part_rows;            // [kv_heads][part_rows][dv], then (m, l) [kv_heads][part_rows][2]
+  b200_paged_cache c;
+  int chunk;
+  float scale;
+  const float* sink;
+  const __nv_bfloat16* gate; long long ldg;
+  int splits, hgroups;
+  int* status;
+  unsigned long long limit_ns;
+};
+
+// ---- prefixes -----------------------------------------------------------------------------------------------------------------------
+// One piece at a time per CTA, two CTAs per SM, which fill each other's gaps: warp 0 fetches pages by TMA (lane <-> page), warp 1 issues the MMAs, warps
+// 4..7 gather the queries, take the softmax (thread <-> row) and keep O in tensor memory.  One tile of keys and one of values in shared memory: the next
+// keys are requested once the scores are there, the next values once they are used.
+constexpr int SX_THREADS = 256, SX_BN = 128, SX_PS = 16;
+// registers: 256 x 128 at launch, 128 x (40 + 216) afterwards, which is as many
+constexpr int SX_REGS_FEW = 40, SX_REGS_MANY = 216;
+constexpr int SX_CHUNK = 128 * 128, SX_TILE = 2 * SX_CHUNK;
+constexpr int SX_SMEM = 3 * SX_TILE + 1024 + 256;
+
+__global__ void __launch_bounds__(SX_THREADS, 2)
+attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ SharedParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sQ = smem_u32(smem), sK = sQ + SX_TILE, sV = sK + SX_TILE;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 3 * SX_TILE);
+  const uint32_t bar0 = smem_u32(bars);
+  enum { B_KFULL = 0, B_VFULL, B_SFULL, B_PFULL, B_PVDONE, B_COUNT };
+  auto bar = [&](int i) { return bar0 + 8u * i; };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + B_COUNT);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* span = reinterpret_cast<int*>(tmem_slot + 2);         // keys that some row of the piece sees: first, end
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int dk = p.c.dk, dv = p.c.dv, hkv = p.c.kv_heads, group = p.hq / hkv;
+  const int kchunks = (dk + 63) >> 6, vchunks = (dv + 63) >> 6, ksteps = (dk + 15) >> 4, dv16 = (dv + 15) & ~15;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < B_COUNT; ++i) mbar_init(bar(i), i == B_PFULL ? 4 : 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) { tmem_alloc(smem_u32(tmem_slot), 256); tmem_relinquish(); }
+  if (threadIdx.x == 32 * 2) { prefetch_tmap(&tmap_k); prefetch_tmap(&tmap_v); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;              // S (then P) in 128 columns, O in the next 128
+  pdl_wait();
+  pdl_launch_dependents();       // what starts now may read all that was written before this kernel
+  auto wait = [&](int i, uint32_t par, int code) { return mbar_wait(bar(i), par, abort_flag, p.status, code | (26 << 8), p.limit_ns); };
+  auto meet = [&] { named_bar_sync(1, SX_THREADS); };        // all warps, from the two branches that they are in
+  const int pieces = min(p.plan[0], p.max_pieces) * hkv;
+  auto piece_of = [&](int item) { return *reinterpret_cast<const SharedPiece*>(p.plan + p.pieces_at + (item / hkv) * SP_PIECE); };
+  // tiles of 128 keys from the page of the first key that counts
+  auto tiles_of = [&](int& kv_start, int& kv_end) {
+    kv_start = span[0] & ~(SX_PS - 1);
+    kv_end = span[1];
+    return kv_end > 0 ? (kv_end - kv_start + SX_BN - 1) / SX_BN : 0;
+  };
+  uint32_t done = 0;                             // tiles so far: their parities
+  if (warp < 4) {
+    warpgroup_regs_dec<SX_REGS_FEW>();
+    for (int item = blockIdx.x; item < pieces; item += gridDim.x) {
+      const int kvh = item % hkv;
+      const SharedPiece e = piece_of(item);
+      if (threadIdx.x == 0) { span[0] = 0x7fffffff; span[1] = 0; }
+      meet();
+      meet();                                    // the queries are in place, and what they see is known
+      int kv_start, kv_end;
+      const int n = tiles_of(kv_start, kv_end);
+      if (warp == 0) {
+        const int lead = p.plan[p.slots_at + e.member0];
+        const int* pt = p.c.page_table + static_cast<size_t>(lead) * p.c.max_pages;
+        auto page_of = [&](int j) {
+          const int tok = kv_start + j * SX_BN + (lane & 7) * SX_PS;
+          const int pg = tok < kv_end ? pt[tok / SX_PS] : p.c.num_pages;       // pages behind the end are filled with zeros
+          if (pg >= 0 && pg <= p.c.num_pages) return pg;
+          if (p.status) atomicCAS(p.status, 0, static_cast<int>(ST_BAD_ARGUMENT) | (26 << 8));
+          return p.c.num_pages;
+        };
+        auto load = [&](uint32_t dst, const CUtensorMap* m, int b, int chunks, int page) {
+          if (lane == 0) mbar_expect_tx(bar(b), chunks * SX_CHUNK);
+          __syncwarp();
+          if (lane < 8)
+            for (int c = 0; c < chunks; ++c) tma_load_3d(dst + c * SX_CHUNK + lane * 2048, m, bar(b), c * 64, kvh * SX_PS, page);
+        };
+        bool ok = true;
+        int page = n > 0 ? page_of(0) : 0;
+        for (int j = 0; j < n && ok; ++j) {
+          const int next = j + 1 < n ? page_of(j + 1) : 0;
+          // the scores of the tile before are there: its keys are no longer needed; its values once they have been multiplied
+          if (j > 0) ok = __all_sync(0xffffffffu, wait(B_SFULL, (done + j - 1) & 1u, ST_TIMEOUT_SMEM_EMPTY)) != 0;
+          if (!ok) break;
+          load(sK, &tmap_k, B_KFULL, kchunks, page);
+          if (j > 0) ok = __all_sync(0xffffffffu, wait(B_PVDONE, (done + j - 1) & 1u, ST_TIMEOUT_SMEM_EMPTY)) != 0;
+          if (!ok) break;
+          load(sV, &tmap_v, B_VFULL, vchunks, page);
+          page = next;
+        }
+        if (!ok) { const uint64_t t0 = globaltimer_ns(); while (globaltimer_ns() - t0 < 2000000ull) { } }   // copies in flight land
+      } else if (warp == 1) {
+        const bool one = elect_one();
+        constexpr uint32_t IDESC_S = umma_idesc_bf16(128, 128, 0, 0);
+        const uint32_t idesc_pv = umma_idesc_bf16(128, dv16, 0, 1);
+        const uint64_t q_desc = umma_desc_k_sw128(sQ), k_desc = umma_desc_k_sw128(sK), v_desc = umma_desc_mn_sw128(sV, SX_CHUNK, 1024);
+        bool ok = true;
+        for (int j = 0; j < n && ok; ++j) {
+          const uint32_t par = (done + j) & 1u;
+          ok = wait(B_KFULL, par, ST_TIMEOUT_SMEM_FULL);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) {
+            const uint32_t off = (kk >> 2) * (SX_CHUNK >> 4) + 2 * (kk & 3);
+            if (one && kk < ksteps) umma_f16_ss(tmem, q_desc + off, k_desc + off, IDESC_S, kk > 0 ? 1u : 0u);
+          }
+          if (one) umma_commit(bar(B_SFULL));
+          ok = wait(B_VFULL, par, ST_TIMEOUT_SMEM_FULL) && wait(B_PFULL, par, ST_TIMEOUT_TMEM_EMPTY);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)
+            if (one) umma_f16_ts(tmem + 128, tmem + kk * 8, v_desc + kk * (2048 >> 4), idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
+          if (one) umma_commit(bar(B_PVDONE));
+        }
+        __syncwarp();
+      }
+      done += n;
+      meet();
+      if (*abort_flag) break;                    // the same for all: nobody sets it between here and the next meeting
+    }
+  } else {
+    warpgroup_regs_inc<SX_REGS_MANY>();
+    const int r = (warp & 3) * 32 + lane;        // row of the piece, TMEM lane
+    const uint32_t t_s = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16), t_o = t_s + 128;
+    const float scale_log2 = p.scale * DW_LOG2E;
+    for (int item = blockIdx.x; item < pieces; item += gridDim.x) {
+      const int kvh = item % hkv;
+      const SharedPiece e = piece_of(item);
+      meet();
+      int low = 0, end = 0;                      // keys that the row sees of this piece
+      {
+        const int row = e.row0 + r, member = row / group;
+        const bool on = r < e.rows;
+        const int slot = on ? p.plan[p.slots_at + e.member0 + member] : 0;
+        const int len = on ? p.seq_lens[slot] : 0;
+        if (len > 0) {
+          low = max(e.key0, p.chunk > 0 ? (len - 1) - (len - 1) % p.chunk : 0);
+          end = min(min(e.key1, len), p.c.max_pages * SX_PS);
+          if (low >= end) end = 0;
+        }
+        if (end > 0) { atomicMin(&span[0], low); atomicMax(&span[1], end); }
+        const __nv_bfloat16* q = p.q + static_cast<size_t>(slot) * p.ldq + static_cast<size_t>(kvh * group + row - member * group) * dk;
+        for (int c = 0; c < kchunks; ++c)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int d = c * 64 + i * 8;
+            const uint4 w = on && d < dk ? *reinterpret_cast<const uint4*>(q + d) : make_uint4(0u, 0u, 0u, 0u);
+            *reinterpret_cast<uint4*>(smem + c * SX_CHUNK + r * 128 + ((i ^ (r & 7)) << 4)) = w;
+          }
+        fence_proxy_async_smem();
+      }
+      meet();
+      int kv_start, kv_end;
+      const int n = tiles_of(kv_start, kv_end);
+      const bool idle = (warp & 3) * 32 >= e.rows;          // rows that nobody asked for: their weights are never looked at
+      float m_ref = -INFINITY, l = 0.f;
+      bool ok = true;
+      for (int j = 0; j < n && ok; ++j) {
+        const uint32_t par = (done + j) & 1u;
+        ok = __all_sync(0xffffffffu, wait(B_SFULL, par, ST_TIMEOUT_TMEM_FULL)) != 0;
+        if (!ok) break;
+        tc_fence_after();
+        if (!idle) {
+          uint32_t v[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld_x32(t_s + c * 32, v[c]);
+          tmem_ld_wait();
+          const int kv0 = kv_start + j * SX_BN, a = low - kv0, b = end - kv0;
+          if (__any_sync(0xffffffffu, a > 0 || b < SX_BN)) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int i = 0; i < 32; ++i) if (c * 32 + i < a || c * 32 + i >= b) v[c][i] = 0xff800000u;      // -inf
+          }
+          float mx[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            mx[c] = __uint_as_float(v[c][0]);
+#pragma unroll
+            for (int i = 1; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(v[c][i]));
+          }
+          const float m_new = fmaxf(m_ref, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2);
+          if (__any_sync(0xffffffffu, m_new > m_ref)) {
+            const float alpha = m_ref == -INFINITY ? 0.f : dw_exp2(m_ref - m_new);
+            l *= alpha;
+            m_ref = m_new;
+            if (j > 0) {       // the product before has completed: S of this tile was issued after it
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                if (c * 32 >= dv16) break;
+                uint32_t o[32];
+                tmem_ld_x32(t_o + c * 32, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                tmem_st_x32(t_o + c * 32, o);
+              }
+            }
+          }
+          const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float e0 = dw_exp2(__uint_as_float(v[c][2 * i]) * scale_log2 - m_use), e1 = dw_exp2(__uint_as_float(v[c][2 * i + 1]) * scale_log2 - m_use);
+              const __nv_bfloat162 pb = __floats2bfloat162_rn(e0, e1);
+              pk[i] = *reinterpret_cast<const uint32_t*>(&pb);
+              sum[c] += __uint_as_float(pk[i] << 16) + __uint_as_float(pk[i] & 0xffff0000u);     // what the MMA will actually see
+            }
+            tmem_st_x16(t_s + c * 16, pk);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_st_wait();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_PFULL));
+      }
+      if (ok && n > 0) ok = __all_sync(0xffffffffu, wait(B_PVDONE, (done + n - 1) & 1u, ST_TIMEOUT_TMEM_FULL)) != 0;
+      tc_fence_after();
+      if (ok && !idle) {
+        const size_t to = static_cast<size_t>(kvh) * p.part_rows + e.part + e.row0 + r;
+        const bool mine = r < e.rows;
+        if (mine) {
+          float* ml = p.part + static_cast<size_t>(hkv) * p.part_rows * dv + 2 * to;
+          ml[0] = n > 0 ? m_ref : -INFINITY;
+          ml[1] = l;
+        }
+        if (n > 0) {
+          float4* dst = reinterpret_cast<float4*>(p.part + to * dv);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            if (c * 32 >= dv16) break;
+            uint32_t o[32];
+            tmem_ld_x32(t_o + c * 32, o);
+            tmem_ld_wait();
+            if (mine) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (c * 32 + i * 4 < dv)
+                  dst[c * 8 + i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+            }
+          }
+        }
+      }
+      tc_fence_before();
+      done += n;
+      meet();
+      tc_fence_after();
+      if (*abort_flag) break;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem, 256); }
+}
+
+// ---- own keys, and the join ---------------------------------------------------------------------------------------------------------
+// Grid (split, KV head x group of up to 16 query heads, slot); the splits of a slot are a cluster.  Four warps take pages in turn.
+constexpr int SO_THREADS = 128, SO_WARPS = 4, SO_PARTS = 32;
+template <int DV> struct SoShape {
+  static constexpr int PITCH = DV + 4, SIZE = 16 * PITCH + 32;
+  static constexpr int SMEM = ((SO_WARPS + 1) * SIZE + 16 * (8 + SO_PARTS)) * 4;
+};
+
+template <int DK, int DV, bool FULL>
+__global__ void __launch_bounds__(SO_THREADS, 2) attn_shared_own_kernel(const __grid_constant__ SharedParams p) {
+  using Sh = SoShape<DV>;
+  extern __shared__ __align__(16) float so_smem[];
+  pdl_launch_dependents();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = blockIdx.x, S = p.splits, b = blockIdx.z;
+  const int kvh = blockIdx.y / p.hgroups, hg = blockIdx.y - kvh * p.hgroups;
+  const int group = p.hq / p.c.kv_heads, g0 = hg * 16, G = min(16, group - g0), h0 = kvh * group + g0;
+  const int dk = FULL ? DK : p.c.dk, dv = FULL ? DV : p.c.dv;
+  // the kernel in front of this one starts it after its own wait: lengths, queries, keys and plan are settled
+  const int len = p.seq_lens[b];
+  const int4 info = *reinterpret_cast<const int4*>(p.plan + SP_INFO + 4 * b);       // first row of the parts, rows between them, parts, tokens
+  const bool bad = len > p.c.max_pages * SX_PS;
+  if (len <= 0 || bad) {                         // the same for all CTAs of the cluster
+    if (bad && tid == 0 && p.status) atomicCAS(p.status, 0, static_cast<int>(ST_BAD_ARGUMENT) | (26 << 8));
+    pdl_wait();
+    if (rank == 0)
+      for (int i = tid; i < G * dv; i += SO_THREADS) p.out[static_cast<size_t>(b) * p.ldo + static_cast<size_t>(h0) * dv + i] = __float2bfloat16(0.f);
+    return;
+  }
+  const int low = max(p.chunk > 0 ? (len - 1) - (len - 1) % p.chunk : 0, min(info.w, len));      // first key that is this kernel's
+  const int t0 = low / SX_PS, tiles = low < len ? (len - 1) / SX_PS - t0 + 1 : 0;
+  const int ta = t0 + static_cast<int>(static_cast<long long>(tiles) * rank / S), tb = t0 + static_cast<int>(static_cast<long long>(tiles) * (rank + 1) / S);
+  const int mine = tb - ta > warp ? (tb - ta - warp + SO_WARPS - 1) / SO_WARPS : 0;
+  const int* pt = p.c.page_table + static_cast<size_t>(b) * p.c.max_pages;
+  const size_t rec = static_cast<size_t>(p.c.kv_heads) * SX_PS * (dk + dv);
+  const __nv_bfloat16* kbase = static_cast<const __nv_bfloat16*>(p.c.data) + static_cast<size_t>(kvh) * SX_PS * dk;
+  const __nv_bfloat16* vbase = static_cast<const __nv_bfloat16*>(p.c.data) + static_cast<size_t>(p.c.kv_heads) * SX_PS * dk + static_cast<size_t>(kvh) * SX_PS * dv;
+
+  DecodeWarp<DK, DV, FULL> w;
+  w.begin(dk, dv, p.scale);
+  // the ids of this warp's next 32 pages are in its lanes
+  int ids = 0, ids_from = -32;
+  auto page_of = [&](int i) {
+    if (i >= ids_from + 32) {
+      ids_from = i;
+      ids = i + lane < mine ? pt[ta + warp + (i + lane) * SO_WARPS] : -1;
+    }
+    const int page = __shfl_sync(0xffffffffu, ids, i - ids_from);
+    return page < p.c.num_pages ? page : -1;
+  };
+  auto lo_of = [&](int i) { return max(0, low - (ta + warp + i * SO_WARPS) * SX_PS); };
+  auto hi_of = [&](int i) { return min(SX_PS, len - (ta + warp + i * SO_WARPS) * SX_PS); };
+  if (mine > 0) {
+    int page = page_of(0);
+    w.load_k(kbase + (page >= 0 ? page * rec : 0), page >= 0);
+    w.q.load(p.q + static_cast<size_t>(b) * p.ldq + static_cast<size_t>(h0) * dk, G, dk);
+    w.load_v(vbase + (page >= 0 ? page * rec : 0), lo_of(0), page >= 0 ? hi_of(0) : 0);
+    for (int i = 0; i < mine; ++i) {
+      if (page < 0 && lane == 0 && p.status) atomicCAS(p.status, 0, static_cast<int>(ST_BAD_ARGUMENT) | (26 << 8));
+      float s[2][4];
+      w.scores(s);
+      const int here = page;
+      if (i + 1 < mine) {
+        page = page_of(i + 1);
+        w.load_k(kbase + (page >= 0 ? page * rec : 0), page >= 0);
+      }
+      if (here >= 0) {
+        uint32_t pr[4];
+        w.weigh(s, lo_of(i), hi_of(i), pr);
+        w.add(pr);
+      }
+      if (i + 1 < mine) w.load_v(vbase + (page >= 0 ? page * rec : 0), lo_of(i + 1), page >= 0 ? hi_of(i + 1) : 0);
+    }
+  }
+  w.end();
+  w.put(so_smem + warp * Sh::SIZE, Sh::PITCH, G);
+  __syncthreads();
+  float* own = so_smem + SO_WARPS * Sh::SIZE;
+  float* share = own + Sh::SIZE;                 // [16][8 + SO_PARTS]: what each part counts in the end
+  dw_join<SO_WARPS, SO_THREADS>(so_smem, Sh::SIZE, Sh::PITCH, G, dv, own);
+  if (S > 1) cluster_sync_all(); else __syncthreads();
+  pdl_wait();                                    // the parts of the prefix
+  const uint32_t own_addr = smem_u32(own);
+  const float* parts = p.part + (static_cast<size_t>(kvh) * p.part_rows + info.x + g0) * dv;
+  const float* ml = p.part + static_cast<size_t>(p.c.kv_heads) * p.part_rows * dv + 2 * (static_cast<size_t>(kvh) * p.part_rows + info.x + g0);
+  const int n_parts = min(info.z, SO_PARTS), all = S + n_parts;
+  // a warp per row: lanes take the parts
+  for (int g = warp; g < G; g += SO_WARPS) {
+    float m[2], l[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int i = lane + 32 * u;
+      m[u] = -INFINITY; l[u] = 0.f;
+      if (i < S) {
+        const uint32_t base = S > 1 ? mapa_shared(own_addr, i) : own_addr;
+        m[u] = dw_ld_cluster(base + 4u * (16 * Sh::PITCH + g));
+        l[u] = dw_ld_cluster(base + 4u * (16 * Sh::PITCH + 16 + g));
+      } else if (i < all) {
+        const float2 x = __ldcg(reinterpret_cast<const float2*>(ml + 2 * (static_cast<size_t>(i - S) * info.y + g)));
+        m[u] = x.x; l[u] = x.y;
+      }
+    }
+    const float sink2 = p.sink ? p.sink[h0 + g] * DW_LOG2E : -INFINITY;
+    float top = fmaxf(fmaxf(m[0], m[1]), sink2);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float use = top == -INFINITY ? 0.f : top;
+    const float f0 = m[0] == -INFINITY ? 0.f : dw_exp2(m[0] - use), f1 = m[1] == -INFINITY ? 0.f : dw_exp2(m[1] - use);
+    float total = f0 * l[0] + f1 * l[1];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    if (p.sink) total += dw_exp2(sink2 - use);
+    float f = total > 0.f ? 1.f / total : 0.f;
+    if (p.gate) f *= 1.f / (1.f + __expf(-__bfloat162float(p.gate[static_cast<size_t>(b) * p.ldg + h0 + g])));
+    if (lane < all) share[g * (8 + SO_PARTS) + lane] = f0 * f;
+    if (lane + 32 < all) share[g * (8 + SO_PARTS) + lane + 32] = f1 * f;
+  }
+  __syncthreads();
+  // four dimensions per thread, the parts in turn: their loads do not wait for one another
+  const int quads = dv >> 2;
+  for (int i = rank * SO_THREADS + tid; i < G * quads; i += S * SO_THREADS) {
+    const int g = i / quads, d = (i - g * quads) * 4;
+    const float* f = share + g * (8 + SO_PARTS);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < S; ++s) {
+      if (f[s] == 0.f) continue;
+      const uint32_t base = (S > 1 ? mapa_shared(own_addr, s) : own_addr) + 4u * (g * Sh::PITCH + d);
+      v.x += f[s] * dw_ld_cluster(base); v.y += f[s] * dw_ld_cluster(base + 4); v.z += f[s] * dw_ld_cluster(base + 8); v.w += f[s] * dw_ld_cluster(base + 12);
+    }
+#pragma unroll 4
+    for (int s = 0; s < n_parts; ++s) {
+      const float fs = f[S + s];
+      if (fs == 0.f) continue;                   // a part without keys has left no numbers
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(parts + (static_cast<size_t>(s) * info.y + g) * dv + d));
+      v.x += fs * x.x; v.y += fs * x.y; v.z += fs * x.z; v.w += fs * x.w;
+    }
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), c = __floats2bfloat162_rn(v.z, v.w);
+    *reinterpret_cast<uint2*>(p.out + static_cast<size_t>(b) * p.ldo + static_cast<size_t>(h0 + g) * dv + d) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&c));
+  }
+  if (S > 1) cluster_sync_all();                 // no CTA leaves while a peer may still read its part
+}
+
+template <int DK, int DV, bool FULL>
+static int launch_shared_own(const SharedParams& p, cudaStream_t stream) {
+  constexpr int SMEM = SoShape<DV>::SMEM;
+  cudaError_t e = cudaFuncSetAttribute(attn_shared_own_kernel<DK, DV, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+  if (e != cudaSuccess) return -1000 - static_cast<int>(e);
+  launch_ex(attn_shared_own_kernel<DK, DV, FULL>, dim3(p.splits, p.c.kv_heads * p.hgroups, p.B), dim3(SO_THREADS), SMEM, stream, p.splits, p);
+  e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : -2000 - static_cast<int>(e);
+}
+
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" int b200_attn_decode_shared_takes(const b200_paged_cache* c, int hq, long long ldq, long long ldo) {
+  return c && !c->f32 && c->page_size == SX_PS && c->dk > 0 && c->dv > 0 && c->dk <= 128 && c->dv <= 128 && c->dk % 8 == 0 && c->dv % 8 == 0 && c->kv_heads > 0 &&
+         hq % c->kv_heads == 0 && ldq % 8 == 0 && ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(c->data) & 15) == 0;
+}
+
+extern "C" int b200_attn_decode_shared(const void* q, long long ldq, void* out, long long ldo, int hq, int B, const int* seq_lens, const b200_paged_cache* c,
+                                       const b200_attn_spec* s, const int* plan, int pieces_at, int slots_at, int max_pieces, float* part, int part_rows,
+                                       int splits, int num_sms, int* status, cudaStream_t stream) {
+  if (B <= 0) return 0;
+  if (!q || !out || !seq_lens || !c || !c->data || !c->page_table || !s || !plan || !part) return -1;
+  if (!b200_attn_decode_shared_takes(c, hq, ldq, ldo) || hq <= 0 || c->num_pages <= 0) return -2;
+  if (B > c->num_seqs || B > 65535 || splits < 1 || splits > 8 || max_pieces < 0 || part_rows <= 0 || num_sms <= 0) return -3;
+  if ((reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(out) & 7) || (reinterpret_cast<uintptr_t>(plan) & 15) ||
+      (reinterpret_cast<uintptr_t>(part) & 15)) return -4;
+  const uint64_t rec = static_cast<uint64_t>(c->kv_heads) * SX_PS * (c->dk + c->dv) * 2, kbytes = static_cast<uint64_t>(c->kv_heads) * SX_PS * c->dk * 2;
+  CUtensorMap tk, tv;
+  if (make_tmap_3d_bf16(&tk, c->data, c->dk, static_cast<uint64_t>(c->kv_heads) * SX_PS, c->num_pages, static_cast<uint64_t>(c->dk) * 2, rec, SX_PS, 1)) return -12;
+  if (make_tmap_3d_bf16(&tv, static_cast<const uint8_t*>(c->data) + kbytes, c->dv, static_cast<uint64_t>(c->kv_heads) * SX_PS, c->num_pages,
+                        static_cast<uint64_t>(c->dv) * 2, rec, SX_PS, 1)) return -13;
+  SharedParams p = {};
+  p.q = static_cast<const __nv_bfloat16*>(q); p.ldq = ldq; p.out = static_cast<__nv_bfloat16*>(out); p.ldo = ldo; p.hq = hq; p.B = B; p.seq_lens = seq_lens;
+  p.plan = plan; p.pieces_at = pieces_at; p.slots_at = slots_at; p.max_pieces = max_pieces; p.part = part; p.part_rows = part_rows; p.c = *c; p.chunk = s->chunk;
+  p.scale = s->scale; p.sink = s->sink; p.gate = static_cast<const __nv_bfloat16*>(s->gate); p.ldg = s->ldg; p.splits = splits;
+  p.hgroups = (hq / c->kv_heads + 15) / 16; p.status = status; p.limit_ns = 2000000000ull;
+  if (static_cast<long long>(c->kv_heads) * p.hgroups > 65535) return -3;
+  cudaError_t e = cudaFuncSetAttribute(attn_shared_prefix_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SX_SMEM);
+  if (e != cudaSuccess) return -1000 - static_cast<int>(e);
+  const long long most = static_cast<long long>(max_pieces) * c->kv_heads;
+  const int grid = most < 2 * num_sms ? static_cast<int>(most > 0 ? most : 1) : 2 * num_sms;
+  launch_ex(attn_shared_prefix_kernel, dim3(grid), dim3(SX_THREADS), SX_SMEM, stream, 0, tk, tv, p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return -2000 - static_cast<int>(e);
+  const int d = c->dk > c->dv ? c->dk : c->dv;
+  if (c->dk == 64 && c->dv == 64) return launch_shared_own<64, 64, true>(p, stream);
+  if (c->dk == 128 && c->dv == 128) return launch_shared_own<128, 128, true>(p, stream);
+  if (d <= 64) return launch_shared_own<64, 64, false>(p, stream);
+  return launch_shared_own<128, 128, false>(p, stream);
+}

@@ -372,12 +372,13 @@ def rotary_paged(qkv: torch.Tensor, hq: int, positions: torch.Tensor, seq_ids: t
     _lib.check(rc, "rotary_paged")
 
 
-def attn_paged(q: torch.Tensor, hq: int, positions: torch.Tensor, seq_ids: torch.Tensor | None, cache: PagedKVCache,
+def attn_paged(q: torch.Tensor, hq: int, positions: torch.Tensor | None, seq_ids: torch.Tensor | None, cache: PagedKVCache,
                page_table: torch.Tensor, spec, out: torch.Tensor, seq_lens: torch.Tensor | None = None) -> torch.Tensor:
-    """General form: rows of q (already rotated; [M, hq dk], row stride free) against the cached keys of their sequence."""
+    """General form: rows of q (already rotated; [M, hq dk], row stride free) against the cached keys of their sequence.
+    ``positions`` None: the rows are the last tokens of sequences of lengths ``seq_lens``."""
     assert q.dtype == cache.data.dtype == out.dtype and q.stride(1) == 1 and out.stride(1) == 1
     rc = _lib.lib().b200_attn_paged(
-        q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), hq, q.shape[0], positions.data_ptr(), _lib.ptr(seq_ids),
+        q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), hq, q.shape[0], _lib.ptr(positions), _lib.ptr(seq_ids),
         _lib.ptr(seq_lens), ctypes.byref(cache.desc(page_table)), ctypes.byref(spec), default_workspace(q.device).status.data_ptr(),
         _lib.stream())
     _lib.check(rc, "attn_paged")

@@ -6,20 +6,88 @@ import ctypes
 import torch
 
 from . import _lib
-from .attention import PAGE, PagedKVCache
+from .attention import PAGE, PagedKVCache, attn_paged, pick_decode_splits_paged
 from .workspace import default_workspace
+
+KEY_TILE = 128                 # keys of a step of the kernel
+ROW_TILE = 128                 # rows (member x query head) of a piece
+MAX_PARTS = 32                 # parts of a prefix
+_INFO, _PIECE = 16, 8          # where the numbers per slot start, numbers per piece
+
+
+def cut_prefixes(groups, num_seqs: int, per_head: int, kv_heads: int, ctas: int):
+    """How the prefixes of ``groups`` (slots, tokens) are shared out: (four numbers per slot, pieces, slots in order, rows of partial results).
+
+    A piece is up to 128 rows of a group (whole members where a member has no more rows than that) and a run of tiles of 128 keys, for every KV head; runs
+    are as long as makes about ``ctas`` pieces of all of them.  A slot's numbers: first row of its partial results, rows between the parts, parts, tokens."""
+    tile_rows = ROW_TILE // per_head * per_head if per_head <= ROW_TILE else ROW_TILE
+    sizes = [(len(slots) * per_head, -(-tokens // KEY_TILE)) for slots, tokens in groups]
+    units = kv_heads * sum(-(-rows // tile_rows) * tiles for rows, tiles in sizes)
+    run = max(1, -(-units // ctas))
+    info, pieces, order, base = [0] * (4 * num_seqs), [], [], 0
+    for (slots, tokens), (rows, tiles) in zip(groups, sizes):
+        parts = min(MAX_PARTS, -(-tiles // run))
+        for i, s in enumerate(slots):
+            info[4 * s:4 * s + 4] = [base + i * per_head, rows, parts, tokens]
+        for row0 in range(0, rows, tile_rows):
+            for k in range(parts):
+                a, b = tiles * k // parts * KEY_TILE, min(tokens, tiles * (k + 1) // parts * KEY_TILE)
+                pieces.append([len(order), len(slots), row0, min(tile_rows, rows - row0), a, b, base + k * rows, 0])
+        base += rows * parts
+        order += slots
+    return info, pieces, order, base
+
+
+class _Cut:
+    """A plan as the kernels read it, for one number of heads, and room for partial results."""
+
+    def __init__(self, num_seqs: int, per_head: int, kv_heads: int, dv: int, device: torch.device):
+        self.per_head, self.kv_heads, self.sms = per_head, kv_heads, _lib.num_sms(device.index)
+        self.ctas = 2 * self.sms
+        per_cta = -(-self.ctas // kv_heads)
+        tiles_each = -(-per_head // ROW_TILE) if per_head > ROW_TILE else 1
+        self.max_pieces = per_cta + num_seqs * tiles_each
+        self.rows = max(1, num_seqs * per_head + ROW_TILE * per_cta)
+        self.pieces_at = (_INFO + 4 * num_seqs + 7) // 8 * 8
+        self.slots_at = self.pieces_at + _PIECE * self.max_pieces
+        n = self.slots_at + num_seqs
+        self.plan = torch.zeros(n, dtype=torch.int32, device=device)
+        self.part = torch.empty(kv_heads * self.rows * (dv + 2), dtype=torch.float32, device=device)
+        # a ring: a copy still queued on the stream never sees an edit that belongs to a later step
+        self.ring = [(torch.zeros(n, dtype=torch.int32).pin_memory(), torch.cuda.Event()) for _ in range(4)]
+        self.turn = 0
+
+    def send(self, groups, num_seqs: int) -> None:
+        info, pieces, order, rows = cut_prefixes(groups, num_seqs, self.per_head, self.kv_heads, self.ctas)
+        assert len(pieces) <= self.max_pieces and rows <= self.rows
+        buf, done = self.ring[self.turn]
+        self.turn = (self.turn + 1) % len(self.ring)
+        done.synchronize()                       # its previous copy has left the buffer
+        buf[0] = len(pieces)
+        buf[_INFO:_INFO + 4 * num_seqs] = torch.tensor(info, dtype=torch.int32)
+        if pieces:
+            buf[self.pieces_at:self.pieces_at + _PIECE * len(pieces)] = torch.tensor(pieces, dtype=torch.int32).flatten()
+            buf[self.slots_at:self.slots_at + len(order)] = torch.tensor(order, dtype=torch.int32)
+        self.plan.copy_(buf, non_blocking=True)
+        done.record()
 
 
 class SharedPrefixes:
     """Which sequence slots share the pages of their first tokens: groups of slots, each with a number of tokens (whole pages of 16).  A slot is in
-    one group at most; one in none reads its keys alone.  Kept from step to step, like the page table."""
+    one group at most; one in none reads its keys alone.
+
+    Kept from step to step, like the page table; ``set`` changes it between steps, also under captured calls, which follow it.  It holds the room for
+    partial results as well: calls that may overlap on the GPU (different streams) use different objects."""
 
     def __init__(self, num_seqs: int, device):
-        self.num_seqs, self.device = num_seqs, torch.device(device)
+        self.num_seqs, self.device = int(num_seqs), torch.device(device)
         self.groups: list[tuple[list[int], int]] = []
+        self.longest = 0                          # tokens of the longest prefix
+        self.alone = 0                            # tokens that every slot shares at least
+        self._cuts: dict[tuple, _Cut] = {}
 
     def set(self, groups) -> None:
-        """``groups``: (slots, tokens) each."""
+        """``groups``: (slots, tokens) each.  Stream-ordered, like ``KVState.flush``."""
         groups = [([int(s) for s in slots], int(tokens)) for slots, tokens in groups]
         every = [s for slots, _ in groups for s in slots]
         if len(set(every)) != len(every) or any(not 0 <= s < self.num_seqs for s in every):
@@ -27,21 +95,51 @@ class SharedPrefixes:
         if any(tokens < 0 or tokens % PAGE for _, tokens in groups):
             raise ValueError(f"prefixes of {[t for _, t in groups]} tokens: whole pages of {PAGE} are shared")
         self.groups = [(slots, tokens) for slots, tokens in groups if slots and tokens]
+        self.longest = max((t for _, t in self.groups), default=0)
+        covered = sum(len(slots) for slots, _ in self.groups)
+        self.alone = min((t for _, t in self.groups), default=0) if covered == self.num_seqs else 0
+        for cut in self._cuts.values():
+            cut.send(self.groups, self.num_seqs)
+
+    def cut_for(self, hq: int, cache: PagedKVCache) -> _Cut:
+        device = cache.data.device
+        key = (hq, cache.kv_heads, cache.dv, device.index)
+        cut = self._cuts.get(key)
+        if cut is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the first call with a plan sends it to the device: make one before the capture")
+            cut = self._cuts[key] = _Cut(self.num_seqs, hq // cache.kv_heads, cache.kv_heads, cache.dv, device)
+            cut.send(self.groups, self.num_seqs)
+        return cut
 
 
 def attn_decode_shared(q: torch.Tensor, hq: int, seq_lens: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor, shared: SharedPrefixes, spec,
-                       out: torch.Tensor) -> torch.Tensor:
+                       out: torch.Tensor, *, splits: int | None = None) -> torch.Tensor:
     """The last token of every slot (row b of q, already rotated, [B, hq dk], row stride free; its key is in the cache) against the first
-    ``seq_lens[b]`` cached tokens of slot b.  Slots of a group of ``shared`` have the same pages in front; an empty slot (length 0) gets zeros."""
+    ``seq_lens[b]`` cached tokens of slot b.  Slots of a group of ``shared`` have the same pages in front, which are read once for all of them (bf16 heads of up
+    to 128, pages of 16; otherwise every slot reads its own way through ``attn_paged``).  An empty slot (length 0) gets zeros.
+
+    ``splits``: CTAs that share a slot's own keys."""
     B = seq_lens.numel()
     assert q.dtype == cache.data.dtype == out.dtype and q.stride(1) == 1 and out.stride(1) == 1 and q.shape[0] == out.shape[0] == B
     assert q.shape[1] >= hq * cache.dk and out.shape[1] >= hq * cache.dv and hq % cache.kv_heads == 0
     assert seq_lens.dtype == page_table.dtype == torch.int32 and page_table.is_contiguous() and seq_lens.is_contiguous()
-    if B > page_table.shape[0] or B != shared.num_seqs:
-        raise ValueError(f"{B} rows, {page_table.shape[0]} sequences, a plan for {shared.num_seqs}")
+    room = page_table.shape[1] * cache.page_size
+    if B > page_table.shape[0] or B != shared.num_seqs or shared.longest > room:
+        raise ValueError(f"{B} rows, {page_table.shape[0]} sequences of up to {room} tokens, a plan for {shared.num_seqs} with prefixes of up to {shared.longest}")
+    desc = cache.desc(page_table)
     with torch.cuda.device(q.device):
-        rc = _lib.lib().b200_attn_paged(
-            q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), hq, B, None, None, seq_lens.data_ptr(), ctypes.byref(cache.desc(page_table)),
-            ctypes.byref(spec), default_workspace(q.device).status.data_ptr(), _lib.stream())
+        L = _lib.lib()
+        if not L.b200_attn_decode_shared_takes(ctypes.byref(desc), hq, q.stride(0), out.stride(0)) or q.data_ptr() % 16 or out.data_ptr() % 8:
+            return attn_paged(q, hq, None, None, cache, page_table, spec, out, seq_lens=seq_lens)
+        cut = shared.cut_for(hq, cache)
+        if splits is None:
+            keys = min(room - shared.alone, spec.chunk) if spec.chunk > 0 else room - shared.alone
+            splits = pick_decode_splits_paged(B, cache.kv_heads * ((hq // cache.kv_heads + 15) // 16), keys, cut.sms)
+        rc = L.b200_attn_decode_shared(
+            q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), hq, B, seq_lens.data_ptr(), ctypes.byref(desc), ctypes.byref(spec),
+            cut.plan.data_ptr(), cut.pieces_at, cut.slots_at, cut.max_pieces, cut.part.data_ptr(), cut.rows, splits, cut.sms,
+            default_workspace(q.device).status.data_ptr(), _lib.stream())
     _lib.check(rc, "attn_decode_shared")
+    _lib.LAUNCHES[0] += 1                        # two kernels
     return out
