@@ -343,10 +343,10 @@ int b200_attn_paged(const void* q, long long ldq, void* out, long long ldo, int 
 // (positions NULL: the last tokens of sequences of lengths seq_lens)
 // Attention of single rows over the pages that always count and those whose keys' bounds promise most (attn_sparse.cu): `top` pages per KV head, the
 // `first` pages and the `last` up to the row's own among them.  bounds [pages][kv_heads][2][dk] as b200_page_bounds leaves them.  splits: CTAs (a
-// cluster) per row and KV head.  chosen [M][kv_heads][top] or NULL: the pages read, ascending, -1 behind them.
+// cluster) per row and KV head.  scores [M][kv_heads][max_pages]: room.  chosen [M][kv_heads][top] or NULL: the pages read, ascending, -1 behind them.
 int b200_attn_paged_sparse(const void* q, long long ldq, void* out, long long ldo, int hq, int M, const int* positions, const int* seq_ids,
                            const int* seq_lens, const b200_paged_cache* cache, const void* bounds, const b200_attn_spec* spec, int top, int first,
-                           int last, int splits, int* chosen, int* status, cudaStream_t stream);
+                           int last, int splits, unsigned* scores, int* chosen, int* status, cudaStream_t stream);
 // Last tokens of sequences of which some share the pages of a prefix (attn_shared.cu; bf16, dk and dv up to 128, page size 16: _takes says which).  plan: which
 // pieces of which prefixes there are, on the device; part: room for their results, part_rows rows per KV head of dv + 2 floats.  splits: CTAs (a cluster)
 // per slot and KV head for the slot's own keys.

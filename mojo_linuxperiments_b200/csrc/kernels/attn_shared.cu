@@ -51,6 +51,8 @@ constexpr int SX_SMEM = 3 * SX_TILE + 1024 + 256;
 __global__ void __launch_bounds__(SX_THREADS, 2)
 attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ SharedParams p) {
   extern __shared__ uint8_t smem_raw[];
+  B200_TRACE_INIT();
+  if (threadIdx.x == 0) B200_TRACE(TK_ATTN_SHARED, TP_START);
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sQ = smem_u32(smem), sK = sQ + SX_TILE, sV = sK + SX_TILE;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 3 * SX_TILE);
@@ -76,6 +78,7 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;              // S (then P) in 128 columns, O in the next 128
   pdl_wait();
+  if (threadIdx.x == 0) B200_TRACE(TK_ATTN_SHARED, TP_DEPS);
   pdl_launch_dependents();       // what starts now may read all that was written before this kernel
   auto wait = [&](int i, uint32_t par, int code) { return mbar_wait(bar(i), par, abort_flag, p.status, code | (26 << 8), p.limit_ns); };
   auto meet = [&] { named_bar_sync(1, SX_THREADS); };        // all warps, from the two branches that they are in
@@ -191,6 +194,7 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
         fence_proxy_async_smem();
       }
       meet();
+      if (r == 0) B200_TRACE(TK_ATTN_SHARED, 2);             // queries in place
       int kv_start, kv_end;
       const int n = tiles_of(kv_start, kv_end);
       const bool idle = (warp & 3) * 32 >= e.rows;          // rows that nobody asked for: their weights are never looked at
@@ -200,6 +204,7 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
         const uint32_t par = (done + j) & 1u;
         ok = __all_sync(0xffffffffu, wait(B_SFULL, par, ST_TIMEOUT_TMEM_FULL)) != 0;
         if (!ok) break;
+        if (r == 0 && j == 0) B200_TRACE(TK_ATTN_SHARED, 3); // first scores
         tc_fence_after();
         if (!idle) {
           uint32_t v[4][32];
@@ -259,8 +264,10 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(B_PFULL));
       }
+      if (r == 0) B200_TRACE(TK_ATTN_SHARED, 4);             // last weights
       if (ok && n > 0) ok = __all_sync(0xffffffffu, wait(B_PVDONE, (done + n - 1) & 1u, ST_TIMEOUT_TMEM_FULL)) != 0;
       tc_fence_after();
+      if (r == 0) B200_TRACE(TK_ATTN_SHARED, 5);             // last product
       if (ok && !idle) {
         const size_t to = static_cast<size_t>(kvh) * p.part_rows + e.part + e.row0 + r;
         const bool mine = r < e.rows;
@@ -289,6 +296,7 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
       tc_fence_before();
       done += n;
       meet();
+      if (r == 0) B200_TRACE(TK_ATTN_SHARED, 6);             // a piece
       tc_fence_after();
       if (*abort_flag) break;
     }
@@ -296,20 +304,25 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
   tc_fence_before();
   __syncthreads();
   if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem, 256); }
+  if (threadIdx.x == 0) B200_TRACE(TK_ATTN_SHARED, TP_EXIT);
+  B200_TRACE_FLUSH(TK_ATTN_SHARED);
 }
 
 // ---- own keys, and the join ---------------------------------------------------------------------------------------------------------
 // Grid (split, KV head x group of up to 16 query heads, slot); the splits of a slot are a cluster.  Four warps take pages in turn.
 constexpr int SO_THREADS = 128, SO_WARPS = 4, SO_PARTS = 32;
+constexpr int SO_AHEAD = 6;              // pages of a warp asked for into L2 ahead of their use
 template <int DV> struct SoShape {
   static constexpr int PITCH = DV + 4, SIZE = 16 * PITCH + 32;
   static constexpr int SMEM = ((SO_WARPS + 1) * SIZE + 16 * (8 + SO_PARTS)) * 4;
 };
 
-template <int DK, int DV, bool FULL>
+template <int DK, int DV, int NH, bool FULL>
 __global__ void __launch_bounds__(SO_THREADS, 2) attn_shared_own_kernel(const __grid_constant__ SharedParams p) {
   using Sh = SoShape<DV>;
   extern __shared__ __align__(16) float so_smem[];
+  B200_TRACE_INIT();
+  if (threadIdx.x == 0) B200_TRACE(TK_ATTN_OWN, TP_START);
   pdl_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = blockIdx.x, S = p.splits, b = blockIdx.z;
@@ -336,50 +349,33 @@ __global__ void __launch_bounds__(SO_THREADS, 2) attn_shared_own_kernel(const __
   const __nv_bfloat16* kbase = static_cast<const __nv_bfloat16*>(p.c.data) + static_cast<size_t>(kvh) * SX_PS * dk;
   const __nv_bfloat16* vbase = static_cast<const __nv_bfloat16*>(p.c.data) + static_cast<size_t>(p.c.kv_heads) * SX_PS * dk + static_cast<size_t>(kvh) * SX_PS * dv;
 
-  DecodeWarp<DK, DV, FULL> w;
+  DecodeWarp<DK, DV, NH, FULL> w;
   w.begin(dk, dv, p.scale);
   // the ids of this warp's next 32 pages are in its lanes
   int ids = 0, ids_from = -32;
-  auto page_of = [&](int i) {
+  w.template walk<NH == 1>(mine, [&](int i) {
     if (i >= ids_from + 32) {
       ids_from = i;
       ids = i + lane < mine ? pt[ta + warp + (i + lane) * SO_WARPS] : -1;
+      if (lane > 0 && lane < SO_AHEAD) dw_prefetch(kbase, vbase, ids, rec, dk, dv, p.c.num_pages);
+    } else if (lane == i - ids_from + SO_AHEAD - 1) {
+      dw_prefetch(kbase, vbase, ids, rec, dk, dv, p.c.num_pages);
     }
-    const int page = __shfl_sync(0xffffffffu, ids, i - ids_from);
-    return page < p.c.num_pages ? page : -1;
-  };
-  auto lo_of = [&](int i) { return max(0, low - (ta + warp + i * SO_WARPS) * SX_PS); };
-  auto hi_of = [&](int i) { return min(SX_PS, len - (ta + warp + i * SO_WARPS) * SX_PS); };
-  if (mine > 0) {
-    int page = page_of(0);
-    w.load_k(kbase + (page >= 0 ? page * rec : 0), page >= 0);
-    w.q.load(p.q + static_cast<size_t>(b) * p.ldq + static_cast<size_t>(h0) * dk, G, dk);
-    w.load_v(vbase + (page >= 0 ? page * rec : 0), lo_of(0), page >= 0 ? hi_of(0) : 0);
-    for (int i = 0; i < mine; ++i) {
-      if (page < 0 && lane == 0 && p.status) atomicCAS(p.status, 0, static_cast<int>(ST_BAD_ARGUMENT) | (26 << 8));
-      float s[2][4];
-      w.scores(s);
-      const int here = page;
-      if (i + 1 < mine) {
-        page = page_of(i + 1);
-        w.load_k(kbase + (page >= 0 ? page * rec : 0), page >= 0);
-      }
-      if (here >= 0) {
-        uint32_t pr[4];
-        w.weigh(s, lo_of(i), hi_of(i), pr);
-        w.add(pr);
-      }
-      if (i + 1 < mine) w.load_v(vbase + (page >= 0 ? page * rec : 0), lo_of(i + 1), page >= 0 ? hi_of(i + 1) : 0);
-    }
-  }
-  w.end();
+    const int page = __shfl_sync(0xffffffffu, ids, i - ids_from), first = (ta + warp + i * SO_WARPS) * SX_PS;
+    const bool there = page >= 0 && page < p.c.num_pages;
+    if (!there && lane == 0 && p.status) atomicCAS(p.status, 0, static_cast<int>(ST_BAD_ARGUMENT) | (26 << 8));
+    const size_t at = there ? page * rec : 0;
+    return DwPage{kbase + at, vbase + at, max(0, low - first), there ? min(SX_PS, len - first) : 0};
+  }, [&] { w.q.load(p.q + static_cast<size_t>(b) * p.ldq + static_cast<size_t>(h0) * dk, G, dk); });
   w.put(so_smem + warp * Sh::SIZE, Sh::PITCH, G);
   __syncthreads();
+  if (tid == 0) B200_TRACE(TK_ATTN_OWN, 2);                  // own keys
   float* own = so_smem + SO_WARPS * Sh::SIZE;
   float* share = own + Sh::SIZE;                 // [16][8 + SO_PARTS]: what each part counts in the end
   dw_join<SO_WARPS, SO_THREADS>(so_smem, Sh::SIZE, Sh::PITCH, G, dv, own);
   if (S > 1) cluster_sync_all(); else __syncthreads();
   pdl_wait();                                    // the parts of the prefix
+  if (tid == 0) B200_TRACE(TK_ATTN_OWN, TP_DEPS);
   const uint32_t own_addr = smem_u32(own);
   const float* parts = p.part + (static_cast<size_t>(kvh) * p.part_rows + info.x + g0) * dv;
   const float* ml = p.part + static_cast<size_t>(p.c.kv_heads) * p.part_rows * dv + 2 * (static_cast<size_t>(kvh) * p.part_rows + info.x + g0);
@@ -439,16 +435,23 @@ __global__ void __launch_bounds__(SO_THREADS, 2) attn_shared_own_kernel(const __
         make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&c));
   }
   if (S > 1) cluster_sync_all();                 // no CTA leaves while a peer may still read its part
+  if (tid == 0) B200_TRACE(TK_ATTN_OWN, TP_EXIT);
+  B200_TRACE_FLUSH(TK_ATTN_OWN);
+}
+
+template <int DK, int DV, int NH, bool FULL>
+static int launch_shared_own_as(const SharedParams& p, cudaStream_t stream) {
+  constexpr int SMEM = SoShape<DV>::SMEM;
+  cudaError_t e = cudaFuncSetAttribute(attn_shared_own_kernel<DK, DV, NH, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+  if (e != cudaSuccess) return -1000 - static_cast<int>(e);
+  launch_ex(attn_shared_own_kernel<DK, DV, NH, FULL>, dim3(p.splits, p.c.kv_heads * p.hgroups, p.B), dim3(SO_THREADS), SMEM, stream, p.splits, p);
+  e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : -2000 - static_cast<int>(e);
 }
 
 template <int DK, int DV, bool FULL>
 static int launch_shared_own(const SharedParams& p, cudaStream_t stream) {
-  constexpr int SMEM = SoShape<DV>::SMEM;
-  cudaError_t e = cudaFuncSetAttribute(attn_shared_own_kernel<DK, DV, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
-  if (e != cudaSuccess) return -1000 - static_cast<int>(e);
-  launch_ex(attn_shared_own_kernel<DK, DV, FULL>, dim3(p.splits, p.c.kv_heads * p.hgroups, p.B), dim3(SO_THREADS), SMEM, stream, p.splits, p);
-  e = cudaGetLastError();
-  return e == cudaSuccess ? 0 : -2000 - static_cast<int>(e);
+  return p.hq / p.c.kv_heads <= 8 ? launch_shared_own_as<DK, DV, 1, FULL>(p, stream) : launch_shared_own_as<DK, DV, 2, FULL>(p, stream);
 }
 
 }  // namespace b200

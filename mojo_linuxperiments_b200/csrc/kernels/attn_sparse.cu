@@ -1,13 +1,13 @@
-// Attention of single rows of queries over the pages of their sequences that look most promising: scores of all pages, selection and attention in one launch.
+// Attention of single rows of queries over the pages of their sequences that look most promising.
 //
 // A page's score for a KV head bounds what any of its query heads can get from any key of the page: with lo <= k <= hi per dimension,
 //   q . k <= sum_d max(q_d lo_d, q_d hi_d) = q+ . hi + q- . lo,      q+ = max(q, 0), q- = min(q, 0),
 // and the score is the largest of the group's heads.  The first pages, and the last up to the row's own position, are read always; the others compete.
 //
-// Grid (split, KV head x group of up to 16 query heads, row); the splits of a row are a thread-block cluster.  Each scores its share of the pages into
-// shared memory, the cluster selects (page_select.cuh), each reads its share of the selected pages, and the parts are joined through distributed
-// shared memory.  Bound by the bytes of the bounds, 2 dk per page, and of the pages taken.
-//
+// Two launches.  The first scores all pages of all rows, spread over the whole chip; bound by the bytes of the bounds, 2 dk per page.  The second has a
+// cluster of CTAs per row and group of heads: each selects (page_select.cuh), reads its share of the pages taken, and the sums are joined
+// through distributed shared memory, every CTA joining a slice of the dimensions.  (One launch of clusters that scored, selected and read took 32 us where these
+// two take 18, 131,071 keys and 8 KV heads: eight clusters keep 64 of 148 SMs busy with the scores, and clusters of 16 do not all run at once.)
 #include "ptx.cuh"
 #include "api.h"
 #include "launch.cuh"
@@ -21,9 +21,185 @@ __device__ __forceinline__ float as_f(float v) { return v; }
 __device__ __forceinline__ float as_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float as_max(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 
-// ---- any head size up to 512, bf16 or fp32: a warp per page, lanes along the dimensions ------------------------------------------------
+// =====================================================================================================================================
+// scores.  Grid (pages, KV head, row)
+// =====================================================================================================================================
+constexpr int SC_WARPS = 8, SC_THREADS = 32 * SC_WARPS;
+
+// ---- any head size, bf16 or fp32: a warp per page, lanes along the dimensions, the queries in shared memory ------------------------------
+constexpr int SCA_PAGES = 4 * SC_WARPS;
 constexpr int AS_MAX_D = 512, AS_PER_LANE = AS_MAX_D / 32;
 
+template <typename T>
+__global__ void __launch_bounds__(SC_THREADS) page_scores_any_kernel(const __grid_constant__ SparseParams p) {
+  extern __shared__ __align__(16) float sc_q[];      // [heads of the group][dk]
+  pdl_wait();
+  pdl_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tok = blockIdx.z, kvh = blockIdx.y;
+  const int group = p.hq / p.c.kv_heads, dk = p.c.dk;
+  SparseRow row;
+  if (!row.find(p, tok) || !row.selects || static_cast<int>(blockIdx.x) * SCA_PAGES >= row.candidates) return;
+  const T* q = static_cast<const T*>(p.q) + static_cast<size_t>(tok) * p.ldq + static_cast<size_t>(kvh) * group * dk;
+  for (int i = threadIdx.x; i < group * dk; i += SC_THREADS) sc_q[i] = as_f(q[i]);
+  __syncthreads();
+  const int* pt = p.c.page_table + static_cast<size_t>(row.seq) * p.c.max_pages + row.place0;
+  unsigned* to = p.scores + (static_cast<size_t>(tok) * p.c.kv_heads + kvh) * p.c.max_pages;
+  for (int i = blockIdx.x * SCA_PAGES + warp; i < min(row.candidates, static_cast<int>(blockIdx.x + 1) * SCA_PAGES); i += SC_WARPS) {
+    const int page = pt[i];
+    float s = -INFINITY;
+    if (page >= 0 && page < p.c.num_pages) {
+      const T* lo = static_cast<const T*>(p.bounds) + (static_cast<size_t>(page) * p.c.kv_heads + kvh) * 2 * dk;
+      float a[AS_PER_LANE], b[AS_PER_LANE];
+#pragma unroll
+      for (int j = 0; j < AS_PER_LANE; ++j) {
+        const int d = lane + 32 * j;
+        a[j] = d < dk ? as_f(lo[d]) : 0.f;
+        b[j] = d < dk ? as_f(lo[dk + d]) : 0.f;
+      }
+      for (int h = 0; h < group; ++h) {
+        float t = 0.f;
+#pragma unroll
+        for (int j = 0; j < AS_PER_LANE; ++j) {
+          const int d = lane + 32 * j;
+          if (d < dk) {
+            const float x = sc_q[h * dk + d];
+            t = fmaf(fmaxf(x, 0.f), b[j], fmaf(fminf(x, 0.f), a[j], t));
+          }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+        s = as_max(s, t);
+      }
+    }
+    if (lane == 0) to[i] = ps_order(s);
+  }
+}
+
+// ---- bf16, head sizes up to 128: tensor cores ----------------------------------------------------------------------------------------------
+// Products with [lo, hi] of 2 dk numbers, q- against lo and q+ against hi: the same MMAs as for keys, 16 pages in the place of 16 keys
+// (decode_warp.cuh has the order of the dimensions).  A warp has two steps of 16 pages, 8 KiB of bounds each, the second's requested as the first's are used.  Sums are
+// fp32 and their terms exact.
+constexpr int SC_PAGES = 32 * SC_WARPS;
+
+__device__ __forceinline__ uint32_t as_above(uint32_t x) {      // the larger of each half and zero; NaN stays
+  const __nv_bfloat162 v = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&x), __floats2bfloat162_rn(0.f, 0.f));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t as_below(uint32_t x) {
+  const __nv_bfloat162 v = __hmin2_nan(*reinterpret_cast<const __nv_bfloat162*>(&x), __floats2bfloat162_rn(0.f, 0.f));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// s += q' . bounds, one half of the bounds of sixteen pages (rows lane / 4 and lane / 4 + 8): pages g, g, g + 8, g + 8 of heads 2 t, 2 t + 1.  Two
+// sums each, so that an MMA need not wait for the one before.
+template <int DK, int NH, bool UP>
+__device__ __forceinline__ void score_half(float (&s)[NH][2][4], const DwQuery<DK, NH>& q, const uint4 (&b)[2][DK / 32]) {
+  auto f = [](uint32_t x) { return UP ? as_above(x) : as_below(x); };
+#pragma unroll
+  for (int c = 0; c < DK / 32; ++c)
+#pragma unroll
+    for (int n = 0; n < NH; ++n) {
+      const uint4 x = q.h[n][c];
+      dw_mma(s[n][0], b[0][c].x, b[1][c].x, b[0][c].y, b[1][c].y, f(x.x), f(x.y));
+      dw_mma(s[n][1], b[0][c].z, b[1][c].z, b[0][c].w, b[1][c].w, f(x.z), f(x.w));
+    }
+}
+
+template <int DK, int NH, bool FULL>
+__global__ void __launch_bounds__(SC_THREADS, NH == 1 ? 2 : 1) page_scores_kernel(const __grid_constant__ SparseParams p) {
+  using bf16 = __nv_bfloat16;
+  B200_TRACE_INIT();
+  if (threadIdx.x == 0) B200_TRACE(TK_ATTN_OWN, TP_START);
+  pdl_wait();
+  pdl_launch_dependents();       // what starts now may read all that was written before this kernel
+  if (threadIdx.x == 0) B200_TRACE(TK_ATTN_OWN, TP_DEPS);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tok = blockIdx.z, kvh = blockIdx.y;
+  const int group = p.hq / p.c.kv_heads, dk = FULL ? DK : p.c.dk, g = lane >> 2, t = lane & 3;
+  SparseRow row;
+  if (!row.find(p, tok) || !row.selects || static_cast<int>(blockIdx.x) * SC_PAGES >= row.candidates) return;
+  const bf16* q = static_cast<const bf16*>(p.q) + static_cast<size_t>(tok) * p.ldq + static_cast<size_t>(kvh) * group * dk;
+  unsigned* to = p.scores + (static_cast<size_t>(tok) * p.c.kv_heads + kvh) * p.c.max_pages;
+  const int a = blockIdx.x * SC_PAGES + warp * 32, b = min(row.candidates, a + 32);
+  if (a < b) {
+    const int ids = a + lane < b ? p.c.page_table[static_cast<size_t>(row.seq) * p.c.max_pages + row.place0 + a + lane] : -1;
+    DwQuery<DK, NH> w;
+    uint4 lo[2][DK / 32], hi[2][DK / 32];
+    const bf16* from[2];
+    auto find = [&](int i) {                     // pages a + i .. a + i + 15: this lane's two; whether they are there
+      unsigned there = 0u;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int page = __shfl_sync(0xffffffffu, ids, i + g + 8 * u);
+        const bool on = page >= 0 && page < p.c.num_pages;
+        from[u] = static_cast<const bf16*>(p.bounds) + (static_cast<size_t>(on ? page : 0) * p.c.kv_heads + kvh) * 2 * dk + t * 8;
+        there |= static_cast<unsigned>(on) << u;
+      }
+      return there;
+    };
+    auto request = [&](uint4 (&x)[2][DK / 32], int at, unsigned there) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int c = 0; c < DK / 32; ++c) x[u][c] = dw_load(from[u] + at + c * 32, ((there >> u) & 1u) && (FULL || c * 32 + t * 8 < dk));
+    };
+    for (int n0 = 0; n0 < group; n0 += 8 * NH) {             // more than 16 heads: the bounds once for every 16
+      const int n = min(8 * NH, group - n0);
+      unsigned there = find(0);
+      request(lo, 0, there);
+      request(hi, dk, there);
+      w.load(q + static_cast<size_t>(n0) * dk, n, dk);
+#pragma unroll 1
+      for (int i = 0; i < b - a; i += 16) {
+        float s[NH][2][4];
+#pragma unroll
+        for (int h = 0; h < NH; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[h][0][e] = s[h][1][e] = 0.f;
+        const unsigned here = there;
+        const bool more = i + 16 < b - a;
+        score_half<DK, NH, false>(s, w, lo);
+        if (more) { there = find(16); request(lo, 0, there); }
+        score_half<DK, NH, true>(s, w, hi);
+        if (more) request(hi, dk, there);
+        float best[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int h = 0; h < NH; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (8 * h + 2 * t + (e & 1) < n) best[e >> 1] = as_max(best[e >> 1], s[h][0][e] + s[h][1][e]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          best[u] = as_max(best[u], __shfl_xor_sync(0xffffffffu, best[u], 1));
+          best[u] = as_max(best[u], __shfl_xor_sync(0xffffffffu, best[u], 2));
+          const int at = a + i + g + 8 * u;
+          if (t == 0 && at < b) {
+            const unsigned key = ps_order((here >> u) & 1u ? best[u] : -INFINITY);
+            to[at] = n0 > 0 ? max(to[at], key) : key;
+          }
+        }
+      }
+    }
+  }
+  if (threadIdx.x == 0) B200_TRACE(TK_ATTN_OWN, TP_EXIT);
+  B200_TRACE_FLUSH(TK_ATTN_OWN);
+}
+
+// =====================================================================================================================================
+// selection and attention.  Grid (split, KV head x group of up to 16 query heads, row); the splits of a row are a cluster
+// =====================================================================================================================================
+
+// zeros for a row that sees nothing
+template <typename T>
+__device__ __forceinline__ void sparse_nothing(const SparseParams& p, int tok, int kvh, int hg, int h0, int G, int rank) {
+  if (rank != 0) return;
+  T* o = static_cast<T*>(p.out) + static_cast<size_t>(tok) * p.ldo + static_cast<size_t>(h0) * p.c.dv;
+  for (int i = threadIdx.x; i < G * p.c.dv; i += PS_THREADS) o[i] = T(0.f);
+  if (p.chosen && hg == 0)
+    for (int i = threadIdx.x; i < p.top; i += PS_THREADS) p.chosen[(static_cast<size_t>(tok) * p.c.kv_heads + kvh) * p.top + i] = -1;
+}
+
+// ---- any head size, bf16 or fp32 ------------------------------------------------------------------------------------------------------------
+// A head at a time, 16 keys per warp: two lanes per key for the scores, then the lanes along the dimensions of the values.
 template <typename T>
 __global__ void __launch_bounds__(PS_THREADS) attn_sparse_any_kernel(const __grid_constant__ SparseParams p) {
   extern __shared__ __align__(16) uint8_t as_smem[];
@@ -36,104 +212,71 @@ __global__ void __launch_bounds__(PS_THREADS) attn_sparse_any_kernel(const __gri
   const int group = p.hq / p.c.kv_heads, g0 = hg * 16, G = min(16, group - g0), h0 = kvh * group + g0;
   const int dk = p.c.dk, dv = p.c.dv, ps = p.c.page_size;
   SparseRow row;
-  if (!row.find(p, tok)) {                       // the same for all CTAs of the cluster
-    if (rank == 0) {
-      T* o = static_cast<T*>(p.out) + static_cast<size_t>(tok) * p.ldo + static_cast<size_t>(h0) * dv;
-      for (int i = tid; i < G * dv; i += PS_THREADS) o[i] = T(0.f);
-      if (p.chosen && hg == 0)
-        for (int i = tid; i < p.top; i += PS_THREADS) p.chosen[(static_cast<size_t>(tok) * p.c.kv_heads + kvh) * p.top + i] = -1;
-    }
-    return;
-  }
-  const T* q = static_cast<const T*>(p.q) + static_cast<size_t>(tok) * p.ldq;
+  if (!row.find(p, tok)) { sparse_nothing<T>(p, tok, kvh, hg, h0, G, rank); return; }      // the same for all CTAs of the cluster
+  const T* q = static_cast<const T*>(p.q) + static_cast<size_t>(tok) * p.ldq + static_cast<size_t>(h0) * dk;
   const int* pt = p.c.page_table + static_cast<size_t>(row.seq) * p.c.max_pages;
-  // shared memory: scores, list, [8 warps][dv + 2], [16 heads][dv + 2]
-  unsigned* keys = reinterpret_cast<unsigned*>(as_smem);
-  int* list = reinterpret_cast<int*>(keys + p.score_cap);
-  float* part = reinterpret_cast<float*>(list + p.list_cap);
+  // [8 warps][dv + 2], [16 heads][dv + 2], queries [16][dk], scores, list
   const int pitch = dv + 2;
+  float* part = reinterpret_cast<float*>(as_smem);
   float* joined = part + PS_WARPS * pitch;
-
-  const int share = row.lists(p, rank, list, S);          // without a selection the list is known
-  if (row.selects) {
-    const int i0 = ps_share(row.candidates, rank, S), i1 = ps_share(row.candidates, rank + 1, S);
-    for (int i = i0 + warp; i < i1; i += PS_WARPS) {
-      const int page = pt[row.place0 + i];
-      float s = -INFINITY;
-      if (page >= 0 && page < p.c.num_pages) {
-        const T* lo = static_cast<const T*>(p.bounds) + (static_cast<size_t>(page) * p.c.kv_heads + kvh) * 2 * dk;
-        float a[AS_PER_LANE], b[AS_PER_LANE];
-#pragma unroll
-        for (int j = 0; j < AS_PER_LANE; ++j) {
-          const int d = lane + 32 * j;
-          a[j] = d < dk ? as_f(lo[d]) : 0.f;
-          b[j] = d < dk ? as_f(lo[dk + d]) : 0.f;
-        }
-        for (int h = 0; h < group; ++h) {
-          float t = 0.f;
-#pragma unroll
-          for (int j = 0; j < AS_PER_LANE; ++j) {
-            const int d = lane + 32 * j;
-            if (d < dk) {
-              const float x = as_f(q[static_cast<size_t>(kvh * group + h) * dk + d]);
-              t = fmaf(fmaxf(x, 0.f), b[j], fmaf(fminf(x, 0.f), a[j], t));
-            }
-          }
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-          s = as_max(s, t);
-        }
-      }
-      if (lane == 0) keys[i - i0] = ps_order(s);
-    }
-    __syncthreads();
-    select_pages(sel, keys, i1 - i0, i0, row.take, row.first, row.entries, row.place0, list, rank, S);
-  }
-  if (S > 1) cluster_sync_all(); else __syncthreads();
+  float* qs = joined + 16 * pitch;
+  unsigned* room = reinterpret_cast<unsigned*>(qs + 16 * dk);
+  int* list = reinterpret_cast<int*>(room + p.score_cap);
+  for (int i = tid; i < G * dk; i += PS_THREADS) qs[i] = as_f(q[i]);
+  const int share = row.lists(p, sel, room, tok, kvh, rank, S, list);
+  __syncthreads();
   if (p.chosen && hg == 0) row.tell(p, tok, kvh, rank, share, list, S);
 
-  // a head at a time, a page per warp: 32 keys or the page's, then the values with the lanes along their dimensions
   const size_t rec = static_cast<size_t>(p.c.kv_heads) * ps * (dk + dv);
+  const int per = (ps + 15) / 16;                // runs of 16 keys of a page
   for (int g = 0; g < G; ++g) {
-    const T* qh = q + static_cast<size_t>(h0 + g) * dk;
+    const float* qh = qs + g * dk;
     float m = -INFINITY, l = 0.f, acc[AS_PER_LANE];
 #pragma unroll
     for (int j = 0; j < AS_PER_LANE; ++j) acc[j] = 0.f;
-    for (int i = warp; i < share; i += PS_WARPS) {
-      const int place = list[i], page = pt[place];
-      if (page < 0 || page >= p.c.num_pages) continue;
-      const T* kp = static_cast<const T*>(p.c.data) + static_cast<size_t>(page) * rec + static_cast<size_t>(kvh) * ps * dk;
-      const T* vp = static_cast<const T*>(p.c.data) + static_cast<size_t>(page) * rec + static_cast<size_t>(p.c.kv_heads) * ps * dk + static_cast<size_t>(kvh) * ps * dv;
-      const int r0 = max(0, row.low - place * ps), r1 = min(ps, row.pos + 1 - place * ps);
-      for (int k0 = r0; k0 < r1; k0 += 32) {
-        const int n = min(32, r1 - k0);
-        float s = -INFINITY;
-        for (int r = 0; r < n; ++r) {
-          float t = 0.f;
-          for (int d = lane; d < dk; d += 32) t = fmaf(as_f(qh[d]), as_f(kp[static_cast<size_t>(k0 + r) * dk + d]), t);
+    for (int i = warp; i < share * per; i += PS_WARPS) {
+      const int place = list[i / per], page = pt[place];
+      if (page < 0 || page >= p.c.num_pages) {
+        if (lane == 0 && p.status) atomicCAS(p.status, 0, static_cast<int>(ST_BAD_ARGUMENT) | (25 << 8));
+        continue;
+      }
+      const int k0 = i % per * 16, r0 = max(0, row.low - place * ps), r1 = min(ps, row.pos + 1 - place * ps), key = k0 + (lane >> 1);
+      const bool on = key >= r0 && key < r1;
+      const T* kp = static_cast<const T*>(p.c.data) + static_cast<size_t>(page) * rec + (static_cast<size_t>(kvh) * ps + (on ? key : r0)) * dk;
+      const T* vp = static_cast<const T*>(p.c.data) + static_cast<size_t>(page) * rec + static_cast<size_t>(p.c.kv_heads) * ps * dk + (static_cast<size_t>(kvh) * ps + k0) * dv;
+      float t0 = 0.f, t1 = 0.f;
+      const int half = ((dk + 7) / 8) * 4, d0 = (lane & 1) * half, d1 = min(dk, d0 + half);
+      int d = d0;
+#pragma unroll 4
+      for (; d + 4 <= d1; d += 4) {
+        t0 = fmaf(qh[d], as_f(kp[d]), t0); t1 = fmaf(qh[d + 1], as_f(kp[d + 1]), t1);
+        t0 = fmaf(qh[d + 2], as_f(kp[d + 2]), t0); t1 = fmaf(qh[d + 3], as_f(kp[d + 3]), t1);
+      }
+      for (; d < d1; ++d) t0 = fmaf(qh[d], as_f(kp[d]), t0);
+      float s = t0 + t1;
+      s += __shfl_xor_sync(0xffffffffu, s, 1);
+      s = on ? s * p.s.scale : -INFINITY;
+      float mx = s;
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-          if (lane == r) s = t * p.s.scale;
-        }
-        float mx = s;
+      for (int o = 16; o > 1; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      const float mn = fmaxf(m, mx);
+      if (mn == -INFINITY) continue;
+      const float a = m == -INFINITY ? 0.f : expf(m - mn), e = s == -INFINITY ? 0.f : expf(s - mn);
+      float sum = e;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        const float mn = fmaxf(m, mx);
-        if (mn == -INFINITY) continue;
-        const float a = m == -INFINITY ? 0.f : expf(m - mn), e = s == -INFINITY ? 0.f : expf(s - mn);
-        float sum = e;
+      for (int o = 16; o > 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      l = l * a + sum;
+      m = mn;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        l = l * a + sum;
-        m = mn;
+      for (int j = 0; j < AS_PER_LANE; ++j) {
+        if (32 * j >= dv) break;
+        const int x = lane + 32 * j;
+        float v[16], t = 0.f;
 #pragma unroll
-        for (int j = 0; j < AS_PER_LANE; ++j) acc[j] *= a;
-        for (int r = 0; r < n; ++r) {
-          const float w = __shfl_sync(0xffffffffu, e, r);
+        for (int r = 0; r < 16; ++r) v[r] = x < dv && k0 + r >= r0 && k0 + r < r1 ? as_f(vp[static_cast<size_t>(r) * dv + x]) : 0.f;
 #pragma unroll
-          for (int j = 0; j < AS_PER_LANE; ++j)
-            if (lane + 32 * j < dv) acc[j] = fmaf(w, as_f(vp[static_cast<size_t>(k0 + r) * dv + lane + 32 * j]), acc[j]);
-        }
+        for (int r = 0; r < 16; ++r) t = fmaf(__shfl_sync(0xffffffffu, e, 2 * r), v[r], t);
+        acc[j] = fmaf(acc[j], a, t);
       }
     }
     float* mine = part + warp * pitch;
@@ -143,24 +286,18 @@ __global__ void __launch_bounds__(PS_THREADS) attn_sparse_any_kernel(const __gri
       if (lane + 32 * j < dv) mine[lane + 32 * j] = acc[j];
     __syncthreads();
     float* to = joined + g * pitch;
-    float top = -INFINITY, total = 0.f;
+    float top = -INFINITY, f[PS_WARPS];
+#pragma unroll
     for (int w = 0; w < PS_WARPS; ++w) top = fmaxf(top, part[w * pitch + dv]);
-    for (int d = tid; d < dv; d += PS_THREADS) {
+#pragma unroll
+    for (int w = 0; w < PS_WARPS; ++w) f[w] = part[w * pitch + dv] == -INFINITY ? 0.f : expf(part[w * pitch + dv] - top);
+    for (int d = tid; d <= dv; d += PS_THREADS) {            // the last: the sums of the weights
       float v = 0.f;
-      for (int w = 0; w < PS_WARPS; ++w) {
-        const float mw = part[w * pitch + dv];
-        if (mw != -INFINITY) v = fmaf(expf(mw - top), part[w * pitch + d], v);
-      }
-      to[d] = v;
+#pragma unroll
+      for (int w = 0; w < PS_WARPS; ++w) v = fmaf(f[w], part[w * pitch + d + (d == dv)], v);
+      to[d + (d == dv)] = v;
     }
-    if (tid == 0) {
-      for (int w = 0; w < PS_WARPS; ++w) {
-        const float mw = part[w * pitch + dv];
-        if (mw != -INFINITY) total = fmaf(expf(mw - top), part[w * pitch + dv + 1], total);
-      }
-      to[dv] = top;
-      to[dv + 1] = total;
-    }
+    if (tid == 0) to[dv] = top;
     __syncthreads();
   }
   if (S > 1) cluster_sync_all();
@@ -171,11 +308,11 @@ __global__ void __launch_bounds__(PS_THREADS) attn_sparse_any_kernel(const __gri
     float m = p.s.sink ? p.s.sink[h0 + g] : -INFINITY, l = p.s.sink ? 1.f : 0.f, v = 0.f;
     for (int r = 0; r < S; ++r) {
       const uint32_t base = (S > 1 ? mapa_shared(j_addr, r) : j_addr) + 4u * (g * pitch);
-      const float mr = __uint_as_float(ps_ld_cluster(base + 4u * dv));
+      const float mr = dw_ld_cluster(base + 4u * dv);
       if (mr == -INFINITY) continue;
       const float mn = fmaxf(m, mr), fo = m == -INFINITY ? 0.f : expf(m - mn), fn = expf(mr - mn);
-      l = l * fo + fn * __uint_as_float(ps_ld_cluster(base + 4u * (dv + 1)));
-      v = v * fo + fn * __uint_as_float(ps_ld_cluster(base + 4u * d));
+      l = l * fo + fn * dw_ld_cluster(base + 4u * (dv + 1));
+      v = v * fo + fn * dw_ld_cluster(base + 4u * d);
       m = mn;
     }
     float f = l > 0.f ? 1.f / l : 0.f;
@@ -185,232 +322,168 @@ __global__ void __launch_bounds__(PS_THREADS) attn_sparse_any_kernel(const __gri
   if (S > 1) cluster_sync_all();                 // no CTA leaves while a peer may still read its part
 }
 
-// ---- bf16, head sizes up to 128, pages of 16: tensor cores --------------------------------------------------------------------------
-// Eight warps, one CTA per SM.  Scores are products with [lo, hi] of 2 dk numbers, q- against lo and q+ against hi: the same MMAs as for keys, eight
-// pages in the place of eight keys (decode_warp.cuh has the order of the dimensions).  Sums are fp32 and their terms exact.
-constexpr int AST_PITCH_PAD = 4;
+// ---- bf16, head sizes up to 128, pages of 16: tensor cores ------------------------------------------------------------------------------------
+// Eight warps, one CTA per SM, a page per warp and step (decode_warp.cuh).
 template <int DV> struct SparseShape {
-  static constexpr int PITCH = DV + AST_PITCH_PAD, SIZE = 16 * PITCH + 32;
-  static constexpr int FLOATS = (PS_WARPS + 1) * SIZE + 16 * 8;
+  static constexpr int MAX_CLUSTER = 8, PITCH = DV + 4, SIZE = 16 * PITCH + 32;
+  static constexpr int SLICES = 16 * DV + 4 * MAX_CLUSTER, FLOATS = PS_WARPS * SIZE + SLICES + 32 * MAX_CLUSTER;
 };
 
-__device__ __forceinline__ uint32_t as_above(uint32_t x) {      // the larger of each half and zero; NaN stays
-  const __nv_bfloat162 v = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&x), __floats2bfloat162_rn(0.f, 0.f));
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-__device__ __forceinline__ uint32_t as_below(uint32_t x) {
-  const __nv_bfloat162 v = __hmin2_nan(*reinterpret_cast<const __nv_bfloat162*>(&x), __floats2bfloat162_rn(0.f, 0.f));
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-
-// s += q' . bound of eight pages, over one half of the bounds
-template <int DK, bool UP>
-__device__ __forceinline__ void score_half(float (&s)[4], const DwQuery<DK>& q, const uint4 (&b)[DK / 32]) {
-#pragma unroll
-  for (int c = 0; c < DK / 32; ++c) {
-    auto f = [](uint32_t x) { return UP ? as_above(x) : as_below(x); };
-    dw_mma(s, f(q.lo[c].x), f(q.hi[c].x), f(q.lo[c].y), f(q.hi[c].y), b[c].x, b[c].y);
-    dw_mma(s, f(q.lo[c].z), f(q.hi[c].z), f(q.lo[c].w), f(q.hi[c].w), b[c].z, b[c].w);
-  }
-}
-
-template <int DK, int DV, bool FULL>
+template <int DK, int DV, int NH, bool FULL>
 __global__ void __launch_bounds__(PS_THREADS, 1) attn_sparse_kernel(const __grid_constant__ SparseParams p) {
   using Sh = SparseShape<DV>;
   using bf16 = __nv_bfloat16;
   extern __shared__ __align__(16) uint8_t as_smem[];
   __shared__ PageSelectShared sel;
+  B200_TRACE_INIT();
+  if (threadIdx.x == 0) B200_TRACE(TK_ATTN_SPARSE, TP_START);
   pdl_launch_dependents();
-  pdl_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = blockIdx.x, S = p.splits, tok = blockIdx.z;
   const int kvh = blockIdx.y / p.hgroups, hg = blockIdx.y - kvh * p.hgroups;
   const int group = p.hq / p.c.kv_heads, g0 = hg * 16, G = min(16, group - g0), h0 = kvh * group + g0;
   const int dk = FULL ? DK : p.c.dk, dv = FULL ? DV : p.c.dv;
+  // the kernel in front of this one starts it after its own wait: all but the scores is settled
   SparseRow row;
-  if (!row.find(p, tok)) {                       // the same for all CTAs of the cluster
-    if (rank == 0) {
-      bf16* o = static_cast<bf16*>(p.out) + static_cast<size_t>(tok) * p.ldo + static_cast<size_t>(h0) * dv;
-      for (int i = tid; i < G * dv; i += PS_THREADS) o[i] = __float2bfloat16(0.f);
-      if (p.chosen && hg == 0)
-        for (int i = tid; i < p.top; i += PS_THREADS) p.chosen[(static_cast<size_t>(tok) * p.c.kv_heads + kvh) * p.top + i] = -1;
-    }
-    return;
-  }
-  const bf16* q = static_cast<const bf16*>(p.q) + static_cast<size_t>(tok) * p.ldq;
-  const int* pt = p.c.page_table + static_cast<size_t>(row.seq) * p.c.max_pages;
-  float* parts = reinterpret_cast<float*>(as_smem);          // [8 warps], then the CTA's own, then shares [16][8]
-  unsigned* keys = reinterpret_cast<unsigned*>(parts + Sh::FLOATS);
-  int* list = reinterpret_cast<int*>(keys + p.score_cap);
-
-  const int share = row.lists(p, rank, list, S);             // without a selection the list is known
-  DecodeWarp<DK, DV, FULL> w;
-  if (row.selects) {
-    const int i0 = ps_share(row.candidates, rank, S), i1 = ps_share(row.candidates, rank + 1, S);
-    const int a = i0 + static_cast<int>(static_cast<long long>(i1 - i0) * warp / PS_WARPS), b = i0 + static_cast<int>(static_cast<long long>(i1 - i0) * (warp + 1) / PS_WARPS);
-    const int r = lane >> 2, d = (lane & 3) * 8, blocks = (group + 15) / 16;
-    if (blocks == 1) w.q.load(q + static_cast<size_t>(kvh) * group * dk, group, dk);
-    uint4 lo[DK / 32], hi[DK / 32];
-    int ids = 0, ids_from = a - 32;
-    auto request = [&](int i) {                  // bounds of pages i .. i + 7: a lane has part of page i + r
-      if (i >= ids_from + 32) {
-        ids_from = i;
-        ids = i + lane < b ? pt[row.place0 + i + lane] : -1;
-      }
-      const int page = __shfl_sync(0xffffffffu, ids, i - ids_from + r);
-      const bool on = page >= 0 && page < p.c.num_pages;
-      const bf16* x = static_cast<const bf16*>(p.bounds) + (static_cast<size_t>(on ? page : 0) * p.c.kv_heads + kvh) * 2 * dk;
-#pragma unroll
-      for (int c = 0; c < DK / 32; ++c) {
-        const bool in = on && (FULL || c * 32 + d < dk);
-        lo[c] = dw_load(x + c * 32 + d, in);
-        hi[c] = dw_load(x + dk + c * 32 + d, in);
-      }
-      return on;
-    };
-    if (a < b) {
-      bool on = request(a);
-      for (int i = a; i < b; i += 8) {
-        float best[2] = {-INFINITY, -INFINITY};
-        uint4 l8[DK / 32], h8[DK / 32];
-#pragma unroll
-        for (int c = 0; c < DK / 32; ++c) { l8[c] = lo[c]; h8[c] = hi[c]; }
-        const unsigned there = __ballot_sync(0xffffffffu, on);
-        if (i + 8 < b) on = request(i + 8);
-        for (int k = 0; k < blocks; ++k) {
-          const int n = min(16, group - 16 * k);
-          if (blocks > 1) w.q.load(q + (static_cast<size_t>(kvh) * group + 16 * k) * dk, n, dk);
-          float s[4] = {0.f, 0.f, 0.f, 0.f};
-          score_half<DK, false>(s, w.q, l8);
-          score_half<DK, true>(s, w.q, h8);
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            if (r < n) best[e] = as_max(best[e], s[e]);
-            if (r + 8 < n) best[e] = as_max(best[e], s[2 + e]);
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          best[e] = as_max(best[e], __shfl_xor_sync(0xffffffffu, best[e], 4));
-          best[e] = as_max(best[e], __shfl_xor_sync(0xffffffffu, best[e], 8));
-          best[e] = as_max(best[e], __shfl_xor_sync(0xffffffffu, best[e], 16));
-          const int page = 2 * (lane & 3) + e;   // of the eight
-          if (r == 0 && i + page < b) keys[i + page - i0] = ps_order((there >> (4 * page)) & 1u ? best[e] : -INFINITY);
-        }
-      }
-    }
-    __syncthreads();
-    select_pages(sel, keys, i1 - i0, i0, row.take, row.first, row.entries, row.place0, list, rank, S);
-  }
+  const bool any = row.find(p, tok);
+  const bf16* q = static_cast<const bf16*>(p.q) + static_cast<size_t>(tok) * p.ldq + static_cast<size_t>(h0) * dk;
+  DecodeWarp<DK, DV, NH, FULL> w;
   w.begin(dk, dv, p.s.scale);
-  w.q.load(q + static_cast<size_t>(h0) * dk, G, dk);
-  if (S > 1) cluster_sync_all(); else __syncthreads();
+  w.q.load(q, any ? G : 0, dk);
+  pdl_wait();
+  if (tid == 0) B200_TRACE(TK_ATTN_SPARSE, TP_DEPS);
+  if (!any) { sparse_nothing<bf16>(p, tok, kvh, hg, h0, G, rank); return; }      // the same for all CTAs of the cluster
+  const int* pt = p.c.page_table + static_cast<size_t>(row.seq) * p.c.max_pages;
+  // [8 warps], slices of every CTA's O for this one to join, (m, l) of every CTA [8][2][16], scores, list
+  float* parts = reinterpret_cast<float*>(as_smem);
+  float* slices = parts + PS_WARPS * Sh::SIZE;
+  float* ml = slices + Sh::SLICES;
+  unsigned* room = reinterpret_cast<unsigned*>(parts + Sh::FLOATS);
+  int* list = reinterpret_cast<int*>(room + p.score_cap);
+  const int share = row.lists(p, sel, room, tok, kvh, rank, S, list);
+  __syncthreads();
+  if (S > 1) cluster_arrive_relaxed();           // all CTAs have started when theirs is waited for, in front of the first access
+  if (tid == 0) B200_TRACE(TK_ATTN_SPARSE, 3);               // lists
   if (p.chosen && hg == 0) row.tell(p, tok, kvh, rank, share, list, S);
 
   const size_t rec = static_cast<size_t>(p.c.kv_heads) * 16 * (dk + dv);
   const bf16* kbase = static_cast<const bf16*>(p.c.data) + static_cast<size_t>(kvh) * 16 * dk;
   const bf16* vbase = static_cast<const bf16*>(p.c.data) + static_cast<size_t>(p.c.kv_heads) * 16 * dk + static_cast<size_t>(kvh) * 16 * dv;
   // the places and pages of this warp's next 32 entries are in its lanes
-  int ids = 0, places = 0, ids_from = -32, place = 0, page = -1;
+  int ids = 0, places = 0, ids_from = -32;
   const int mine = share > warp ? (share - warp + PS_WARPS - 1) / PS_WARPS : 0;
-  auto next = [&](int i) {
+  w.template walk<false>(mine, [&](int i) {
     if (i >= ids_from + 32) {
       ids_from = i;
       places = i + lane < mine ? list[warp + (i + lane) * PS_WARPS] : 0;
       ids = i + lane < mine ? pt[places] : -1;
     }
-    place = __shfl_sync(0xffffffffu, places, i - ids_from);
-    page = __shfl_sync(0xffffffffu, ids, i - ids_from);
-    if (page >= p.c.num_pages) page = -1;
-  };
-  if (mine > 0) {
-    next(0);
-    int lo = max(0, row.low - place * 16), hi = min(16, row.pos + 1 - place * 16);
-    w.load_k(kbase + (page >= 0 ? page * rec : 0), page >= 0);
-    w.load_v(vbase + (page >= 0 ? page * rec : 0), lo, page >= 0 ? hi : 0);
-    for (int i = 0; i < mine; ++i) {
-      float s[2][4];
-      w.scores(s);
-      const int here = page, lo_here = lo, hi_here = hi;
-      if (i + 1 < mine) {
-        next(i + 1);
-        lo = max(0, row.low - place * 16);
-        hi = min(16, row.pos + 1 - place * 16);
-        w.load_k(kbase + (page >= 0 ? page * rec : 0), page >= 0);
-      }
-      if (here >= 0) {
-        uint32_t pr[4];
-        w.weigh(s, lo_here, hi_here, pr);
-        w.add(pr);
-      } else if (lane == 0 && p.status) {
-        atomicCAS(p.status, 0, static_cast<int>(ST_BAD_ARGUMENT) | (25 << 8));
-      }
-      if (i + 1 < mine) w.load_v(vbase + (page >= 0 ? page * rec : 0), lo, page >= 0 ? hi : 0);
-    }
-  }
-  w.end();
+    const int place = __shfl_sync(0xffffffffu, places, i - ids_from), page = __shfl_sync(0xffffffffu, ids, i - ids_from);
+    const bool there = page >= 0 && page < p.c.num_pages;
+    if (!there && lane == 0 && p.status) atomicCAS(p.status, 0, static_cast<int>(ST_BAD_ARGUMENT) | (25 << 8));
+    const size_t at = there ? page * rec : 0;
+    return DwPage{kbase + at, vbase + at, max(0, row.low - place * 16), there ? min(16, row.pos + 1 - place * 16) : 0};
+  }, [] {});
   w.put(parts + warp * Sh::SIZE, Sh::PITCH, G);
   __syncthreads();
-  float* own = parts + PS_WARPS * Sh::SIZE;
-  float* shares = own + Sh::SIZE;
-  dw_join<PS_WARPS, PS_THREADS>(parts, Sh::SIZE, Sh::PITCH, G, dv, own);
-  if (S > 1) cluster_sync_all(); else __syncthreads();
-  const uint32_t own_addr = smem_u32(own);
-  if (tid < 16 * 8) {                            // eight lanes per row, a CTA of the cluster each
-    const int g = tid >> 3, i = tid & 7;
+  if (tid == 0) B200_TRACE(TK_ATTN_SPARSE, 4);               // attention
+  if (S > 1) cluster_wait_acquire();
+  // The CTA's sums go to the CTAs that join them: every one has a slice of the output's quads of dimensions.
+  const int quads = dv >> 2, total = G * quads, slice = (total + S - 1) / S;
+  for (int i = tid; i < total; i += PS_THREADS) {
+    const int g = i / quads, d = (i - g * quads) * 4;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     float m = -INFINITY, l = 0.f;
-    if (g < G && i < S) {
-      const uint32_t base = S > 1 ? mapa_shared(own_addr, i) : own_addr;
-      m = dw_ld_cluster(base + 4u * (16 * Sh::PITCH + g));
-      l = dw_ld_cluster(base + 4u * (16 * Sh::PITCH + 16 + g));
+#pragma unroll 4
+    for (int k = 0; k < PS_WARPS; ++k) m = fmaxf(m, parts[k * Sh::SIZE + 16 * Sh::PITCH + g]);
+    const float use = m == -INFINITY ? 0.f : m;
+#pragma unroll 4
+    for (int k = 0; k < PS_WARPS; ++k) {         // a warp without pages has left zeros
+      const float* x = parts + k * Sh::SIZE;
+      const float f = dw_exp2(x[16 * Sh::PITCH + g] - use);
+      const float4 y = *reinterpret_cast<const float4*>(x + g * Sh::PITCH + d);
+      v.x += f * y.x; v.y += f * y.y; v.z += f * y.z; v.w += f * y.w;
+      l += f * x[16 * Sh::PITCH + 16 + g];
     }
-    const float sink2 = p.s.sink && g < G ? p.s.sink[h0 + g] * DW_LOG2E : -INFINITY;
-    float top = fmaxf(m, sink2);
-#pragma unroll
-    for (int o = 1; o < 8; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float use = top == -INFINITY ? 0.f : top, f0 = m == -INFINITY ? 0.f : dw_exp2(m - use);
-    float total = f0 * l;
-#pragma unroll
-    for (int o = 1; o < 8; o *= 2) total += __shfl_xor_sync(0xffffffffu, total, o);
-    if (p.s.sink) total += dw_exp2(sink2 - use);
-    float f = total > 0.f ? 1.f / total : 0.f;
-    if (p.s.gate && g < G) f *= 1.f / (1.f + __expf(-__bfloat162float(static_cast<const bf16*>(p.s.gate)[static_cast<size_t>(tok) * p.s.ldg + h0 + g])));
-    shares[tid] = f0 * f;
+    const int r = static_cast<int>(((static_cast<long long>(i) + 1) * S - 1) / total);       // whose slice has it
+    const uint32_t to = smem_u32(slices + 4 * (rank * slice + i - ps_share(total, r, S)));
+    st_shared_cluster_v4(S > 1 ? mapa_shared(to, r) : to, __float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w));
+    // the threads of a head's quads tell the CTAs its (m, l)
+#pragma unroll 1
+    for (int k = i - g * quads; k < S; k += quads) {
+      const uint32_t at = smem_u32(ml + 32 * rank + g);
+      st_shared_cluster_u32(S > 1 ? mapa_shared(at, k) : at, __float_as_uint(m));
+      st_shared_cluster_u32((S > 1 ? mapa_shared(at, k) : at) + 64, __float_as_uint(l));
+    }
   }
-  __syncthreads();
+  if (S > 1) cluster_sync_all(); else __syncthreads();       // nothing of another CTA is touched behind this
+  const int x0 = ps_share(total, rank, S), x1 = ps_share(total, rank + 1, S);
   bf16* out = static_cast<bf16*>(p.out) + static_cast<size_t>(tok) * p.ldo + static_cast<size_t>(h0) * dv;
-  for (int i = rank * PS_THREADS + tid; i < G * dv; i += S * PS_THREADS) {
-    const int g = i / dv, x = i - g * dv;
-    float v = 0.f;
+  for (int i = x0 + tid; i < x1; i += PS_THREADS) {
+    const int g = i / quads, d = (i - g * quads) * 4;
+    const float sink2 = p.s.sink ? p.s.sink[h0 + g] * DW_LOG2E : -INFINITY;
+    float m = sink2;
+#pragma unroll 4
+    for (int r = 0; r < S; ++r) m = fmaxf(m, ml[32 * r + g]);
+    const float use = m == -INFINITY ? 0.f : m;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = dw_exp2(sink2 - use);
+#pragma unroll 4
     for (int r = 0; r < S; ++r) {
-      const float f = shares[g * 8 + r];
-      if (f != 0.f) v += f * dw_ld_cluster((S > 1 ? mapa_shared(own_addr, r) : own_addr) + 4u * (g * Sh::PITCH + x));
+      const float f = dw_exp2(ml[32 * r + g] - use);
+      const float4 y = *reinterpret_cast<const float4*>(slices + 4 * (r * slice + i - x0));
+      v.x += f * y.x; v.y += f * y.y; v.z += f * y.z; v.w += f * y.w;
+      l += f * ml[32 * r + 16 + g];
     }
-    out[i] = __float2bfloat16(v);
+    float f = l > 0.f ? 1.f / l : 0.f;
+    if (p.s.gate) f *= 1.f / (1.f + __expf(-__bfloat162float(static_cast<const bf16*>(p.s.gate)[static_cast<size_t>(tok) * p.s.ldg + h0 + g])));
+    *reinterpret_cast<uint2*>(out + g * dv + d) = make_uint2(dw_pack(v.x * f, v.y * f), dw_pack(v.z * f, v.w * f));
   }
-  if (S > 1) cluster_sync_all();                 // no CTA leaves while a peer may still read its part
+  if (tid == 0) B200_TRACE(TK_ATTN_SPARSE, TP_EXIT);
+  B200_TRACE_FLUSH(TK_ATTN_SPARSE);
 }
 
-template <int DK, int DV, bool FULL>
-static int launch_sparse(const SparseParams& p, cudaStream_t stream) {
-  const size_t smem = 4 * (static_cast<size_t>(SparseShape<DV>::FLOATS) + p.score_cap + p.list_cap);
-  if (smem > SPARSE_MAX_SMEM) return -5;
-  cudaError_t e = cudaFuncSetAttribute(attn_sparse_kernel<DK, DV, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SPARSE_MAX_SMEM));
+// ---- launches ---------------------------------------------------------------------------------------------------------------------------------
+template <typename K>
+static int launch_sparse_pair(K scores, dim3 grid1, size_t smem1, K attend, size_t smem2, const SparseParams& p, cudaStream_t stream) {
+  if (smem1 > SPARSE_MAX_SMEM || smem2 > SPARSE_MAX_SMEM) return -5;
+  cudaError_t e = cudaSuccess;
+  if (smem1 > (48u << 10)) e = cudaFuncSetAttribute(scores, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SPARSE_MAX_SMEM));
+  if (e == cudaSuccess && smem2 > (40u << 10)) e = cudaFuncSetAttribute(attend, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SPARSE_MAX_SMEM));
   if (e != cudaSuccess) return -1000 - static_cast<int>(e);
-  launch_ex(attn_sparse_kernel<DK, DV, FULL>, dim3(p.splits, p.c.kv_heads * p.hgroups, p.M), dim3(PS_THREADS), smem, stream, p.splits, p);
+  launch_ex(scores, grid1, dim3(SC_THREADS), smem1, stream, 0, p);
+  launch_ex(attend, dim3(p.splits, p.c.kv_heads * p.hgroups, p.M), dim3(PS_THREADS), smem2, stream, p.splits, p);
   e = cudaGetLastError();
   return e == cudaSuccess ? 0 : -2000 - static_cast<int>(e);
+}
+
+// scores stay in shared memory up to what a CTA has left; more are looked at where the first kernel left them
+static void fit_scores(SparseParams& p, size_t floats) {
+  const size_t used = 4 * (floats + p.list_cap + p.score_cap);
+  const size_t room = used < SPARSE_MAX_SMEM ? (SPARSE_MAX_SMEM - used) / 4 : 0, most = (static_cast<size_t>(p.c.max_pages) + 3) & ~size_t(3);
+  p.score_cap = static_cast<int>(most < room ? most : room & ~size_t(3));
 }
 
 template <typename T>
-static int launch_sparse_any(const SparseParams& p, cudaStream_t stream) {
-  const size_t smem = 4 * (static_cast<size_t>(p.score_cap) + p.list_cap + static_cast<size_t>(PS_WARPS + 16) * (p.c.dv + 2));
-  if (smem > SPARSE_MAX_SMEM) return -5;
-  cudaError_t e = cudaFuncSetAttribute(attn_sparse_any_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SPARSE_MAX_SMEM));
-  if (e != cudaSuccess) return -1000 - static_cast<int>(e);
-  launch_ex(attn_sparse_any_kernel<T>, dim3(p.splits, p.c.kv_heads * p.hgroups, p.M), dim3(PS_THREADS), smem, stream, p.splits, p);
-  e = cudaGetLastError();
-  return e == cudaSuccess ? 0 : -2000 - static_cast<int>(e);
+static int launch_sparse_any(SparseParams p, cudaStream_t stream) {
+  const size_t floats = static_cast<size_t>(PS_WARPS + 16) * (p.c.dv + 2) + 16 * static_cast<size_t>(p.c.dk);
+  fit_scores(p, floats);
+  const dim3 grid((p.c.max_pages + SCA_PAGES - 1) / SCA_PAGES, p.c.kv_heads, p.M);
+  return launch_sparse_pair(page_scores_any_kernel<T>, grid, 4 * static_cast<size_t>(p.hq / p.c.kv_heads) * p.c.dk, attn_sparse_any_kernel<T>,
+                            4 * (floats + p.list_cap + p.score_cap), p, stream);
+}
+
+template <int DK, int DV, int NH, bool FULL>
+static int launch_sparse(SparseParams p, cudaStream_t stream) {
+  fit_scores(p, SparseShape<DV>::FLOATS);
+  const dim3 grid((p.c.max_pages + SC_PAGES - 1) / SC_PAGES, p.c.kv_heads, p.M);
+  return launch_sparse_pair(page_scores_kernel<DK, NH, FULL>, grid, 0, attn_sparse_kernel<DK, DV, NH, FULL>,
+                            4 * (static_cast<size_t>(SparseShape<DV>::FLOATS) + p.score_cap + p.list_cap), p, stream);
+}
+
+template <int DK, int DV, bool FULL>
+static int launch_sparse_heads(const SparseParams& p, cudaStream_t stream) {
+  return p.hq / p.c.kv_heads <= 8 ? launch_sparse<DK, DV, 1, FULL>(p, stream) : launch_sparse<DK, DV, 2, FULL>(p, stream);
 }
 
 }  // namespace b200
@@ -419,25 +492,25 @@ using namespace b200;
 
 extern "C" int b200_attn_paged_sparse(const void* q, long long ldq, void* out, long long ldo, int hq, int M, const int* positions, const int* seq_ids,
                                       const int* seq_lens, const b200_paged_cache* c, const void* bounds, const b200_attn_spec* s, int top, int first,
-                                      int last, int splits, int* chosen, int* status, cudaStream_t stream) {
+                                      int last, int splits, unsigned* scores, int* chosen, int* status, cudaStream_t stream) {
   if (M <= 0) return 0;
-  if (!q || !out || !positions || !c || !c->data || !c->page_table || !bounds || !s) return -1;
+  if (!q || !out || !positions || !c || !c->data || !c->page_table || !bounds || !s || !scores) return -1;
   if (hq <= 0 || c->kv_heads <= 0 || hq % c->kv_heads || c->page_size <= 0 || c->dk <= 0 || c->dv <= 0 || c->dk > AS_MAX_D || c->dv > AS_MAX_D ||
       c->num_pages <= 0) return -2;
   if (first < 0 || last < 1 || top < first + last || splits < 1 || splits > 8 || M > 65535 || !(s->scale > 0.f)) return -3;
   SparseParams p = {};
   p.q = q; p.ldq = ldq; p.out = out; p.ldo = ldo; p.hq = hq; p.M = M; p.hgroups = (hq / c->kv_heads + 15) / 16;
-  p.positions = positions; p.seq_ids = seq_ids; p.seq_lens = seq_lens; p.c = *c; p.s = *s; p.bounds = bounds;
+  p.positions = positions; p.seq_ids = seq_ids; p.seq_lens = seq_lens; p.c = *c; p.s = *s; p.bounds = bounds; p.scores = scores;
   p.top = top; p.first = first; p.last = last; p.splits = splits; p.chosen = chosen; p.status = status;
-  p.score_cap = (((c->max_pages + splits - 1) / splits + 1) + 3) & ~3;
   p.list_cap = (((top < c->max_pages ? top : c->max_pages) + splits - 1) / splits + 1 + 3) & ~3;
   if (static_cast<long long>(c->kv_heads) * p.hgroups > 65535) return -3;
   if (c->f32) return launch_sparse_any<float>(p, stream);
-  if (c->page_size != 16 || c->dk > 128 || c->dv > 128 || c->dk % 8 || c->dv % 8 || ldq % 8 || (reinterpret_cast<uintptr_t>(q) & 15) ||
-      (reinterpret_cast<uintptr_t>(c->data) & 15) || (reinterpret_cast<uintptr_t>(bounds) & 15)) return launch_sparse_any<__nv_bfloat16>(p, stream);
+  if (c->page_size != 16 || c->dk > 128 || c->dv > 128 || c->dk % 8 || c->dv % 8 || ldq % 8 || ldo % 4 || (reinterpret_cast<uintptr_t>(q) & 15) ||
+      (reinterpret_cast<uintptr_t>(out) & 7) || (reinterpret_cast<uintptr_t>(c->data) & 15) || (reinterpret_cast<uintptr_t>(bounds) & 15))
+    return launch_sparse_any<__nv_bfloat16>(p, stream);
   const int d = c->dk > c->dv ? c->dk : c->dv;
-  if (c->dk == 64 && c->dv == 64) return launch_sparse<64, 64, true>(p, stream);
-  if (c->dk == 128 && c->dv == 128) return launch_sparse<128, 128, true>(p, stream);
-  if (d <= 64) return launch_sparse<64, 64, false>(p, stream);
-  return launch_sparse<128, 128, false>(p, stream);
+  if (c->dk == 64 && c->dv == 64) return launch_sparse_heads<64, 64, true>(p, stream);
+  if (c->dk == 128 && c->dv == 128) return launch_sparse_heads<128, 128, true>(p, stream);
+  if (d <= 64) return launch_sparse_heads<64, 64, false>(p, stream);
+  return launch_sparse_heads<128, 128, false>(p, stream);
 }

@@ -16,8 +16,9 @@ struct SparseParams {
   b200_paged_cache c;
   b200_attn_spec s;
   const void* bounds;                    // [pages][kv_heads][2][dk]
+  unsigned* scores;                      // [M][kv_heads][max_pages], candidates' in their order
   int top, first, last;
-  int splits, score_cap, list_cap;       // numbers that a CTA has room for
+  int splits, list_cap, score_cap;       // entries and scores that a CTA has room for
   int* chosen;                           // [M][kv_heads][top] or NULL
   int* status;
 };
@@ -42,20 +43,31 @@ struct SparseRow {
     page0 = low / p.c.page_size;
     pages = pos / p.c.page_size - page0 + 1;
     entries = min(pages, p.top);
-    selects = pages > p.top;
     first = p.first;
     take = p.top - p.first - p.last;
+    selects = pages > p.top && take > 0;
     candidates = pages - p.first - p.last;
     place0 = page0 + p.first;
-    if (take == 0) selects = false;
     return true;
   }
-  // The entries of the lists that need no score: all of them, or the first and the last.  How many entries this CTA reads.
-  __device__ __forceinline__ int lists(const SparseParams& p, int rank, int* list, int S) const {
+  // The entries of this CTA's list: those that need no score (all of them, or the first and the last), and those that do.  All threads; the list is
+  // complete behind the next barrier.
+  __device__ __forceinline__ int lists(const SparseParams& p, PageSelectShared& sel, unsigned* room, int tok, int kvh, int rank, int S, int* list) const {
     const int a = ps_share(entries, rank, S), b = ps_share(entries, rank + 1, S);
     for (int x = a + threadIdx.x; x < b; x += PS_THREADS) {
       if (pages == entries || x < first) list[x - a] = page0 + x;
       else if (x >= entries - p.last) list[x - a] = page0 + pages - (entries - x);
+    }
+    if (selects && a < entries - p.last && b > first) {
+      const unsigned* keys = p.scores + (static_cast<size_t>(tok) * p.c.kv_heads + kvh) * p.c.max_pages;
+      unsigned lo = 0xffffffffu, hi = 0u;
+      const bool near = candidates <= p.score_cap;
+      ps_each(keys, candidates, [&](int i, unsigned k) {
+        lo = min(lo, k);
+        hi = max(hi, k);
+        if (near) room[i] = k;
+      });
+      select_pages(sel, near ? room : keys, candidates, lo, hi, take, first, place0, list, a, b - a);
     }
     return b - a;
   }

@@ -17,7 +17,7 @@ namespace b200 {
 
 enum TraceKernel : unsigned {
   TK_ACT_QUANT = 1, TK_GEMM_DECODE = 2, TK_GEMM_PREFILL = 3, TK_ROPE_KV = 4, TK_ATTN_DECODE = 5, TK_ATTN_PREFILL = 6,
-  TK_PEER_ALLREDUCE = 7, TK_GEMM_TP = 8, TK_MOE = 9, TK_ARGMAX = 10,
+  TK_PEER_ALLREDUCE = 7, TK_GEMM_TP = 8, TK_MOE = 9, TK_ARGMAX = 10, TK_ATTN_SHARED = 11, TK_ATTN_OWN = 12, TK_ATTN_SPARSE = 13,
 };
 // phases are free-form per kernel; by convention 0 = CTA started, 1 = dependency wait passed, 63 = CTA about to exit
 enum TracePhase : unsigned { TP_START = 0, TP_DEPS = 1, TP_EXIT = 63 };

@@ -11,14 +11,13 @@ from .pages import check_bounds
 from .workspace import default_workspace
 
 MAX_HEAD_DIM = 512
-SCORES_PER_CTA = 24 << 10      # pages whose scores a CTA has room for
 
 
-def pick_sparse_splits(pairs: int, max_pages: int, num_sms: int = 148) -> int:
-    """CTAs (one cluster) per row and KV head: as many as still make one wave of two per SM, with 16 pages each at least, and as many as the
-    scores of a sequence of ``max_pages`` need."""
+def pick_sparse_splits(pairs: int, pages: int, num_sms: int = 148) -> int:
+    """CTAs (one cluster of up to eight) per row and group of heads, which share ``pages`` pages: as many as still make one wave of one per SM, with 16
+    pages, two for a warp, each."""
     s = 1
-    while s < 8 and ((pairs * s * 2 <= 2 * num_sms and max_pages // (2 * s) >= 16) or max_pages > s * SCORES_PER_CTA):
+    while s < 8 and pairs * s * 2 <= num_sms and pages // (2 * s) >= 16:
         s *= 2
     return s
 
@@ -52,11 +51,13 @@ def attn_paged_sparse(q: torch.Tensor, hq: int, positions: torch.Tensor, seq_ids
     most = page_table.shape[1]
     if splits is None:
         seen = min(most, spec.chunk // cache.page_size + 2) if spec.chunk > 0 else most
-        splits = pick_sparse_splits(M * cache.kv_heads * ((hq // cache.kv_heads + 15) // 16), seen, _lib.num_sms(q.device.index))
+        splits = pick_sparse_splits(M * cache.kv_heads * ((hq // cache.kv_heads + 15) // 16), min(top, seen), _lib.num_sms(q.device.index))
+    scores = torch.empty(M * cache.kv_heads * most, dtype=torch.int32, device=q.device)
     with torch.cuda.device(q.device):
         rc = _lib.lib().b200_attn_paged_sparse(
             q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), hq, M, positions.data_ptr(), _lib.ptr(seq_ids), _lib.ptr(seq_lens),
-            ctypes.byref(cache.desc(page_table)), bounds.data_ptr(), ctypes.byref(spec), int(top), int(first), int(last), splits, _lib.ptr(chosen),
-            default_workspace(q.device).status.data_ptr(), _lib.stream())
+            ctypes.byref(cache.desc(page_table)), bounds.data_ptr(), ctypes.byref(spec), int(top), int(first), int(last), splits, scores.data_ptr(),
+            _lib.ptr(chosen), default_workspace(q.device).status.data_ptr(), _lib.stream())
     _lib.check(rc, "attn_paged_sparse")
+    _lib.LAUNCHES[0] += 1                        # two kernels
     return out

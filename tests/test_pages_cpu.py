@@ -56,7 +56,7 @@ def test_groups_that_make_no_sense_are_refused(groups):
         SH.SharedPrefixes(4, "cpu").set(groups)
 
 
-@pytest.mark.parametrize("pairs,pages,want", [(8, 8192, 8), (64, 1000, 4), (512, 8192, 1), (512, 60000, 4), (2, 20, 1), (1, 40, 2)])
+@pytest.mark.parametrize("pairs,pages,want", [(8, 128, 8), (64, 64, 2), (512, 256, 1), (20, 100, 4), (2, 31, 1), (1, 32, 2)])
 def test_clusters_for_selections(pairs, pages, want):
     assert SP.pick_sparse_splits(pairs, pages) == want
 

@@ -197,3 +197,29 @@ def test_a_captured_call_follows_its_positions():
         SP.attn_paged_sparse(q, 8, pos, None, S.cache, S.table, bounds, spec, other, top=6)
         assert torch.equal(out, other)
     status_ok()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_more_pages_than_a_selection_holds_at_once(dtype):
+    """20,000 and 9,000 pages: whole numbers with many equal scores, whose order is known."""
+    from mojo_linuxperiments_b200.ops import attention as A
+    from mojo_linuxperiments_b200.ops import sparse as SP
+    g = torch.Generator(device=DEV).manual_seed(3)
+    n = [20000, 9000]
+    cache = A.PagedKVCache(64, 1, 16, DEV, dk=16, dv=16, dtype=torch.float32 if dtype == "float32" else torch.bfloat16)
+    cache.data.normal_(generator=g)
+    table = torch.randint(0, 64, (2, n[0]), generator=g, device=DEV, dtype=torch.int32)            # pages seen many times over
+    bounds = torch.randint(-2, 3, (64, 1, 2, 16), generator=g, device=DEV).sort(2).values.to(cache.data.dtype)
+    q = torch.randint(-1, 2, (2, 32), generator=g, device=DEV).to(cache.data.dtype)
+    pos = torch.tensor([16 * k - 3 for k in n], dtype=torch.int32, device=DEV)
+    for top in (100, 1500, 3):
+        chosen, out = torch.empty((2, 1, top), dtype=torch.int32, device=DEV), torch.empty((2, 32), dtype=cache.data.dtype, device=DEV)
+        SP.attn_paged_sparse(q, 2, pos, None, cache, table, bounds, A.attn_spec(0.1), out, top=top, chosen=chosen)
+        status_ok()
+        for i, k in enumerate(n):
+            x = q[i].double().view(2, 1, 16)
+            b = bounds[:, 0].double()
+            score = torch.maximum(x * b[:, 0], x * b[:, 1]).sum(-1).amax(0)[table[i, :k].long()]
+            score[0], score[k - 2:] = 1e9, 1e9
+            want = torch.sort(score, descending=True, stable=True).indices[:top].sort().values
+            assert torch.equal(chosen[i, 0].long(), want), (top, i)
