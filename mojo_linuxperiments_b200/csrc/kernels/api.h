@@ -352,7 +352,7 @@ int b200_attn_paged_sparse(const void* q, long long ldq, void* out, long long ld
 // per slot and KV head for the slot's own keys.
 int b200_attn_decode_shared_takes(const b200_paged_cache* cache, int hq, long long ldq, long long ldo);
 int b200_attn_decode_shared(const void* q, long long ldq, void* out, long long ldo, int hq, int B, const int* seq_lens, const b200_paged_cache* cache,
-                            const b200_attn_spec* spec, const int* plan, int pieces_at, int slots_at, int max_pieces, float* part, int part_rows,
+                            const b200_attn_spec* spec, int* plan, int pieces_at, int slots_at, int max_pieces, float* part, int part_rows,
                             int splits, int num_sms, int* status, cudaStream_t stream);
 // Smallest and largest element per dimension over the keys of a page that a sequence has, for the pages of tokens starts[i] .. ends[i] of every
 // portion (at most max_tokens of them; seq_ids NULL: portion i is of sequence i).

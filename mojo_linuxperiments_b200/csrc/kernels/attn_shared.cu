@@ -4,7 +4,7 @@
 //   m = max(m_1, m_2), l = sum l_i exp(m_i - m), O = sum O_i exp(m_i - m).
 //
 // Two launches.  The first takes the prefixes: the rows (member x query head) of a group are the M of tcgen05 MMAs over tiles of 128 keys, in pieces of
-// 128 rows and of some tiles, which leave (m, l, O) in fp32.  Which pieces there are is a list on the device, made when groups change, so that a captured call
+// up to 256 rows and of some tiles, which leave (m, l, O) in fp32.  Which pieces there are is a list on the device, made when groups change, so that a captured call
 // follows them.  The second takes each sequence's own keys (decode_warp.cuh) while the first still runs, joins the pieces of the prefix, adds sink
 // and gate and writes the output; it waits for the first only there.
 #include "ptx.cuh"
@@ -16,18 +16,22 @@
 namespace b200 {
 
 // ---- the plan: int32 on the device -------------------------------------------------------------------------------------------------
-// [0] pieces, then at SP_INFO four numbers per slot: first row of its partial results, rows between the parts of the prefix, parts, tokens;
+// [0] pieces; [4] pieces of this call that are done, [5] CTAs of the second kernel that have seen it (both zero between calls); at SP_INFO four numbers per slot: first row of its partial results, rows between the parts of the prefix, parts, tokens;
 // then the pieces, eight numbers each; then the slots of the groups' members.
-constexpr int SP_INFO = 16, SP_PIECE = 8;
-struct SharedPiece { int member0, members, row0, rows, key0, key1, part, unused; };   // members: place in the list of slots, number of them in the group; rows within the group
+constexpr int SP_DONE = 4, SP_SEEN = 5, SP_INFO = 16, SP_PIECE = 8;
+// member0: of the group, in the list of slots; rows row0 .. row0 + rows of the group (member x query head); keys key0 .. key1; part: first row of the partial
+// results of the group's rows for this run of keys; lead: slot whose pages are read; mode: what the two units of a CTA do, and above it the group's rows
+struct SharedPiece { int member0, row0, rows, key0, key1, part, lead, mode, group_rows; };
+// two tiles of 128 rows; the same 128 rows and every other tile of keys, whose results are the next part; one unit
+enum SharedMode : int { SM_ROWS = 0, SM_KEYS = 1, SM_ONE = 2 };
 
 struct SharedParams {
   const __nv_bfloat16* q; long long ldq;
   __nv_bfloat16* out; long long ldo;
   int hq, B;
   const int* seq_lens;
-  const int* plan; int pieces_at, slots_at, max_pieces;
-  float* part; int part_rows;            // [kv_heads][part_rows][dv], then (m, l) [kv_heads][part_rows][2]
+  int* plan; int pieces_at, slots_at, max_pieces;
+  float* part; int part_rows;            // [kv_heads][dv / 4][part_rows][4], then (m, l) [kv_heads][part_rows][2]
   b200_paged_cache c;
   int chunk;
   float scale;
@@ -38,72 +42,93 @@ struct SharedParams {
   unsigned long long limit_ns;
 };
 
-// ---- prefixes -----------------------------------------------------------------------------------------------------------------------
-// One piece at a time per CTA, two CTAs per SM, which fill each other's gaps: warp 0 fetches pages by TMA (lane <-> page), warp 1 issues the MMAs, warps
-// 4..7 gather the queries, take the softmax (thread <-> row) and keep O in tensor memory.  One tile of keys and one of values in shared memory: the next
-// keys are requested once the scores are there, the next values once they are used.
-constexpr int SX_THREADS = 256, SX_BN = 128, SX_PS = 16;
-// registers: 256 x 128 at launch, 128 x (40 + 216) afterwards, which is as many
-constexpr int SX_REGS_FEW = 40, SX_REGS_MANY = 216;
-constexpr int SX_CHUNK = 128 * 128, SX_TILE = 2 * SX_CHUNK;
-constexpr int SX_SMEM = 3 * SX_TILE + 1024 + 256;
+// pairs of floats in a 64-bit register: one instruction for both
+__device__ __forceinline__ uint64_t sx_pair(float a, float b) { uint64_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ void sx_split(uint64_t x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ uint64_t sx_fma2(uint64_t a, uint64_t b, uint64_t c) { uint64_t r; asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ uint64_t sx_add2(uint64_t a, uint64_t b) { uint64_t r; asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ float sx_max3(float a, float b, float c) { float r; asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
 
-__global__ void __launch_bounds__(SX_THREADS, 2)
+__device__ __forceinline__ void sx_copy16(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void sx_copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// ---- prefixes -----------------------------------------------------------------------------------------------------------------------
+// One CTA per SM with two units, which take turns on the tensor cores: warp 0 fetches pages by TMA (lane <-> page) into two-stage rings, warp 1 issues the
+// MMAs, warps 4..7 and 8..11 gather the queries of a unit, take its softmax (thread <-> row) and keep O in tensor memory.  Where a group has more than 128 rows
+// the units share the keys, otherwise each has every other tile.  Results are stored with the rows of a tile next to each other, so that a warp's stores and the loads of
+// a slot's heads are whole sectors.
+constexpr int SX_THREADS = 384, SX_BN = 128, SX_PS = 16;
+// registers: 384 x 168 at launch, 128 x (72 + 216 + 216) afterwards, which is as many
+constexpr int SX_REGS_FEW = 72, SX_REGS_MANY = 216;
+constexpr int SX_CHUNK = 128 * 128, SX_TILE = 2 * SX_CHUNK;
+constexpr int SX_SMEM = 6 * SX_TILE + 1024 + 256;
+
+__global__ void __launch_bounds__(SX_THREADS, 1)
 attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ SharedParams p) {
   extern __shared__ uint8_t smem_raw[];
   B200_TRACE_INIT();
   if (threadIdx.x == 0) B200_TRACE(TK_ATTN_SHARED, TP_START);
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const uint32_t sQ = smem_u32(smem), sK = sQ + SX_TILE, sV = sK + SX_TILE;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 3 * SX_TILE);
+  const uint32_t sQ = smem_u32(smem), sK = sQ + 2 * SX_TILE, sV = sK + 2 * SX_TILE;        // two units, two stages, two stages
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 6 * SX_TILE);
   const uint32_t bar0 = smem_u32(bars);
-  enum { B_KFULL = 0, B_VFULL, B_SFULL, B_PFULL, B_PVDONE, B_COUNT };
+  enum { B_KFULL = 0, B_KEMPTY = 2, B_VFULL = 4, B_VEMPTY = 6, B_SFULL = 8, B_PFULL = 10, B_OFULL = 12, B_COUNT = 14 };      // two of each: stages or units
   auto bar = [&](int i) { return bar0 + 8u * i; };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + B_COUNT);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* span = reinterpret_cast<int*>(tmem_slot + 2);         // keys that some row of the piece sees: first, end
+  int* spans = reinterpret_cast<int*>(tmem_slot + 2);        // keys that some row of the piece sees: first, end; two pieces in turn
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int dk = p.c.dk, dv = p.c.dv, hkv = p.c.kv_heads, group = p.hq / hkv;
   const int kchunks = (dk + 63) >> 6, vchunks = (dv + 63) >> 6, ksteps = (dk + 15) >> 4, dv16 = (dv + 15) & ~15;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < B_COUNT; ++i) mbar_init(bar(i), i == B_PFULL ? 4 : 1);
+    for (int i = 0; i < B_COUNT; ++i) mbar_init(bar(i), (i & ~1) == B_PFULL ? 4 : 1);
     *abort_flag = 0;
+    spans[0] = spans[2] = 0x7fffffff;
+    spans[1] = spans[3] = 0;
     mbar_fence_init();
   }
-  if (warp == 1) { tmem_alloc(smem_u32(tmem_slot), 256); tmem_relinquish(); }
+  if (warp == 1) { tmem_alloc(smem_u32(tmem_slot), 512); tmem_relinquish(); }
   if (threadIdx.x == 32 * 2) { prefetch_tmap(&tmap_k); prefetch_tmap(&tmap_v); }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;              // S (then P) in 128 columns, O in the next 128
+  const uint32_t tmem = *tmem_slot;              // S (then P) of unit u at 128 u, O at 256 + 128 u
   pdl_wait();
   if (threadIdx.x == 0) B200_TRACE(TK_ATTN_SHARED, TP_DEPS);
   pdl_launch_dependents();       // what starts now may read all that was written before this kernel
+
   auto wait = [&](int i, uint32_t par, int code) { return mbar_wait(bar(i), par, abort_flag, p.status, code | (26 << 8), p.limit_ns); };
   auto meet = [&] { named_bar_sync(1, SX_THREADS); };        // all warps, from the two branches that they are in
-  const int pieces = min(p.plan[0], p.max_pieces) * hkv;
-  auto piece_of = [&](int item) { return *reinterpret_cast<const SharedPiece*>(p.plan + p.pieces_at + (item / hkv) * SP_PIECE); };
-  // tiles of 128 keys from the page of the first key that counts
-  auto tiles_of = [&](int& kv_start, int& kv_end) {
-    kv_start = span[0] & ~(SX_PS - 1);
-    kv_end = span[1];
-    return kv_end > 0 ? (kv_end - kv_start + SX_BN - 1) / SX_BN : 0;
+  auto piece_of = [&](int item) {
+    const int4* at = reinterpret_cast<const int4*>(p.plan + p.pieces_at + (item / hkv) * SP_PIECE);
+    const int4 a = at[0], b = at[1];
+    return SharedPiece{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w & 3, b.w >> 2};
   };
-  uint32_t done = 0;                             // tiles so far: their parities
+  const int room = p.c.max_pages * SX_PS;
+  // Tiles of 128 keys.  Without chunks they are the piece's; a sequence that ends within it sees less of them.  With chunks: from the page of the
+  // first key that counts for somebody, known when the queries are in place.
+  auto tiles_of = [&](const SharedPiece& e, int turn, int& kv_start, int& kv_end) {
+    kv_start = p.chunk > 0 ? spans[2 * turn] & ~(SX_PS - 1) : e.key0;
+    kv_end = p.chunk > 0 ? spans[2 * turn + 1] : min(e.key1, room);
+    return kv_end > kv_start ? (kv_end - kv_start + SX_BN - 1) / SX_BN : 0;
+  };
+  auto units_of = [&](const SharedPiece& e) { return e.mode == SM_KEYS || (e.mode == SM_ROWS && e.rows > 128) ? 2 : 1; };
+  SharedPiece e = piece_of(blockIdx.x);          // there is room for as many pieces as there are CTAs
+  const int pieces = min(p.plan[0], p.max_pieces) * hkv;
+  int turn = 0;
   if (warp < 4) {
     warpgroup_regs_dec<SX_REGS_FEW>();
-    for (int item = blockIdx.x; item < pieces; item += gridDim.x) {
+    uint32_t kv = 0, p_par = 0;                  // tiles so far; bit u: parity of unit u's P
+    for (int item = blockIdx.x; item < pieces; item += gridDim.x, turn ^= 1) {
       const int kvh = item % hkv;
-      const SharedPiece e = piece_of(item);
-      if (threadIdx.x == 0) { span[0] = 0x7fffffff; span[1] = 0; }
-      meet();
-      meet();                                    // the queries are in place, and what they see is known
-      int kv_start, kv_end;
-      const int n = tiles_of(kv_start, kv_end);
+      int kv_start = 0, kv_end = 0, n = 0;
       if (warp == 0) {
-        const int lead = p.plan[p.slots_at + e.member0];
-        const int* pt = p.c.page_table + static_cast<size_t>(lead) * p.c.max_pages;
+        const int* pt = p.c.page_table + static_cast<size_t>(e.lead) * p.c.max_pages;
+        bool ok = true;
+        int page = 0;
         auto page_of = [&](int j) {
           const int tok = kv_start + j * SX_BN + (lane & 7) * SX_PS;
           const int pg = tok < kv_end ? pt[tok / SX_PS] : p.c.num_pages;       // pages behind the end are filled with zeros
@@ -111,100 +136,140 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
           if (p.status) atomicCAS(p.status, 0, static_cast<int>(ST_BAD_ARGUMENT) | (26 << 8));
           return p.c.num_pages;
         };
-        auto load = [&](uint32_t dst, const CUtensorMap* m, int b, int chunks, int page) {
+        auto load = [&](uint32_t dst, const CUtensorMap* m, int b, int chunks, int pg) {
           if (lane == 0) mbar_expect_tx(bar(b), chunks * SX_CHUNK);
           __syncwarp();
           if (lane < 8)
-            for (int c = 0; c < chunks; ++c) tma_load_3d(dst + c * SX_CHUNK + lane * 2048, m, bar(b), c * 64, kvh * SX_PS, page);
+            for (int c = 0; c < chunks; ++c) tma_load_3d(dst + c * SX_CHUNK + lane * 2048, m, bar(b), c * 64, kvh * SX_PS, pg);
         };
-        bool ok = true;
-        int page = n > 0 ? page_of(0) : 0;
-        for (int j = 0; j < n && ok; ++j) {
+        auto fetch = [&](int j) {
           const int next = j + 1 < n ? page_of(j + 1) : 0;
-          // the scores of the tile before are there: its keys are no longer needed; its values once they have been multiplied
-          if (j > 0) ok = __all_sync(0xffffffffu, wait(B_SFULL, (done + j - 1) & 1u, ST_TIMEOUT_SMEM_EMPTY)) != 0;
-          if (!ok) break;
-          load(sK, &tmap_k, B_KFULL, kchunks, page);
-          if (j > 0) ok = __all_sync(0xffffffffu, wait(B_PVDONE, (done + j - 1) & 1u, ST_TIMEOUT_SMEM_EMPTY)) != 0;
-          if (!ok) break;
-          load(sV, &tmap_v, B_VFULL, vchunks, page);
+          const int st = (kv + j) & 1;
+          const uint32_t ph = (((kv + j) >> 1) & 1u) ^ 1u;
+          ok = __all_sync(0xffffffffu, wait(B_KEMPTY + st, ph, ST_TIMEOUT_SMEM_EMPTY)) != 0;
+          if (!ok) return;
+          load(sK + st * SX_TILE, &tmap_k, B_KFULL + st, kchunks, page);
+          ok = __all_sync(0xffffffffu, wait(B_VEMPTY + st, ph, ST_TIMEOUT_SMEM_EMPTY)) != 0;
+          if (!ok) return;
+          load(sV + st * SX_TILE, &tmap_v, B_VFULL + st, vchunks, page);
           page = next;
+        };
+        int j = 0;
+        if (p.chunk <= 0) {                      // the first tiles need not wait for the queries: both stages are free between pieces
+          n = tiles_of(e, turn, kv_start, kv_end);
+          if (n > 0) page = page_of(0);
+          for (; j < min(n, 2) && ok; ++j) fetch(j);
         }
+        meet();                                  // the queries are in place, and what they see is known
+        if (p.chunk > 0) {
+          n = tiles_of(e, turn, kv_start, kv_end);
+          if (n > 0) page = page_of(0);
+        }
+        for (; j < n && ok; ++j) fetch(j);
         if (!ok) { const uint64_t t0 = globaltimer_ns(); while (globaltimer_ns() - t0 < 2000000ull) { } }   // copies in flight land
-      } else if (warp == 1) {
-        const bool one = elect_one();
-        constexpr uint32_t IDESC_S = umma_idesc_bf16(128, 128, 0, 0);
-        const uint32_t idesc_pv = umma_idesc_bf16(128, dv16, 0, 1);
-        const uint64_t q_desc = umma_desc_k_sw128(sQ), k_desc = umma_desc_k_sw128(sK), v_desc = umma_desc_mn_sw128(sV, SX_CHUNK, 1024);
-        bool ok = true;
-        for (int j = 0; j < n && ok; ++j) {
-          const uint32_t par = (done + j) & 1u;
-          ok = wait(B_KFULL, par, ST_TIMEOUT_SMEM_FULL);
-          if (!ok) break;
-          tc_fence_after();
+      } else {
+        meet();
+        n = tiles_of(e, turn, kv_start, kv_end);
+        if (warp == 1) {
+          const bool one = elect_one();
+          constexpr uint32_t IDESC_S = umma_idesc_bf16(128, 128, 0, 0);
+          const uint32_t idesc_pv = umma_idesc_bf16(128, dv16, 0, 1);
+          const uint64_t q_desc = umma_desc_k_sw128(sQ), k_desc = umma_desc_k_sw128(sK), v_desc = umma_desc_mn_sw128(sV, SX_CHUNK, 1024);
+          const int units = units_of(e), lag = e.mode == SM_KEYS ? 2 : 1;      // tiles between two of a unit
+          bool ok = true;
+          // the product of tile j - lag and the scores of tile j, which go to where its weights were
+          for (int j = 0; j < n + lag && ok && n > 0; ++j) {
+            const int past = j - lag;
+            const uint32_t ks = (kv + j) & 1, vs = (kv + past) & 1;
+            if (j < n) ok = wait(B_KFULL + ks, ((kv + j) >> 1) & 1u, ST_TIMEOUT_SMEM_FULL);
+            if (ok && past >= 0) ok = wait(B_VFULL + vs, ((kv + past) >> 1) & 1u, ST_TIMEOUT_SMEM_FULL);
+#pragma unroll 1
+            for (int u = e.mode == SM_KEYS ? j & 1 : 0; u < (e.mode == SM_KEYS ? (j & 1) + 1 : units) && ok; ++u) {
+              if (past >= 0) {
+                ok = wait(B_PFULL + u, (p_par >> u) & 1u, ST_TIMEOUT_TMEM_EMPTY);
+                if (!ok) break;
+                p_par ^= 1u << u;
+                tc_fence_after();
+                const uint64_t bd = v_desc + vs * (SX_TILE >> 4);
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk) {
-            const uint32_t off = (kk >> 2) * (SX_CHUNK >> 4) + 2 * (kk & 3);
-            if (one && kk < ksteps) umma_f16_ss(tmem, q_desc + off, k_desc + off, IDESC_S, kk > 0 ? 1u : 0u);
+                for (int kk = 0; kk < 8; ++kk)
+                  if (one) umma_f16_ts(tmem + 256 + u * 128, tmem + u * 128 + kk * 8, bd + kk * (2048 >> 4), idesc_pv, (past >= lag || kk > 0) ? 1u : 0u);
+                if (one && past + lag >= n) umma_commit(bar(B_OFULL + u));
+              }
+              if (j < n) {
+                tc_fence_after();
+                const uint64_t ad = q_desc + static_cast<uint32_t>(u * (SX_TILE >> 4)), bd = k_desc + ks * (SX_TILE >> 4);
+#pragma unroll
+                for (int kk = 0; kk < 8; ++kk) {
+                  const uint32_t off = (kk >> 2) * (SX_CHUNK >> 4) + 2 * (kk & 3);
+                  if (one && kk < ksteps) umma_f16_ss(tmem + u * 128, ad + off, bd + off, IDESC_S, kk > 0 ? 1u : 0u);
+                }
+                if (one) umma_commit(bar(B_SFULL + u));
+              }
+            }
+            if (ok && one) {
+              if (j < n) umma_commit(bar(B_KEMPTY + ks));
+              if (past >= 0) umma_commit(bar(B_VEMPTY + vs));
+            }
           }
-          if (one) umma_commit(bar(B_SFULL));
-          ok = wait(B_VFULL, par, ST_TIMEOUT_SMEM_FULL) && wait(B_PFULL, par, ST_TIMEOUT_TMEM_EMPTY);
-          if (!ok) break;
-          tc_fence_after();
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
-            if (one) umma_f16_ts(tmem + 128, tmem + kk * 8, v_desc + kk * (2048 >> 4), idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
-          if (one) umma_commit(bar(B_PVDONE));
+          __syncwarp();
+        } else if (threadIdx.x == 64) {          // the other piece's, of which nobody reads any more
+          spans[2 * (turn ^ 1)] = 0x7fffffff;
+          spans[2 * (turn ^ 1) + 1] = 0;
         }
-        __syncwarp();
       }
-      done += n;
+      kv += n;
       meet();
       if (*abort_flag) break;                    // the same for all: nobody sets it between here and the next meeting
+      if (item + static_cast<int>(gridDim.x) < pieces) e = piece_of(item + gridDim.x);
     }
   } else {
     warpgroup_regs_inc<SX_REGS_MANY>();
-    const int r = (warp & 3) * 32 + lane;        // row of the piece, TMEM lane
-    const uint32_t t_s = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16), t_o = t_s + 128;
+    const int u = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;   // unit; row of its tile, TMEM lane
+    const uint32_t t_s = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + u * 128, t_o = t_s + 256;
     const float scale_log2 = p.scale * DW_LOG2E;
-    for (int item = blockIdx.x; item < pieces; item += gridDim.x) {
+    uint32_t tiles = 0, items = 0;               // of this unit: their parities
+    for (int item = blockIdx.x; item < pieces; item += gridDim.x, turn ^= 1) {
       const int kvh = item % hkv;
-      const SharedPiece e = piece_of(item);
-      meet();
+      const int row0 = e.row0 + (e.mode == SM_ROWS ? 128 * u : 0), rows = u < units_of(e) ? min(128, e.rows - (row0 - e.row0)) : 0;
+      const bool idle = (warp & 3) * 32 >= rows;             // rows that nobody asked for: their weights are never looked at
       int low = 0, end = 0;                      // keys that the row sees of this piece
-      {
-        const int row = e.row0 + r, member = row / group;
-        const bool on = r < e.rows;
+      if (!idle) {
+        const int row = row0 + r, member = row / group;
+        const bool on = r < rows;
         const int slot = on ? p.plan[p.slots_at + e.member0 + member] : 0;
         const int len = on ? p.seq_lens[slot] : 0;
+        const long long from = on ? slot * p.ldq + static_cast<long long>(kvh * group + row - member * group) * dk : -1;
         if (len > 0) {
           low = max(e.key0, p.chunk > 0 ? (len - 1) - (len - 1) % p.chunk : 0);
-          end = min(min(e.key1, len), p.c.max_pages * SX_PS);
+          end = min(min(e.key1, len), room);
           if (low >= end) end = 0;
         }
-        if (end > 0) { atomicMin(&span[0], low); atomicMax(&span[1], end); }
-        const __nv_bfloat16* q = p.q + static_cast<size_t>(slot) * p.ldq + static_cast<size_t>(kvh * group + row - member * group) * dk;
-        for (int c = 0; c < kchunks; ++c)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int d = c * 64 + i * 8;
-            const uint4 w = on && d < dk ? *reinterpret_cast<const uint4*>(q + d) : make_uint4(0u, 0u, 0u, 0u);
-            *reinterpret_cast<uint4*>(smem + c * SX_CHUNK + r * 128 + ((i ^ (r & 7)) << 4)) = w;
-          }
+        if (end > 0 && p.chunk > 0) { atomicMin(&spans[2 * turn], low); atomicMax(&spans[2 * turn + 1], end); }
+        // half a warp per row: 256 neighbouring bytes at a time
+        const int col = lane & 15;
+        if (p.chunk <= 0 || __any_sync(0xffffffffu, end > 0))      // with chunks: nobody may see anything
+#pragma unroll 2
+        for (int i = 0; i < 16; ++i) {
+          const long long at = __shfl_sync(0xffffffffu, from, 2 * i + (lane >> 4));
+          const int x = (warp & 3) * 32 + 2 * i + (lane >> 4);
+          const bool there = at >= 0 && col * 8 < dk;        // zeros otherwise
+          sx_copy16(sQ + u * SX_TILE + (col >> 3) * SX_CHUNK + x * 128 + (((col & 7) ^ (x & 7)) << 4), p.q + (there ? at + col * 8 : 0), there);
+        }
+        sx_copies_done();
         fence_proxy_async_smem();
       }
       meet();
-      if (r == 0) B200_TRACE(TK_ATTN_SHARED, 2);             // queries in place
+      if (threadIdx.x == 128) B200_TRACE(TK_ATTN_SHARED, 2); // queries in place
       int kv_start, kv_end;
-      const int n = tiles_of(kv_start, kv_end);
-      const bool idle = (warp & 3) * 32 >= e.rows;          // rows that nobody asked for: their weights are never looked at
+      const int n = rows > 0 ? tiles_of(e, turn, kv_start, kv_end) : 0;
+      const int j0 = e.mode == SM_KEYS ? u : 0, step = e.mode == SM_KEYS ? 2 : 1;
       float m_ref = -INFINITY, l = 0.f;
       bool ok = true;
-      for (int j = 0; j < n && ok; ++j) {
-        const uint32_t par = (done + j) & 1u;
-        ok = __all_sync(0xffffffffu, wait(B_SFULL, par, ST_TIMEOUT_TMEM_FULL)) != 0;
+      for (int j = j0; j < n && ok; j += step) {
+        ok = __all_sync(0xffffffffu, wait(B_SFULL + u, tiles++ & 1u, ST_TIMEOUT_TMEM_FULL)) != 0;
         if (!ok) break;
-        if (r == 0 && j == 0) B200_TRACE(TK_ATTN_SHARED, 3); // first scores
+        if (threadIdx.x == 128 && j == 0) B200_TRACE(TK_ATTN_SHARED, 3);       // first scores
         tc_fence_after();
         if (!idle) {
           uint32_t v[4][32];
@@ -223,87 +288,95 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
           for (int c = 0; c < 4; ++c) {
             mx[c] = __uint_as_float(v[c][0]);
 #pragma unroll
-            for (int i = 1; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(v[c][i]));
+            for (int i = 1; i < 31; i += 2) mx[c] = sx_max3(mx[c], __uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1]));
+            mx[c] = fmaxf(mx[c], __uint_as_float(v[c][31]));
           }
           const float m_new = fmaxf(m_ref, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2);
           if (__any_sync(0xffffffffu, m_new > m_ref)) {
             const float alpha = m_ref == -INFINITY ? 0.f : dw_exp2(m_ref - m_new);
             l *= alpha;
             m_ref = m_new;
-            if (j > 0) {       // the product before has completed: S of this tile was issued after it
-#pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                if (c * 32 >= dv16) break;
+            if (j > j0) {      // the product before has completed: S of this tile was issued after it
+#pragma unroll 1
+              for (int c = 0; c < dv16; c += 32) {
                 uint32_t o[32];
-                tmem_ld_x32(t_o + c * 32, o);
+                tmem_ld_x32(t_o + c, o);
                 tmem_ld_wait();
 #pragma unroll
                 for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                tmem_st_x32(t_o + c * 32, o);
+                tmem_st_x32(t_o + c, o);
               }
             }
           }
           const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          // two at a time; rounded to bf16 for the MMA, the denominator adds what was rounded (which is off by as much to either side)
+          const uint64_t scale2 = sx_pair(scale_log2, scale_log2), shift2 = sx_pair(-m_use, -m_use);
+          uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             uint32_t pk[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const float e0 = dw_exp2(__uint_as_float(v[c][2 * i]) * scale_log2 - m_use), e1 = dw_exp2(__uint_as_float(v[c][2 * i + 1]) * scale_log2 - m_use);
-              const __nv_bfloat162 pb = __floats2bfloat162_rn(e0, e1);
-              pk[i] = *reinterpret_cast<const uint32_t*>(&pb);
-              sum[c] += __uint_as_float(pk[i] << 16) + __uint_as_float(pk[i] & 0xffff0000u);     // what the MMA will actually see
+              float e0, e1;
+              sx_split(sx_fma2(sx_pair(__uint_as_float(v[c][2 * i]), __uint_as_float(v[c][2 * i + 1])), scale2, shift2), e0, e1);
+              e0 = dw_exp2(e0);
+              e1 = dw_exp2(e1);
+              pk[i] = dw_pack(e0, e1);
+              sum[i & 1] = sx_add2(sum[i & 1], sx_pair(e0, e1));
             }
             tmem_st_x16(t_s + c * 16, pk);
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          float l0, l1, l2, l3;
+          sx_split(sum[0], l0, l1);
+          sx_split(sum[1], l2, l3);
+          l += (l0 + l1) + (l2 + l3);
           tmem_st_wait();
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(B_PFULL));
+        if (lane == 0) mbar_arrive(bar(B_PFULL + u));
       }
-      if (r == 0) B200_TRACE(TK_ATTN_SHARED, 4);             // last weights
-      if (ok && n > 0) ok = __all_sync(0xffffffffu, wait(B_PVDONE, (done + n - 1) & 1u, ST_TIMEOUT_TMEM_FULL)) != 0;
+      if (threadIdx.x == 128) B200_TRACE(TK_ATTN_SHARED, 4); // last weights
+      const bool some = j0 < n;
+      if (ok && some) ok = __all_sync(0xffffffffu, wait(B_OFULL + u, items++ & 1u, ST_TIMEOUT_TMEM_FULL)) != 0;
       tc_fence_after();
-      if (r == 0) B200_TRACE(TK_ATTN_SHARED, 5);             // last product
+      if (threadIdx.x == 128) B200_TRACE(TK_ATTN_SHARED, 5); // last product
       if (ok && !idle) {
-        const size_t to = static_cast<size_t>(kvh) * p.part_rows + e.part + e.row0 + r;
-        const bool mine = r < e.rows;
+        // the second unit's results of the same rows are the next part
+        const size_t to = static_cast<size_t>(e.part) + (e.mode == SM_KEYS && u > 0 ? e.group_rows : 0) + row0 + r;
+        const bool mine = r < rows;
         if (mine) {
-          float* ml = p.part + static_cast<size_t>(hkv) * p.part_rows * dv + 2 * to;
-          ml[0] = n > 0 ? m_ref : -INFINITY;
-          ml[1] = l;
+          float2* ml = reinterpret_cast<float2*>(p.part + static_cast<size_t>(hkv) * p.part_rows * dv) + static_cast<size_t>(kvh) * p.part_rows + to;
+          *ml = make_float2(some ? m_ref : -INFINITY, l);
         }
-        if (n > 0) {
-          float4* dst = reinterpret_cast<float4*>(p.part + to * dv);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            if (c * 32 >= dv16) break;
+        // nothing for a run of keys that nobody sees: its weights say so
+        float4* dst = reinterpret_cast<float4*>(p.part) + static_cast<size_t>(kvh) * (dv >> 2) * p.part_rows + to;
+        if (some)
+#pragma unroll 1
+          for (int c = 0; c < dv16; c += 32) {
             uint32_t o[32];
-            tmem_ld_x32(t_o + c * 32, o);
+            tmem_ld_x32(t_o + c, o);
             tmem_ld_wait();
-            if (mine) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                if (c * 32 + i * 4 < dv)
-                  dst[c * 8 + i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
-            }
+            for (int i = 0; i < 8; ++i)
+              if (mine && c + i * 4 < dv)
+                dst[static_cast<size_t>((c >> 2) + i) * p.part_rows] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
           }
-        }
       }
       tc_fence_before();
-      done += n;
       meet();
-      if (r == 0) B200_TRACE(TK_ATTN_SHARED, 6);             // a piece
+      if (threadIdx.x == 128) {
+        if (!*abort_flag) red_release_gpu_add(reinterpret_cast<uint32_t*>(p.plan + SP_DONE), 1u);
+        B200_TRACE(TK_ATTN_SHARED, 6);           // a piece
+      }
       tc_fence_after();
       if (*abort_flag) break;
+      if (item + static_cast<int>(gridDim.x) < pieces) e = piece_of(item + gridDim.x);
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem, 256); }
+  if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem, 512); }
   if (threadIdx.x == 0) B200_TRACE(TK_ATTN_SHARED, TP_EXIT);
   B200_TRACE_FLUSH(TK_ATTN_SHARED);
 }
@@ -311,14 +384,27 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
 // ---- own keys, and the join ---------------------------------------------------------------------------------------------------------
 // Grid (split, KV head x group of up to 16 query heads, slot); the splits of a slot are a cluster.  Four warps take pages in turn.
 constexpr int SO_THREADS = 128, SO_WARPS = 4, SO_PARTS = 32;
-constexpr int SO_AHEAD = 6;              // pages of a warp asked for into L2 ahead of their use
+constexpr int SO_AHEAD = 3;              // pages of a warp asked for into L2 ahead of their use
 template <int DV> struct SoShape {
   static constexpr int PITCH = DV + 4, SIZE = 16 * PITCH + 32;
   static constexpr int SMEM = ((SO_WARPS + 1) * SIZE + 16 * (8 + SO_PARTS)) * 4;
 };
 
+// The last CTA to leave clears the counters for the next call, which starts behind this kernel; every CTA leaves behind the first kernel.
+__device__ __forceinline__ void so_leave(const SharedParams& p) {
+  if (threadIdx.x == 0) {
+    const unsigned all = gridDim.x * gridDim.y * gridDim.z;
+    if (atomicAdd(reinterpret_cast<unsigned*>(p.plan + SP_SEEN), 1u) == all - 1u) {
+      pdl_wait();                                // no piece is still to be counted, not even one that was given up
+      p.plan[SP_DONE] = 0;
+      p.plan[SP_SEEN] = 0;
+    }
+  }
+  pdl_wait();
+}
+
 template <int DK, int DV, int NH, bool FULL>
-__global__ void __launch_bounds__(SO_THREADS, 2) attn_shared_own_kernel(const __grid_constant__ SharedParams p) {
+__global__ void __launch_bounds__(SO_THREADS, NH == 1 ? 3 : 2) attn_shared_own_kernel(const __grid_constant__ SharedParams p) {
   using Sh = SoShape<DV>;
   extern __shared__ __align__(16) float so_smem[];
   B200_TRACE_INIT();
@@ -335,9 +421,9 @@ __global__ void __launch_bounds__(SO_THREADS, 2) attn_shared_own_kernel(const __
   const bool bad = len > p.c.max_pages * SX_PS;
   if (len <= 0 || bad) {                         // the same for all CTAs of the cluster
     if (bad && tid == 0 && p.status) atomicCAS(p.status, 0, static_cast<int>(ST_BAD_ARGUMENT) | (26 << 8));
-    pdl_wait();
     if (rank == 0)
       for (int i = tid; i < G * dv; i += SO_THREADS) p.out[static_cast<size_t>(b) * p.ldo + static_cast<size_t>(h0) * dv + i] = __float2bfloat16(0.f);
+    so_leave(p);
     return;
   }
   const int low = max(p.chunk > 0 ? (len - 1) - (len - 1) % p.chunk : 0, min(info.w, len));      // first key that is this kernel's
@@ -353,7 +439,7 @@ __global__ void __launch_bounds__(SO_THREADS, 2) attn_shared_own_kernel(const __
   w.begin(dk, dv, p.scale);
   // the ids of this warp's next 32 pages are in its lanes
   int ids = 0, ids_from = -32;
-  w.template walk<NH == 1>(mine, [&](int i) {
+  w.template walk<false>(mine, [&](int i) {
     if (i >= ids_from + 32) {
       ids_from = i;
       ids = i + lane < mine ? pt[ta + warp + (i + lane) * SO_WARPS] : -1;
@@ -373,11 +459,15 @@ __global__ void __launch_bounds__(SO_THREADS, 2) attn_shared_own_kernel(const __
   float* own = so_smem + SO_WARPS * Sh::SIZE;
   float* share = own + Sh::SIZE;                 // [16][8 + SO_PARTS]: what each part counts in the end
   dw_join<SO_WARPS, SO_THREADS>(so_smem, Sh::SIZE, Sh::PITCH, G, dv, own);
+  // The parts of the prefix.  All CTAs of the first kernel run when this one starts, so their pieces may be waited for; the wait for its end takes 2 us longer.
+  if (tid == 0 && info.z > 0) {
+    const uint32_t pieces = static_cast<uint32_t>(min(p.plan[0], p.max_pieces)) * p.c.kv_heads;
+    wait_count_gpu(reinterpret_cast<const uint32_t*>(p.plan + SP_DONE), pieces, p.status, static_cast<int>(ST_TIMEOUT_PEER_FLAG) | (26 << 8), p.limit_ns);
+  }
   if (S > 1) cluster_sync_all(); else __syncthreads();
-  pdl_wait();                                    // the parts of the prefix
   if (tid == 0) B200_TRACE(TK_ATTN_OWN, TP_DEPS);
   const uint32_t own_addr = smem_u32(own);
-  const float* parts = p.part + (static_cast<size_t>(kvh) * p.part_rows + info.x + g0) * dv;
+  const float4* parts = reinterpret_cast<const float4*>(p.part) + static_cast<size_t>(kvh) * (dv >> 2) * p.part_rows + info.x + g0;
   const float* ml = p.part + static_cast<size_t>(p.c.kv_heads) * p.part_rows * dv + 2 * (static_cast<size_t>(kvh) * p.part_rows + info.x + g0);
   const int n_parts = min(info.z, SO_PARTS), all = S + n_parts;
   // a warp per row: lanes take the parts
@@ -415,26 +505,26 @@ __global__ void __launch_bounds__(SO_THREADS, 2) attn_shared_own_kernel(const __
   // four dimensions per thread, the parts in turn: their loads do not wait for one another
   const int quads = dv >> 2;
   for (int i = rank * SO_THREADS + tid; i < G * quads; i += S * SO_THREADS) {
-    const int g = i / quads, d = (i - g * quads) * 4;
+    const int d = i / G * 4, g = i - i / G * G;              // heads side by side, as the parts of the prefix have them
     const float* f = share + g * (8 + SO_PARTS);
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < S; ++s) {
-      if (f[s] == 0.f) continue;
-      const uint32_t base = (S > 1 ? mapa_shared(own_addr, s) : own_addr) + 4u * (g * Sh::PITCH + d);
-      v.x += f[s] * dw_ld_cluster(base); v.y += f[s] * dw_ld_cluster(base + 4); v.z += f[s] * dw_ld_cluster(base + 8); v.w += f[s] * dw_ld_cluster(base + 12);
-    }
 #pragma unroll 4
+    for (int s = 0; s < S; ++s) {
+      const float4 x = dw_ld_cluster4(own_addr + 4u * (g * Sh::PITCH + d), s, S > 1);
+      v.x += f[s] * x.x; v.y += f[s] * x.y; v.z += f[s] * x.z; v.w += f[s] * x.w;
+    }
+#pragma unroll 8
     for (int s = 0; s < n_parts; ++s) {
-      const float fs = f[S + s];
-      if (fs == 0.f) continue;                   // a part without keys has left no numbers
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(parts + (static_cast<size_t>(s) * info.y + g) * dv + d));
+      const float fs = f[S + s];                 // zero: a part without keys, which has left no numbers
+      const float4 x = fs != 0.f ? __ldcg(parts + static_cast<size_t>(d >> 2) * p.part_rows + static_cast<size_t>(s) * info.y + g) : make_float4(0.f, 0.f, 0.f, 0.f);
       v.x += fs * x.x; v.y += fs * x.y; v.z += fs * x.z; v.w += fs * x.w;
     }
     const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), c = __floats2bfloat162_rn(v.z, v.w);
     *reinterpret_cast<uint2*>(p.out + static_cast<size_t>(b) * p.ldo + static_cast<size_t>(h0 + g) * dv + d) =
         make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&c));
   }
-  if (S > 1) cluster_sync_all();                 // no CTA leaves while a peer may still read its part
+  if (S > 1) cluster_sync_all(); else __syncthreads();       // no CTA leaves while a peer may still read its part
+  so_leave(p);
   if (tid == 0) B200_TRACE(TK_ATTN_OWN, TP_EXIT);
   B200_TRACE_FLUSH(TK_ATTN_OWN);
 }
@@ -464,7 +554,7 @@ extern "C" int b200_attn_decode_shared_takes(const b200_paged_cache* c, int hq, 
 }
 
 extern "C" int b200_attn_decode_shared(const void* q, long long ldq, void* out, long long ldo, int hq, int B, const int* seq_lens, const b200_paged_cache* c,
-                                       const b200_attn_spec* s, const int* plan, int pieces_at, int slots_at, int max_pieces, float* part, int part_rows,
+                                       const b200_attn_spec* s, int* plan, int pieces_at, int slots_at, int max_pieces, float* part, int part_rows,
                                        int splits, int num_sms, int* status, cudaStream_t stream) {
   if (B <= 0) return 0;
   if (!q || !out || !seq_lens || !c || !c->data || !c->page_table || !s || !plan || !part) return -1;
@@ -486,7 +576,7 @@ extern "C" int b200_attn_decode_shared(const void* q, long long ldq, void* out, 
   cudaError_t e = cudaFuncSetAttribute(attn_shared_prefix_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SX_SMEM);
   if (e != cudaSuccess) return -1000 - static_cast<int>(e);
   const long long most = static_cast<long long>(max_pieces) * c->kv_heads;
-  const int grid = most < 2 * num_sms ? static_cast<int>(most > 0 ? most : 1) : 2 * num_sms;
+  const int grid = most < num_sms ? static_cast<int>(most > 0 ? most : 1) : num_sms;
   launch_ex(attn_shared_prefix_kernel, dim3(grid), dim3(SX_THREADS), SX_SMEM, stream, 0, tk, tv, p);
   e = cudaGetLastError();
   if (e != cudaSuccess) return -2000 - static_cast<int>(e);

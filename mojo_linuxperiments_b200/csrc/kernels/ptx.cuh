@@ -331,10 +331,22 @@ __device__ __forceinline__ void st_release_gpu(uint32_t* p, uint32_t v) {
 __device__ __forceinline__ void fence_proxy_async_all() {
   asm volatile("fence.proxy.async;" ::: "memory");
 }
+__device__ __forceinline__ void red_release_gpu_add(uint32_t* p, uint32_t v) {
+  asm volatile("red.release.gpu.global.add.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+}
 __device__ __forceinline__ uint32_t ld_acquire_gpu(const uint32_t* p) {
   uint32_t v;
   asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
   return v;
+}
+// Wait until *p >= count, which CTAs of this GPU that are known to run add to. Bounded.
+__device__ __forceinline__ bool wait_count_gpu(const uint32_t* p, uint32_t count, int* status, int code, uint64_t limit_ns) {
+  if (ld_acquire_gpu(p) >= count) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (globaltimer_ns() - t0 <= limit_ns)
+    if (ld_acquire_gpu(p) >= count) return true;
+  if (status) atomicCAS(status, 0, code);
+  return false;
 }
 // Wait until *p >= target (monotonic epochs; wrap-safe signed compare). Bounded.
 __device__ __forceinline__ bool wait_flag_ge(const uint32_t* p, uint32_t target, int* status, uint64_t limit_ns) {

@@ -10,29 +10,61 @@ from .attention import PAGE, PagedKVCache, attn_paged, pick_decode_splits_paged
 from .workspace import default_workspace
 
 KEY_TILE = 128                 # keys of a step of the kernel
-ROW_TILE = 128                 # rows (member x query head) of a piece
+ROW_TILE = 128                 # rows (member x query head) of one of its two units
 MAX_PARTS = 32                 # parts of a prefix
 _INFO, _PIECE = 16, 8          # where the numbers per slot start, numbers per piece
+_ROWS, _KEYS, _ONE = 0, 1, 2   # two tiles of rows; one, and every other tile of keys for each unit; one unit
 
 
-def cut_prefixes(groups, num_seqs: int, per_head: int, kv_heads: int, ctas: int):
+def room_for(num_seqs: int, per_head: int, kv_heads: int, ctas: int) -> tuple[int, int]:
+    """Pieces, and rows of partial results per KV head, that a plan has room for: every prefix as one run, and two rounds of the CTAs beyond that."""
+    more = -(-2 * ctas // kv_heads)
+    return num_seqs * per_head // (2 * ROW_TILE) + num_seqs + more, 2 * num_seqs * per_head + 2 * ROW_TILE * more
+
+
+def cut_prefixes(groups, num_seqs: int, per_head: int, kv_heads: int, ctas: int, others: int = 0):
     """How the prefixes of ``groups`` (slots, tokens) are shared out: (four numbers per slot, pieces, slots in order, rows of partial results).
 
-    A piece is up to 128 rows of a group (whole members where a member has no more rows than that) and a run of tiles of 128 keys, for every KV head; runs
-    are as long as makes about ``ctas`` pieces of all of them.  A slot's numbers: first row of its partial results, rows between the parts, parts, tokens."""
-    tile_rows = ROW_TILE // per_head * per_head if per_head <= ROW_TILE else ROW_TILE
-    sizes = [(len(slots) * per_head, -(-tokens // KEY_TILE)) for slots, tokens in groups]
-    units = kv_heads * sum(-(-rows // tile_rows) * tiles for rows, tiles in sizes)
-    run = max(1, -(-units // ctas))
+    A piece is up to 256 rows of a group and a run of tiles of 128 keys, for every KV head.  The two units of a CTA have 128 rows each, or, in a group of no
+    more than 128, the same rows and every other tile.  Runs are as long as ends soonest: pieces of L steps take L + 4 (their start and end), ``ctas`` of
+    them at a time, and ``others``, the CTAs of the slots' own keys, three of which fit where there is no piece, another 4 if some of them have to wait.  A slot's numbers: first row of its partial results, rows between the parts, parts, tokens."""
     info, pieces, order, base = [0] * (4 * num_seqs), [], [], 0
+    if not groups:
+        return info, pieces, order, base
+    sizes = [(len(slots) * per_head, -(-tokens // KEY_TILE)) for slots, tokens in groups]
+    most = room_for(num_seqs, per_head, kv_heads, ctas)
+
+    def shape(rows, tiles, steps):
+        """mode, runs of keys of ``steps`` steps each at most, parts of the results"""
+        if rows > ROW_TILE:
+            runs = min(MAX_PARTS, -(-tiles // steps))
+            return _ROWS, runs, runs
+        runs = min(MAX_PARTS // 2, max(1, tiles // 2), -(-tiles // (2 * steps)))
+        return (_ONE, 1, 1) if tiles == 1 else (_KEYS, runs, 2 * runs)
+
+    def took(steps):
+        longest = count = room = 0
+        for rows, tiles in sizes:
+            mode, runs, parts = shape(rows, tiles, steps)
+            longest = max(longest, -(-tiles // runs) if mode == _ROWS else -(-tiles // (2 * runs)))
+            count += -(-rows // (2 * ROW_TILE)) * runs
+            room += rows * parts
+        fits, count = count <= most[0] and room <= most[1], kv_heads * count
+        return not fits, -(-count // ctas) * (longest + 4) + (4 if others > 3 * max(0, ctas - count) else 0)
+
+    tried, at = [], max(tiles for _, tiles in sizes)       # one run each always fits
+    while at >= 1:
+        tried.append(at)
+        at = min(at - 1, int(at / 1.06))
+    steps = min(tried, key=took)
     for (slots, tokens), (rows, tiles) in zip(groups, sizes):
-        parts = min(MAX_PARTS, -(-tiles // run))
+        mode, runs, parts = shape(rows, tiles, steps)
         for i, s in enumerate(slots):
             info[4 * s:4 * s + 4] = [base + i * per_head, rows, parts, tokens]
-        for row0 in range(0, rows, tile_rows):
-            for k in range(parts):
-                a, b = tiles * k // parts * KEY_TILE, min(tokens, tiles * (k + 1) // parts * KEY_TILE)
-                pieces.append([len(order), len(slots), row0, min(tile_rows, rows - row0), a, b, base + k * rows, 0])
+        for k in range(runs):
+            a, b = tiles * k // runs * KEY_TILE, min(tokens, tiles * (k + 1) // runs * KEY_TILE)
+            for row0 in range(0, rows, 2 * ROW_TILE):
+                pieces.append([len(order), row0, min(2 * ROW_TILE, rows - row0), a, b, base + k * (parts // runs) * rows, slots[0], mode + 4 * rows])
         base += rows * parts
         order += slots
     return info, pieces, order, base
@@ -43,11 +75,7 @@ class _Cut:
 
     def __init__(self, num_seqs: int, per_head: int, kv_heads: int, dv: int, device: torch.device):
         self.per_head, self.kv_heads, self.sms = per_head, kv_heads, _lib.num_sms(device.index)
-        self.ctas = 2 * self.sms
-        per_cta = -(-self.ctas // kv_heads)
-        tiles_each = -(-per_head // ROW_TILE) if per_head > ROW_TILE else 1
-        self.max_pieces = per_cta + num_seqs * tiles_each
-        self.rows = max(1, num_seqs * per_head + ROW_TILE * per_cta)
+        self.max_pieces, self.rows = room_for(num_seqs, per_head, kv_heads, self.sms)
         self.pieces_at = (_INFO + 4 * num_seqs + 7) // 8 * 8
         self.slots_at = self.pieces_at + _PIECE * self.max_pieces
         n = self.slots_at + num_seqs
@@ -58,12 +86,13 @@ class _Cut:
         self.turn = 0
 
     def send(self, groups, num_seqs: int) -> None:
-        info, pieces, order, rows = cut_prefixes(groups, num_seqs, self.per_head, self.kv_heads, self.ctas)
+        others = num_seqs * self.kv_heads * -(-self.per_head // 16)
+        info, pieces, order, rows = cut_prefixes(groups, num_seqs, self.per_head, self.kv_heads, self.sms, others)
         assert len(pieces) <= self.max_pieces and rows <= self.rows
         buf, done = self.ring[self.turn]
         self.turn = (self.turn + 1) % len(self.ring)
         done.synchronize()                       # its previous copy has left the buffer
-        buf[0] = len(pieces)
+        buf[0] = len(pieces)                     # the counters behind it are the kernels' own: zero between calls
         buf[_INFO:_INFO + 4 * num_seqs] = torch.tensor(info, dtype=torch.int32)
         if pieces:
             buf[self.pieces_at:self.pieces_at + _PIECE * len(pieces)] = torch.tensor(pieces, dtype=torch.int32).flatten()

@@ -63,27 +63,37 @@ def test_clusters_for_selections(pairs, pages, want):
 
 @pytest.mark.parametrize("per_head,kv_heads,groups", [
     (4, 8, [(list(range(32)), 2048)]), (4, 8, [(list(range(128)), 32768)]), (20, 1, [([3, 1, 2], 16), ([0, 7], 160), ([5], 4096)]),
-    (160, 1, [([1, 0, 2], 272)]), (1, 1, [(list(range(200)), 16)]), (7, 3, [([i, 199 - i], 16 * (1 + i)) for i in range(90)]), (4, 8, [])])
+    (160, 1, [([1, 0, 2], 272)]), (1, 1, [(list(range(200)), 16)]), (7, 3, [([i, 199 - i], 16 * (1 + i)) for i in range(90)]), (4, 8, []),
+    (16, 4, [(list(range(i, 200, 16)), 16 * (300 + 7 * i)) for i in range(16)]), (4, 8, [([i], 16) for i in range(200)]), (4, 1, [([7, 9], 16 * 60000)])])
 def test_pieces_of_prefixes_cover_every_row_and_key_once(per_head, kv_heads, groups):
-    n, ctas = 200, 296
+    n, ctas = 200, 148
     info, pieces, order, rows = SH.cut_prefixes(groups, n, per_head, kv_heads, ctas)
-    # what a plan has room for
-    per_cta = -(-ctas // kv_heads)
-    assert len(pieces) <= per_cta + n * (-(-per_head // 128) if per_head > 128 else 1) and rows <= n * per_head + 128 * per_cta and len(order) <= n
+    room = SH.room_for(n, per_head, kv_heads, ctas)
+    assert len(pieces) <= room[0] and rows <= room[1] and len(order) <= n
+    size = {slots[0]: (len(slots) * per_head, tokens) for slots, tokens in groups}
     seen, used = {}, set()
-    for member0, members, row0, count, key0, key1, part, _ in pieces:
-        assert 0 < count <= 128 and row0 + count <= members * per_head and key0 % 128 == 0 and key0 < key1
-        for r in range(row0, row0 + count):
-            slot, head = order[member0 + r // per_head], r % per_head
-            seen.setdefault((slot, head), []).append((key0, key1, part + r))
-            used.add(part + r)
-    assert len(used) == sum(len(v) for v in seen.values()) and all(0 <= u < rows for u in used)
+    for member0, row0, count, key0, key1, part, lead, mode in pieces:
+        group_rows, tokens = size[lead]
+        assert mode >> 2 == group_rows
+        mode &= 3
+        assert order[member0] == lead and 0 < count <= 256 and row0 + count <= group_rows and key0 % 128 == 0 and key0 < key1 <= tokens
+        tiles = list(range(key0, key1, 128))
+        assert count <= 128 or mode == 0
+        assert len(tiles) > 1 or mode != 1
+        for unit in range(2 if mode == 1 else 1):
+            for r in range(row0, row0 + count):
+                slot, head = order[member0 + r // per_head], r % per_head
+                at = part + unit * group_rows + r
+                assert at not in used
+                used.add(at)
+                seen.setdefault((slot, head), []).append((tiles[unit::2] if mode == 1 else tiles, at))
+    assert all(0 <= u < rows for u in used)
     for slots, tokens in groups:
         for s in slots:
             first, step, parts, t = info[4 * s:4 * s + 4]
             assert t == tokens and 0 < parts <= SH.MAX_PARTS
             for h in range(per_head):
-                runs = sorted(seen.pop((s, h)))
-                assert runs[0][0] == 0 and runs[-1][1] == tokens and all(a[1] == b[0] for a, b in zip(runs, runs[1:]))
-                assert [r[2] for r in runs] == [first + h + k * step for k in range(parts)]
+                runs = seen.pop((s, h))
+                assert sorted(k for tiles, _ in runs for k in tiles) == list(range(0, tokens, 128))
+                assert sorted(at for _, at in runs) == [first + h + k * step for k in range(parts)]
     assert not seen and all(info[4 * s + 2] == 0 for s in range(n) if s not in set(order))
