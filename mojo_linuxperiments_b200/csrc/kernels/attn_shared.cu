@@ -532,7 +532,7 @@ __global__ void __launch_bounds__(SO_THREADS, NH == 1 ? 3 : 2) attn_shared_own_k
 template <int DK, int DV, int NH, bool FULL>
 static int launch_shared_own_as(const SharedParams& p, cudaStream_t stream) {
   constexpr int SMEM = SoShape<DV>::SMEM;
-  cudaError_t e = cudaFuncSetAttribute(attn_shared_own_kernel<DK, DV, NH, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+  cudaError_t e = allow_smem<attn_shared_own_kernel<DK, DV, NH, FULL>>(SMEM);
   if (e != cudaSuccess) return -1000 - static_cast<int>(e);
   launch_ex(attn_shared_own_kernel<DK, DV, NH, FULL>, dim3(p.splits, p.c.kv_heads * p.hgroups, p.B), dim3(SO_THREADS), SMEM, stream, p.splits, p);
   e = cudaGetLastError();
@@ -573,7 +573,7 @@ extern "C" int b200_attn_decode_shared(const void* q, long long ldq, void* out, 
   p.scale = s->scale; p.sink = s->sink; p.gate = static_cast<const __nv_bfloat16*>(s->gate); p.ldg = s->ldg; p.splits = splits;
   p.hgroups = (hq / c->kv_heads + 15) / 16; p.status = status; p.limit_ns = 2000000000ull;
   if (static_cast<long long>(c->kv_heads) * p.hgroups > 65535) return -3;
-  cudaError_t e = cudaFuncSetAttribute(attn_shared_prefix_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SX_SMEM);
+  cudaError_t e = allow_smem<attn_shared_prefix_kernel>(SX_SMEM);
   if (e != cudaSuccess) return -1000 - static_cast<int>(e);
   const long long most = static_cast<long long>(max_pieces) * c->kv_heads;
   const int grid = most < num_sms ? static_cast<int>(most > 0 ? most : 1) : num_sms;

@@ -444,15 +444,14 @@ __global__ void __launch_bounds__(PS_THREADS, 1) attn_sparse_kernel(const __grid
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------------------------
-template <typename K>
-static int launch_sparse_pair(K scores, dim3 grid1, size_t smem1, K attend, size_t smem2, const SparseParams& p, cudaStream_t stream) {
+template <auto Scores, auto Attend>
+static int launch_sparse_pair(dim3 grid1, size_t smem1, size_t smem2, const SparseParams& p, cudaStream_t stream) {
   if (smem1 > SPARSE_MAX_SMEM || smem2 > SPARSE_MAX_SMEM) return -5;
-  cudaError_t e = cudaSuccess;
-  if (smem1 > (48u << 10)) e = cudaFuncSetAttribute(scores, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SPARSE_MAX_SMEM));
-  if (e == cudaSuccess && smem2 > (40u << 10)) e = cudaFuncSetAttribute(attend, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SPARSE_MAX_SMEM));
+  cudaError_t e = smem1 > (48u << 10) ? allow_smem<Scores>(static_cast<int>(SPARSE_MAX_SMEM)) : cudaSuccess;
+  if (e == cudaSuccess) e = allow_smem<Attend>(static_cast<int>(SPARSE_MAX_SMEM));
   if (e != cudaSuccess) return -1000 - static_cast<int>(e);
-  launch_ex(scores, grid1, dim3(SC_THREADS), smem1, stream, 0, p);
-  launch_ex(attend, dim3(p.splits, p.c.kv_heads * p.hgroups, p.M), dim3(PS_THREADS), smem2, stream, p.splits, p);
+  launch_ex(Scores, grid1, dim3(SC_THREADS), smem1, stream, 0, p);
+  launch_ex(Attend, dim3(p.splits, p.c.kv_heads * p.hgroups, p.M), dim3(PS_THREADS), smem2, stream, p.splits, p);
   e = cudaGetLastError();
   return e == cudaSuccess ? 0 : -2000 - static_cast<int>(e);
 }
@@ -469,16 +468,16 @@ static int launch_sparse_any(SparseParams p, cudaStream_t stream) {
   const size_t floats = static_cast<size_t>(PS_WARPS + 16) * (p.c.dv + 2) + 16 * static_cast<size_t>(p.c.dk);
   fit_scores(p, floats);
   const dim3 grid((p.c.max_pages + SCA_PAGES - 1) / SCA_PAGES, p.c.kv_heads, p.M);
-  return launch_sparse_pair(page_scores_any_kernel<T>, grid, 4 * static_cast<size_t>(p.hq / p.c.kv_heads) * p.c.dk, attn_sparse_any_kernel<T>,
-                            4 * (floats + p.list_cap + p.score_cap), p, stream);
+  return launch_sparse_pair<page_scores_any_kernel<T>, attn_sparse_any_kernel<T>>(grid, 4 * static_cast<size_t>(p.hq / p.c.kv_heads) * p.c.dk,
+                                                                                 4 * (floats + p.list_cap + p.score_cap), p, stream);
 }
 
 template <int DK, int DV, int NH, bool FULL>
 static int launch_sparse(SparseParams p, cudaStream_t stream) {
   fit_scores(p, SparseShape<DV>::FLOATS);
   const dim3 grid((p.c.max_pages + SC_PAGES - 1) / SC_PAGES, p.c.kv_heads, p.M);
-  return launch_sparse_pair(page_scores_kernel<DK, NH, FULL>, grid, 0, attn_sparse_kernel<DK, DV, NH, FULL>,
-                            4 * (static_cast<size_t>(SparseShape<DV>::FLOATS) + p.score_cap + p.list_cap), p, stream);
+  return launch_sparse_pair<page_scores_kernel<DK, NH, FULL>, attn_sparse_kernel<DK, DV, NH, FULL>>(
+      grid, 0, 4 * (static_cast<size_t>(SparseShape<DV>::FLOATS) + p.score_cap + p.list_cap), p, stream);
 }
 
 template <int DK, int DV, bool FULL>

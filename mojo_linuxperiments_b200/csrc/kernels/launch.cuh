@@ -62,6 +62,19 @@ static inline cudaError_t launch_ex_cluster(void (*kernel)(KArgs...), dim3 grid,
   return launch_with(true, cluster, kernel, grid, block, smem, stream, static_cast<Args&&>(args)...);
 }
 
+// Let a kernel use `bytes` of dynamic shared memory: once per kernel and device
+template <auto Kernel>
+static inline cudaError_t allow_smem(int bytes) {
+  static bool done[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 64 && done[dev]) return cudaSuccess;
+  e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done[dev] = true;
+  return e;
+}
+
 // First kernel of a step: starts when everything before it in the stream has completed.  Kernels of the step read what was settled
 // before it (lengths, positions, page table) ahead of their own dependency wait, which orders them behind their predecessor alone, and
 // that one behind its own; this launch is what orders the whole chain behind the end of the step before (decode_advance,

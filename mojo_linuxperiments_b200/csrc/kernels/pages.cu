@@ -5,8 +5,8 @@
 // written once; a CTA takes 16 KiB of one record, four loads of 16 bytes per thread in flight.
 //
 // page_bounds: lo[d] = min_t k[t][d], hi[d] = max_t k[t][d] over the tokens of a page that a sequence has, per KV head.  Both are values of the
-// keys' own type, so nothing is rounded.  A warp takes one head of one page; lanes lie along the row of 16-byte pieces and, where a row has fewer
-// than 32 of them, along the tokens.
+// keys' own type, so nothing is rounded.  Bound by the bytes of the keys.  A CTA takes eight pages, whose numbers it looks up at once, and a warp one head of one of
+// them after the other; lanes lie along the row of 16-byte pieces and, where a row has fewer than 32 of them, along the tokens.
 #include "ptx.cuh"
 #include "api.h"
 #include "launch.cuh"
@@ -58,7 +58,7 @@ static int copy_pages_some(void* const* arrays, const long long* records, int n_
 }
 
 // ---- bounds ------------------------------------------------------------------------------------------------------------------
-constexpr int PB_WARPS = 8;
+constexpr int PB_WARPS = 8, PB_PAGES = 8;
 
 struct PageBoundsParams {
   b200_paged_cache c;
@@ -67,78 +67,97 @@ struct PageBoundsParams {
   int* status;
 };
 
-// the smaller and the larger of two, NaN where one of them is: a page with a key that is not a number is not left out
-__device__ __forceinline__ float pb_min(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
-__device__ __forceinline__ float pb_max(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
-template <typename T> struct PbVec;
-template <> struct PbVec<float> {
-  static __device__ void first(float (&x)[4], uint4 r) { x[0] = __uint_as_float(r.x); x[1] = __uint_as_float(r.y); x[2] = __uint_as_float(r.z); x[3] = __uint_as_float(r.w); }
+// The smaller and the larger of two (of two pairs, in bf16), NaN where one of them is: a page with a key that is not a number is not left out.  All on the words that
+// a row is read in: nothing is converted.
+template <typename T> struct PbWord;
+template <> struct PbWord<float> {
+  using W = uint32_t;
+  static constexpr uint32_t MOST = 0x7f800000u, LEAST = 0xff800000u;
+  static __device__ __forceinline__ uint32_t lesser(uint32_t a, uint32_t b) { uint32_t r; asm("min.NaN.f32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { uint32_t r; asm("max.NaN.f32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
 };
-template <> struct PbVec<__nv_bfloat16> {
-  static __device__ void first(float (&x)[8], uint4 r) {
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-  }
+template <> struct PbWord<__nv_bfloat16> {
+  using W = uint16_t;
+  static constexpr uint32_t MOST = 0x7f807f80u, LEAST = 0xff80ff80u;
+  static __device__ __forceinline__ uint32_t lesser(uint32_t a, uint32_t b) { uint32_t r; asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { uint32_t r; asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
 };
-__device__ __forceinline__ float pb_f(float v) { return v; }
-__device__ __forceinline__ float pb_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ void pb_put(float* p, float v) { *p = v; }
-__device__ __forceinline__ void pb_put(__nv_bfloat16* p, float v) { *p = __float2bfloat16(v); }      // exact: the value is one of the keys'
 
-// VEC: rows are whole pieces of 16 bytes
+// VEC: rows are whole pieces of 16 bytes; otherwise a piece is one element
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(32 * PB_WARPS) page_bounds_kernel(const __grid_constant__ PageBoundsParams p) {
-  constexpr int N = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
+  using P = PbWord<T>;
+  constexpr int N = VEC ? 16 / static_cast<int>(sizeof(T)) : 1, WORDS = VEC ? 4 : 1, BATCH = 8;
   pdl_launch_dependents();
   pdl_wait();
+  __shared__ int ids[PB_PAGES];
   const int lane = threadIdx.x & 31, b = blockIdx.y, ps = p.c.page_size, dk = p.c.dk;
-  const int unit = blockIdx.x * PB_WARPS + (threadIdx.x >> 5), at = unit / p.c.kv_heads, h = unit - at * p.c.kv_heads;
   const int start = p.starts[b], end = p.ends[b], seq = p.seq_ids ? p.seq_ids[b] : b;
   if (end <= start) return;
   if (start < 0 || seq < 0 || seq >= p.c.num_seqs || (end - 1) / ps >= p.c.max_pages) {
     if (threadIdx.x == 0 && blockIdx.x == 0 && p.status) atomicCAS(p.status, 0, static_cast<int>(ST_BAD_ARGUMENT) | (24 << 8));
     return;
   }
-  const int place = start / ps + at;
-  if (place > (end - 1) / ps) return;
-  const int page = p.c.page_table[static_cast<size_t>(seq) * p.c.max_pages + place];
-  if (page < 0 || page >= p.c.num_pages) {
-    if (lane == 0 && p.status) atomicCAS(p.status, 0, static_cast<int>(ST_BAD_ARGUMENT) | (24 << 8));
-    return;
+  const int place0 = start / ps + blockIdx.x * PB_PAGES, pages = min(PB_PAGES, (end - 1) / ps + 1 - place0);
+  if (pages <= 0) return;
+  if (static_cast<int>(threadIdx.x) < pages) {
+    const int page = p.c.page_table[static_cast<size_t>(seq) * p.c.max_pages + place0 + threadIdx.x];
+    const bool there = page >= 0 && page < p.c.num_pages;
+    if (!there && p.status) atomicCAS(p.status, 0, static_cast<int>(ST_BAD_ARGUMENT) | (24 << 8));
+    ids[threadIdx.x] = there ? page : -1;
   }
-  const int rows = min(ps, end - place * ps), pieces = dk / N;
-  const T* k = static_cast<const T*>(p.c.data) + static_cast<size_t>(page) * p.c.kv_heads * ps * (dk + p.c.dv) + static_cast<size_t>(h) * ps * dk;
-  T* lo = static_cast<T*>(p.out) + (static_cast<size_t>(page) * p.c.kv_heads + h) * 2 * dk;
+  __syncthreads();
+  const int pieces = dk / N;
   // lanes along a row: the least power of two that holds it, at most the warp; the others take other rows
   int wide = 1;
   while (wide < pieces && wide < 32) wide *= 2;
   const int col = lane & (wide - 1), r0 = lane / wide, step = 32 / wide;
-  for (int c0 = 0; c0 < pieces; c0 += wide) {
-    const int c = c0 + col;
-    float mn[N], mx[N];
+  for (int unit = threadIdx.x >> 5; unit < pages * p.c.kv_heads; unit += PB_WARPS) {
+    const int at = unit / p.c.kv_heads, h = unit - at * p.c.kv_heads, page = ids[at], rows = min(ps, end - (place0 + at) * ps);
+    if (page < 0) continue;
+    const T* k = static_cast<const T*>(p.c.data) + static_cast<size_t>(page) * p.c.kv_heads * ps * (dk + p.c.dv) + static_cast<size_t>(h) * ps * dk;
+    T* lo = static_cast<T*>(p.out) + (static_cast<size_t>(page) * p.c.kv_heads + h) * 2 * dk;
+    for (int c0 = 0; c0 < pieces; c0 += wide) {
+      const int c = c0 + col;
+      uint32_t mn[WORDS], mx[WORDS];
 #pragma unroll
-    for (int i = 0; i < N; ++i) { mn[i] = INFINITY; mx[i] = -INFINITY; }
-    if (c < pieces) {
-#pragma unroll 8
-      for (int r = r0; r < rows; r += step) {
-        float x[N];
-        if constexpr (VEC) PbVec<T>::first(x, *reinterpret_cast<const uint4*>(k + static_cast<size_t>(r) * dk + c * N));
-        else x[0] = pb_f(k[static_cast<size_t>(r) * dk + c]);
+      for (int i = 0; i < WORDS; ++i) { mn[i] = P::MOST; mx[i] = P::LEAST; }
+      if (c < pieces)
+        for (int r1 = r0; r1 < rows; r1 += BATCH * step) {
+          uint32_t x[BATCH][WORDS];
 #pragma unroll
-        for (int i = 0; i < N; ++i) { mn[i] = pb_min(mn[i], x[i]); mx[i] = pb_max(mx[i], x[i]); }
+          for (int j = 0; j < BATCH; ++j) {
+            // rows behind the end: the first of the batch once more, which changes nothing
+            const T* at_row = k + static_cast<size_t>(r1 + j * step < rows ? r1 + j * step : r1) * dk + c * N;
+            if constexpr (VEC) {
+              const uint4 v = __ldcg(reinterpret_cast<const uint4*>(at_row));
+              x[j][0] = v.x; x[j][1] = v.y; x[j][2] = v.z; x[j][3] = v.w;
+            } else {
+              const typename P::W w = *reinterpret_cast<const typename P::W*>(at_row);
+              x[j][0] = sizeof(T) == 2 ? w * 0x10001u : w;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < BATCH; ++j)
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) { mn[i] = P::lesser(mn[i], x[j][i]); mx[i] = P::larger(mx[i], x[j][i]); }
+        }
+      for (int o = wide; o < 32; o *= 2) {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) {
+          mn[i] = P::lesser(mn[i], __shfl_xor_sync(0xffffffffu, mn[i], o));
+          mx[i] = P::larger(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], o));
+        }
       }
-    }
-    for (int o = wide; o < 32; o *= 2) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        mn[i] = pb_min(mn[i], __shfl_xor_sync(0xffffffffu, mn[i], o));
-        mx[i] = pb_max(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], o));
+      if (c < pieces && r0 == 0) {
+        if constexpr (VEC) {
+          *reinterpret_cast<uint4*>(lo + c * N) = make_uint4(mn[0], mn[1], mn[2], mn[3]);
+          *reinterpret_cast<uint4*>(lo + dk + c * N) = make_uint4(mx[0], mx[1], mx[2], mx[3]);
+        } else {
+          *reinterpret_cast<typename P::W*>(lo + c) = static_cast<typename P::W>(mn[0]);
+          *reinterpret_cast<typename P::W*>(lo + dk + c) = static_cast<typename P::W>(mx[0]);
+        }
       }
-    }
-    if (c < pieces && r0 == 0) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) { pb_put(lo + c * N + i, mn[i]); pb_put(lo + dk + c * N + i, mx[i]); }
     }
   }
 }
@@ -181,10 +200,10 @@ extern "C" int b200_page_bounds(const b200_paged_cache* c, const int* starts, co
   PageBoundsParams p{*c, starts, ends, seq_ids, out, status};
   const long long pages = (static_cast<long long>(max_tokens) + 2 * c->page_size - 2) / c->page_size;
   const long long most = pages < c->max_pages ? pages : c->max_pages;
-  const dim3 grid(static_cast<unsigned>((most * c->kv_heads + PB_WARPS - 1) / PB_WARPS), portions);
+  const dim3 grid(static_cast<unsigned>((most + PB_PAGES - 1) / PB_PAGES), portions);
   const size_t size = c->f32 ? 4 : 2;
   const bool vec = c->dk * size % 16 == 0 && static_cast<size_t>(c->kv_heads) * c->page_size * (c->dk + c->dv) * size % 16 == 0 &&
-                   (reinterpret_cast<uintptr_t>(c->data) & 15) == 0;
+                   ((reinterpret_cast<uintptr_t>(c->data) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
   if (c->f32) return vec ? launch_page_bounds<float, true>(p, grid, stream) : launch_page_bounds<float, false>(p, grid, stream);
   return vec ? launch_page_bounds<__nv_bfloat16, true>(p, grid, stream) : launch_page_bounds<__nv_bfloat16, false>(p, grid, stream);
 }

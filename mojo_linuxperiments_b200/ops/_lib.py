@@ -207,6 +207,15 @@ def stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+def on_device(device: torch.device, fn, *args) -> int:
+    """``fn(*args, stream)`` with ``device`` current: its own current stream, whichever device is current outside."""
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+
+
 LAUNCHES = [0]     # kernels of this library launched (or captured into a CUDA graph) by this process
 
 

@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes
+from array import array
 
 import torch
 
@@ -16,32 +17,37 @@ def copy_pages(caches, src, dst) -> None:
 
     The page numbers are on the host, as those who hand pages out have them.  No page is written twice or read as well as written, so the
     order of the copies does not matter; a captured call copies the same pages in every replay."""
-    arrays = [c.data if isinstance(c, PagedKVCache) else c for c in (caches if isinstance(caches, (list, tuple)) else [caches])]
-    src, dst = [int(p) for p in src], [int(p) for p in dst]
-    if len(src) != len(dst):
-        raise ValueError(f"{len(src)} pages to copy to {len(dst)}")
-    if not src or not arrays:
+    if not isinstance(caches, (list, tuple)):
+        caches = [caches]
+    arrays = [c.data if isinstance(c, PagedKVCache) else c for c in caches]
+    src, dst = array("i", src), array("i", dst)
+    n = len(src)
+    if n != len(dst):
+        raise ValueError(f"{n} pages to copy to {len(dst)}")
+    if not n or not arrays:
         return
     written = set(dst)
-    if len(written) != len(dst) or not written.isdisjoint(src):
+    if len(written) != n or not written.isdisjoint(src):
         raise ValueError("a page is written twice, or written and read")
-    lo, hi = min(min(src), min(written)), max(max(src), max(written))
-    device = arrays[0].device
+    lo, hi, index = min(min(src), min(dst)), max(max(src), max(dst)), arrays[0].get_device()
+    if lo < 0:
+        raise IndexError(f"page {lo}")
+    at, sizes = array("Q"), array("q")
     for a in arrays:
-        if a.device != device or not a.is_cuda or not a.is_contiguous() or a.dim() < 2:
+        if a.get_device() != index or index < 0 or not a.is_contiguous() or a.dim() < 2:
             raise ValueError("records lie in contiguous tensors on one GPU")
-        if lo < 0 or hi >= a.shape[0]:
-            raise IndexError(f"pages {lo} to {hi} of {a.shape[0]}")
-    arrays = [a for a in arrays if a.numel() > 0]
-    if not arrays:
-        return
-    sizes = [a.stride(0) * a.element_size() for a in arrays]
-    if any(n % 16 or a.data_ptr() % 16 for n, a in zip(sizes, arrays)):
-        raise ValueError("records are whole pieces of 16 bytes")
-    n = len(src)
-    with torch.cuda.device(device):
-        rc = _lib.lib().b200_copy_pages((ctypes.c_void_p * len(arrays))(*[a.data_ptr() for a in arrays]), (ctypes.c_longlong * len(arrays))(*sizes),
-                                        len(arrays), (ctypes.c_int * n)(*src), (ctypes.c_int * n)(*dst), n, _lib.stream())
+        records = a.shape[0]
+        if hi >= records:
+            raise IndexError(f"pages {lo} to {hi} of {records}")
+        start, size = a.data_ptr(), a.nbytes // records
+        if size == 0:
+            continue
+        if size % 16 or start % 16:
+            raise ValueError("records are whole pieces of 16 bytes")
+        at.append(start)
+        sizes.append(size)
+    rc = _lib.on_device(arrays[0].device, _lib.lib().b200_copy_pages, at.buffer_info()[0], sizes.buffer_info()[0], len(at), src.buffer_info()[0],
+                        dst.buffer_info()[0], n)
     _lib.check(rc, "copy_pages")
 
 
@@ -51,8 +57,8 @@ def bounds_for(cache: PagedKVCache) -> torch.Tensor:
 
 
 def check_bounds(cache: PagedKVCache, bounds: torch.Tensor) -> None:
-    if tuple(bounds.shape) != (cache.num_pages, cache.kv_heads, 2, cache.dk) or bounds.dtype != cache.data.dtype or not bounds.is_contiguous() \
-            or bounds.device != cache.data.device:
+    if bounds.shape != (cache.num_pages, cache.kv_heads, 2, cache.dk) or bounds.dtype != cache.data.dtype or not bounds.is_contiguous() \
+            or bounds.get_device() != cache.data.get_device():
         raise ValueError(f"bounds {tuple(bounds.shape)} {bounds.dtype} of a cache of {cache.num_pages} pages, {cache.kv_heads} heads of {cache.dk}, {cache.data.dtype}")
 
 
@@ -69,8 +75,7 @@ def page_bounds(cache: PagedKVCache, page_table: torch.Tensor, starts: torch.Ten
             raise ValueError(f"{n} portions of {page_table.shape[0]} sequences")
     else:
         assert seq_ids.dtype == torch.int32 and seq_ids.is_contiguous() and seq_ids.numel() == n
-    with torch.cuda.device(cache.data.device):
-        rc = _lib.lib().b200_page_bounds(ctypes.byref(cache.desc(page_table)), starts.data_ptr(), ends.data_ptr(), _lib.ptr(seq_ids), n, int(max_tokens),
-                                         bounds.data_ptr(), default_workspace(bounds.device).status.data_ptr(), _lib.stream())
+    rc = _lib.on_device(bounds.device, _lib.lib().b200_page_bounds, ctypes.byref(cache.desc(page_table)), starts.data_ptr(), ends.data_ptr(), _lib.ptr(seq_ids),
+                        n, int(max_tokens), bounds.data_ptr(), default_workspace(bounds.device).status.data_ptr())
     _lib.check(rc, "page_bounds")
     return bounds

@@ -6,7 +6,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .attention import PAGE, PagedKVCache, attn_paged, pick_decode_splits_paged
+from .attention import PAGE, PagedKVCache, pick_decode_splits_paged
 from .workspace import default_workspace
 
 KEY_TILE = 128                 # keys of a step of the kernel
@@ -97,8 +97,9 @@ class _Cut:
         if pieces:
             buf[self.pieces_at:self.pieces_at + _PIECE * len(pieces)] = torch.tensor(pieces, dtype=torch.int32).flatten()
             buf[self.slots_at:self.slots_at + len(order)] = torch.tensor(order, dtype=torch.int32)
-        self.plan.copy_(buf, non_blocking=True)
-        done.record()
+        with torch.cuda.device(self.plan.device):
+            self.plan.copy_(buf, non_blocking=True)
+            done.record()
 
 
 class SharedPrefixes:
@@ -135,6 +136,8 @@ class SharedPrefixes:
         key = (hq, cache.kv_heads, cache.dv, device.index)
         cut = self._cuts.get(key)
         if cut is None:
+            if device != self.device and (device.type != self.device.type or self.device.index is not None):
+                raise ValueError(f"a plan for {self.device} and a cache on {device}")
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("the first call with a plan sends it to the device: make one before the capture")
             cut = self._cuts[key] = _Cut(self.num_seqs, hq // cache.kv_heads, cache.kv_heads, cache.dv, device)
@@ -156,19 +159,20 @@ def attn_decode_shared(q: torch.Tensor, hq: int, seq_lens: torch.Tensor, cache: 
     room = page_table.shape[1] * cache.page_size
     if B > page_table.shape[0] or B != shared.num_seqs or shared.longest > room:
         raise ValueError(f"{B} rows, {page_table.shape[0]} sequences of up to {room} tokens, a plan for {shared.num_seqs} with prefixes of up to {shared.longest}")
-    desc = cache.desc(page_table)
-    with torch.cuda.device(q.device):
-        L = _lib.lib()
-        if not L.b200_attn_decode_shared_takes(ctypes.byref(desc), hq, q.stride(0), out.stride(0)) or q.data_ptr() % 16 or out.data_ptr() % 8:
-            return attn_paged(q, hq, None, None, cache, page_table, spec, out, seq_lens=seq_lens)
-        cut = shared.cut_for(hq, cache)
-        if splits is None:
-            keys = min(room - shared.alone, spec.chunk) if spec.chunk > 0 else room - shared.alone
-            splits = pick_decode_splits_paged(B, cache.kv_heads * ((hq // cache.kv_heads + 15) // 16), keys, cut.sms)
-        rc = L.b200_attn_decode_shared(
-            q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), hq, B, seq_lens.data_ptr(), ctypes.byref(desc), ctypes.byref(spec),
-            cut.plan.data_ptr(), cut.pieces_at, cut.slots_at, cut.max_pieces, cut.part.data_ptr(), cut.rows, splits, cut.sms,
-            default_workspace(q.device).status.data_ptr(), _lib.stream())
+    L, desc = _lib.lib(), cache.desc(page_table)
+    if not L.b200_attn_decode_shared_takes(ctypes.byref(desc), hq, q.stride(0), out.stride(0)) or q.data_ptr() % 16 or out.data_ptr() % 8:
+        rc = _lib.on_device(q.device, L.b200_attn_paged, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), hq, B, None, None, seq_lens.data_ptr(),
+                            ctypes.byref(desc), ctypes.byref(spec), default_workspace(q.device).status.data_ptr())
+        _lib.check(rc, "attn_paged")
+        return out
+    cut = shared.cut_for(hq, cache)
+    if splits is None:
+        keys = min(room - shared.alone, spec.chunk) if spec.chunk > 0 else room - shared.alone
+        splits = pick_decode_splits_paged(B, cache.kv_heads * ((hq // cache.kv_heads + 15) // 16), keys, cut.sms)
+    rc = _lib.on_device(
+        q.device, L.b200_attn_decode_shared, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), hq, B, seq_lens.data_ptr(), ctypes.byref(desc),
+        ctypes.byref(spec), cut.plan.data_ptr(), cut.pieces_at, cut.slots_at, cut.max_pieces, cut.part.data_ptr(), cut.rows, splits, cut.sms,
+        default_workspace(q.device).status.data_ptr())
     _lib.check(rc, "attn_decode_shared")
     _lib.LAUNCHES[0] += 1                        # two kernels
     return out

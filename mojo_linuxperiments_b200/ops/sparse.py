@@ -41,7 +41,8 @@ def attn_paged_sparse(q: torch.Tensor, hq: int, positions: torch.Tensor, seq_ids
     assert q.dtype == cache.data.dtype == out.dtype and q.stride(1) == 1 and out.stride(1) == 1 and q.shape[0] == out.shape[0] == M
     assert q.shape[1] >= hq * cache.dk and out.shape[1] >= hq * cache.dv and hq % cache.kv_heads == 0
     assert positions.dtype == page_table.dtype == torch.int32 and page_table.is_contiguous() and positions.is_contiguous()
-    assert all(t is None or (t.dtype == torch.int32 and t.is_contiguous() and t.numel() == M) for t in (seq_ids, seq_lens))
+    for t in (seq_ids, seq_lens):
+        assert t is None or (t.dtype == torch.int32 and t.is_contiguous() and t.numel() == M)
     if max(cache.dk, cache.dv) > MAX_HEAD_DIM or cache.dv == 0:
         raise ValueError(f"heads of {cache.dk} and {cache.dv}")
     if seq_ids is None and M > page_table.shape[0]:
@@ -53,11 +54,10 @@ def attn_paged_sparse(q: torch.Tensor, hq: int, positions: torch.Tensor, seq_ids
         seen = min(most, spec.chunk // cache.page_size + 2) if spec.chunk > 0 else most
         splits = pick_sparse_splits(M * cache.kv_heads * ((hq // cache.kv_heads + 15) // 16), min(top, seen), _lib.num_sms(q.device.index))
     scores = torch.empty(M * cache.kv_heads * most, dtype=torch.int32, device=q.device)
-    with torch.cuda.device(q.device):
-        rc = _lib.lib().b200_attn_paged_sparse(
-            q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), hq, M, positions.data_ptr(), _lib.ptr(seq_ids), _lib.ptr(seq_lens),
-            ctypes.byref(cache.desc(page_table)), bounds.data_ptr(), ctypes.byref(spec), int(top), int(first), int(last), splits, scores.data_ptr(),
-            _lib.ptr(chosen), default_workspace(q.device).status.data_ptr(), _lib.stream())
+    rc = _lib.on_device(
+        q.device, _lib.lib().b200_attn_paged_sparse, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), hq, M, positions.data_ptr(), _lib.ptr(seq_ids),
+        _lib.ptr(seq_lens), ctypes.byref(cache.desc(page_table)), bounds.data_ptr(), ctypes.byref(spec), int(top), int(first), int(last), splits,
+        scores.data_ptr(), _lib.ptr(chosen), default_workspace(q.device).status.data_ptr())
     _lib.check(rc, "attn_paged_sparse")
     _lib.LAUNCHES[0] += 1                        # two kernels
     return out
