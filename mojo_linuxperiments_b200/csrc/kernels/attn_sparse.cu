@@ -26,53 +26,88 @@ __device__ __forceinline__ float as_max(float a, float b) { float r; asm("max.Na
 // =====================================================================================================================================
 constexpr int SC_WARPS = 8, SC_THREADS = 32 * SC_WARPS;
 
-// ---- any head size, bf16 or fp32: a warp per page, lanes along the dimensions, the queries in shared memory ------------------------------
-constexpr int SCA_PAGES = 4 * SC_WARPS;
-constexpr int AS_MAX_D = 512, AS_PER_LANE = AS_MAX_D / 32;
+// ---- any head size, bf16 or fp32: four pages per warp, lanes along the dimensions, the queries in shared memory -------------------------
+constexpr int SCA_EACH = 4, SCA_PAGES = SCA_EACH * SC_WARPS;
+constexpr int AS_MAX_D = 512, AS_RUNS = AS_MAX_D / 128;      // dimensions 128 at a time: four for a lane
 
-template <typename T>
+// elements d .. d + 3 of a row of n, zeros behind it; VEC: rows are whole fours of elements that lie on as many bytes
+template <bool VEC, typename T>
+__device__ __forceinline__ float4 as_f4(const T* row, int d, int n) {
+  if constexpr (VEC) {
+    if (d >= n) return make_float4(0.f, 0.f, 0.f, 0.f);
+    if constexpr (sizeof(T) == 4) return __ldcg(reinterpret_cast<const float4*>(row + d));
+    else {
+      const uint2 r = __ldcg(reinterpret_cast<const uint2*>(row + d));
+      return make_float4(__uint_as_float(r.x << 16), __uint_as_float(r.x & 0xffff0000u), __uint_as_float(r.y << 16), __uint_as_float(r.y & 0xffff0000u));
+    }
+  }
+  return make_float4(d < n ? as_f(row[d]) : 0.f, d + 1 < n ? as_f(row[d + 1]) : 0.f, d + 2 < n ? as_f(row[d + 2]) : 0.f, d + 3 < n ? as_f(row[d + 3]) : 0.f);
+}
+__device__ __forceinline__ int as_padded(int d) { return (d + 127) & ~127; }
+
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(SC_THREADS) page_scores_any_kernel(const __grid_constant__ SparseParams p) {
-  extern __shared__ __align__(16) float sc_q[];      // [heads of the group][dk]
+  extern __shared__ __align__(16) float sc_q[];      // [heads of the group][dk, zeros up to whole 128]
   pdl_wait();
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tok = blockIdx.z, kvh = blockIdx.y;
-  const int group = p.hq / p.c.kv_heads, dk = p.c.dk;
+  const int group = p.hq / p.c.kv_heads, dk = p.c.dk, wide = as_padded(dk);
   SparseRow row;
   if (!row.find(p, tok) || !row.selects || static_cast<int>(blockIdx.x) * SCA_PAGES >= row.candidates) return;
   const T* q = static_cast<const T*>(p.q) + static_cast<size_t>(tok) * p.ldq + static_cast<size_t>(kvh) * group * dk;
-  for (int i = threadIdx.x; i < group * dk; i += SC_THREADS) sc_q[i] = as_f(q[i]);
+  for (int i = threadIdx.x; i < group * wide; i += SC_THREADS) {
+    const int h = i / wide, d = i - h * wide;
+    sc_q[i] = d < dk ? as_f(q[static_cast<size_t>(h) * dk + d]) : 0.f;
+  }
   __syncthreads();
-  const int* pt = p.c.page_table + static_cast<size_t>(row.seq) * p.c.max_pages + row.place0;
-  unsigned* to = p.scores + (static_cast<size_t>(tok) * p.c.kv_heads + kvh) * p.c.max_pages;
-  for (int i = blockIdx.x * SCA_PAGES + warp; i < min(row.candidates, static_cast<int>(blockIdx.x + 1) * SCA_PAGES); i += SC_WARPS) {
-    const int page = pt[i];
-    float s = -INFINITY;
-    if (page >= 0 && page < p.c.num_pages) {
-      const T* lo = static_cast<const T*>(p.bounds) + (static_cast<size_t>(page) * p.c.kv_heads + kvh) * 2 * dk;
-      float a[AS_PER_LANE], b[AS_PER_LANE];
+  const int i0 = blockIdx.x * SCA_PAGES + warp * SCA_EACH, n = min(row.candidates - i0, SCA_EACH);
+  if (n <= 0) return;
+  const int* pt = p.c.page_table + static_cast<size_t>(row.seq) * p.c.max_pages + row.place0 + i0;
+  const T* lo[SCA_EACH];
+  bool there[SCA_EACH];
+  float s[SCA_EACH];
 #pragma unroll
-      for (int j = 0; j < AS_PER_LANE; ++j) {
-        const int d = lane + 32 * j;
-        a[j] = d < dk ? as_f(lo[d]) : 0.f;
-        b[j] = d < dk ? as_f(lo[dk + d]) : 0.f;
-      }
-      for (int h = 0; h < group; ++h) {
-        float t = 0.f;
+  for (int j = 0; j < SCA_EACH; ++j) {
+    const int page = j < n ? pt[j] : -1;
+    there[j] = page >= 0 && page < p.c.num_pages;
+    lo[j] = static_cast<const T*>(p.bounds) + (static_cast<size_t>(there[j] ? page : 0) * p.c.kv_heads + kvh) * 2 * dk;
+    s[j] = -INFINITY;
+  }
+  // four heads at a time, so that the bounds are read once for them
+  for (int h0 = 0; h0 < group; h0 += 4) {
+    float t[SCA_EACH][4] = {};
+    for (int d0 = 0; d0 < dk; d0 += 128) {
+      float4 a[SCA_EACH], b[SCA_EACH];
 #pragma unroll
-        for (int j = 0; j < AS_PER_LANE; ++j) {
-          const int d = lane + 32 * j;
-          if (d < dk) {
-            const float x = sc_q[h * dk + d];
-            t = fmaf(fmaxf(x, 0.f), b[j], fmaf(fminf(x, 0.f), a[j], t));
-          }
+      for (int j = 0; j < SCA_EACH; ++j) { a[j] = as_f4<VEC>(lo[j], d0 + 4 * lane, dk); b[j] = as_f4<VEC>(lo[j] + dk, d0 + 4 * lane, dk); }
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        if (h0 + h >= group) break;
+        const float4 x = *reinterpret_cast<const float4*>(sc_q + (h0 + h) * wide + d0 + 4 * lane);
+#pragma unroll
+        for (int j = 0; j < SCA_EACH; ++j) {
+          float u = fmaf(fmaxf(x.x, 0.f), b[j].x, fmaf(fminf(x.x, 0.f), a[j].x, t[j][h]));
+          u = fmaf(fmaxf(x.y, 0.f), b[j].y, fmaf(fminf(x.y, 0.f), a[j].y, u));
+          u = fmaf(fmaxf(x.z, 0.f), b[j].z, fmaf(fminf(x.z, 0.f), a[j].z, u));
+          t[j][h] = fmaf(fmaxf(x.w, 0.f), b[j].w, fmaf(fminf(x.w, 0.f), a[j].w, u));
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-        s = as_max(s, t);
       }
     }
-    if (lane == 0) to[i] = ps_order(s);
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      if (h0 + h >= group) break;
+#pragma unroll
+      for (int j = 0; j < SCA_EACH; ++j) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) t[j][h] += __shfl_xor_sync(0xffffffffu, t[j][h], o);
+        s[j] = as_max(s[j], t[j][h]);
+      }
+    }
   }
+  unsigned* to = p.scores + (static_cast<size_t>(tok) * p.c.kv_heads + kvh) * p.c.max_pages + i0;
+#pragma unroll
+  for (int j = 0; j < SCA_EACH; ++j)
+    if (lane == j && j < n) to[j] = ps_order(there[j] ? s[j] : -INFINITY);
 }
 
 // ---- bf16, head sizes up to 128: tensor cores ----------------------------------------------------------------------------------------------
@@ -199,8 +234,10 @@ __device__ __forceinline__ void sparse_nothing(const SparseParams& p, int tok, i
 }
 
 // ---- any head size, bf16 or fp32 ------------------------------------------------------------------------------------------------------------
-// A head at a time, 16 keys per warp: two lanes per key for the scores, then the lanes along the dimensions of the values.
-template <typename T>
+// A warp takes 16 keys of a page for four heads at a time, lanes along the dimensions: all rows of the keys, then of the values, are on their way at once.
+constexpr int ASA_HEADS = 4;
+
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(PS_THREADS) attn_sparse_any_kernel(const __grid_constant__ SparseParams p) {
   extern __shared__ __align__(16) uint8_t as_smem[];
   __shared__ PageSelectShared sel;
@@ -210,94 +247,131 @@ __global__ void __launch_bounds__(PS_THREADS) attn_sparse_any_kernel(const __gri
   const int rank = blockIdx.x, S = p.splits, tok = blockIdx.z;
   const int kvh = blockIdx.y / p.hgroups, hg = blockIdx.y - kvh * p.hgroups;
   const int group = p.hq / p.c.kv_heads, g0 = hg * 16, G = min(16, group - g0), h0 = kvh * group + g0;
-  const int dk = p.c.dk, dv = p.c.dv, ps = p.c.page_size;
+  const int dk = p.c.dk, dv = p.c.dv, ps = p.c.page_size, wide = as_padded(dk), pitch = as_padded(dv) + 4;
   SparseRow row;
   if (!row.find(p, tok)) { sparse_nothing<T>(p, tok, kvh, hg, h0, G, rank); return; }      // the same for all CTAs of the cluster
   const T* q = static_cast<const T*>(p.q) + static_cast<size_t>(tok) * p.ldq + static_cast<size_t>(h0) * dk;
   const int* pt = p.c.page_table + static_cast<size_t>(row.seq) * p.c.max_pages;
-  // [8 warps][dv + 2], [16 heads][dv + 2], queries [16][dk], scores, list
-  const int pitch = dv + 2;
+  // [8 warps][4 heads][pitch], [16 heads][pitch] (the last four of a row: m, l), queries [16][wide], scores, list
   float* part = reinterpret_cast<float*>(as_smem);
-  float* joined = part + PS_WARPS * pitch;
+  float* joined = part + PS_WARPS * ASA_HEADS * pitch;
   float* qs = joined + 16 * pitch;
-  unsigned* room = reinterpret_cast<unsigned*>(qs + 16 * dk);
+  unsigned* room = reinterpret_cast<unsigned*>(qs + 16 * wide);
   int* list = reinterpret_cast<int*>(room + p.score_cap);
-  for (int i = tid; i < G * dk; i += PS_THREADS) qs[i] = as_f(q[i]);
+  for (int i = tid; i < 16 * wide; i += PS_THREADS) {
+    const int h = i / wide, d = i - h * wide;
+    qs[i] = h < G && d < dk ? as_f(q[static_cast<size_t>(h) * dk + d]) : 0.f;
+  }
   const int share = row.lists(p, sel, room, tok, kvh, rank, S, list);
   __syncthreads();
   if (p.chosen && hg == 0) row.tell(p, tok, kvh, rank, share, list, S);
 
   const size_t rec = static_cast<size_t>(p.c.kv_heads) * ps * (dk + dv);
   const int per = (ps + 15) / 16;                // runs of 16 keys of a page
-  for (int g = 0; g < G; ++g) {
-    const float* qh = qs + g * dk;
-    float m = -INFINITY, l = 0.f, acc[AS_PER_LANE];
+  for (int g4 = 0; g4 < G; g4 += ASA_HEADS) {
+    float m[ASA_HEADS], l[ASA_HEADS];
+    float4 acc[ASA_HEADS][AS_RUNS];
 #pragma unroll
-    for (int j = 0; j < AS_PER_LANE; ++j) acc[j] = 0.f;
+    for (int h = 0; h < ASA_HEADS; ++h) {
+      m[h] = -INFINITY; l[h] = 0.f;
+#pragma unroll
+      for (int j = 0; j < AS_RUNS; ++j) acc[h][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
     for (int i = warp; i < share * per; i += PS_WARPS) {
       const int place = list[i / per], page = pt[place];
       if (page < 0 || page >= p.c.num_pages) {
         if (lane == 0 && p.status) atomicCAS(p.status, 0, static_cast<int>(ST_BAD_ARGUMENT) | (25 << 8));
         continue;
       }
-      const int k0 = i % per * 16, r0 = max(0, row.low - place * ps), r1 = min(ps, row.pos + 1 - place * ps), key = k0 + (lane >> 1);
-      const bool on = key >= r0 && key < r1;
-      const T* kp = static_cast<const T*>(p.c.data) + static_cast<size_t>(page) * rec + (static_cast<size_t>(kvh) * ps + (on ? key : r0)) * dk;
-      const T* vp = static_cast<const T*>(p.c.data) + static_cast<size_t>(page) * rec + static_cast<size_t>(p.c.kv_heads) * ps * dk + (static_cast<size_t>(kvh) * ps + k0) * dv;
-      float t0 = 0.f, t1 = 0.f;
-      const int half = ((dk + 7) / 8) * 4, d0 = (lane & 1) * half, d1 = min(dk, d0 + half);
-      int d = d0;
-#pragma unroll 4
-      for (; d + 4 <= d1; d += 4) {
-        t0 = fmaf(qh[d], as_f(kp[d]), t0); t1 = fmaf(qh[d + 1], as_f(kp[d + 1]), t1);
-        t0 = fmaf(qh[d + 2], as_f(kp[d + 2]), t0); t1 = fmaf(qh[d + 3], as_f(kp[d + 3]), t1);
+      const int k0 = i % per * 16, r0 = max(0, row.low - place * ps), r1 = min(ps, row.pos + 1 - place * ps);
+      if (k0 >= r1 || k0 + 16 <= r0) continue;
+      const T* kp = static_cast<const T*>(p.c.data) + static_cast<size_t>(page) * rec + static_cast<size_t>(kvh) * ps * dk;
+      const T* vp = static_cast<const T*>(p.c.data) + static_cast<size_t>(page) * rec + static_cast<size_t>(p.c.kv_heads) * ps * dk + static_cast<size_t>(kvh) * ps * dv;
+      auto seen = [&](int r) { return k0 + r >= r0 && k0 + r < r1; };
+      float s[ASA_HEADS] = {};                   // of key lane / 2
+      for (int d0 = 0; d0 < dk; d0 += 128) {
+        float4 k[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) k[r] = as_f4<VEC>(kp + static_cast<size_t>(seen(r) ? k0 + r : max(k0, r0)) * dk, d0 + 4 * lane, dk);
+#pragma unroll
+        for (int h = 0; h < ASA_HEADS; ++h) {
+          if (g4 + h >= G) break;
+          const float4 x = *reinterpret_cast<const float4*>(qs + (g4 + h) * wide + d0 + 4 * lane);
+          // sixteen sums over the lanes: half of what is left goes to the partner each time
+          float t[16];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) t[r] = fmaf(x.x, k[r].x, fmaf(x.y, k[r].y, fmaf(x.z, k[r].z, x.w * k[r].w)));
+#pragma unroll
+          for (int o = 16, half = 8; o > 1; o >>= 1, half >>= 1)
+#pragma unroll
+            for (int r = 0; r < half; ++r) {
+              const bool upper = lane & o;
+              const float mine = upper ? t[r + half] : t[r], other = upper ? t[r] : t[r + half];
+              t[r] = mine + __shfl_xor_sync(0xffffffffu, other, o);
+            }
+          s[h] += t[0] + __shfl_xor_sync(0xffffffffu, t[0], 1);
+        }
       }
-      for (; d < d1; ++d) t0 = fmaf(qh[d], as_f(kp[d]), t0);
-      float s = t0 + t1;
-      s += __shfl_xor_sync(0xffffffffu, s, 1);
-      s = on ? s * p.s.scale : -INFINITY;
-      float mx = s;
+      float e[ASA_HEADS], a[ASA_HEADS];
 #pragma unroll
-      for (int o = 16; o > 1; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      const float mn = fmaxf(m, mx);
-      if (mn == -INFINITY) continue;
-      const float a = m == -INFINITY ? 0.f : expf(m - mn), e = s == -INFINITY ? 0.f : expf(s - mn);
-      float sum = e;
+      for (int h = 0; h < ASA_HEADS; ++h) {
+        const float x = seen(lane >> 1) ? s[h] * p.s.scale : -INFINITY;
+        float mx = x;
 #pragma unroll
-      for (int o = 16; o > 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      l = l * a + sum;
-      m = mn;
+        for (int o = 16; o > 1; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const float mn = fmaxf(m[h], mx), use = mn == -INFINITY ? 0.f : mn;
+        a[h] = m[h] == -INFINITY ? 0.f : expf(m[h] - use);
+        e[h] = x == -INFINITY ? 0.f : expf(x - use);
+        float sum = e[h];
 #pragma unroll
-      for (int j = 0; j < AS_PER_LANE; ++j) {
-        if (32 * j >= dv) break;
-        const int x = lane + 32 * j;
-        float v[16], t = 0.f;
+        for (int o = 16; o > 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        l[h] = l[h] * a[h] + sum;
+        m[h] = mn;
+      }
 #pragma unroll
-        for (int r = 0; r < 16; ++r) v[r] = x < dv && k0 + r >= r0 && k0 + r < r1 ? as_f(vp[static_cast<size_t>(r) * dv + x]) : 0.f;
+      for (int j = 0; j < AS_RUNS; ++j) {
+        if (128 * j >= dv) break;
+        float4 v[16];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) t = fmaf(__shfl_sync(0xffffffffu, e, 2 * r), v[r], t);
-        acc[j] = fmaf(acc[j], a, t);
+        for (int r = 0; r < 16; ++r) v[r] = seen(r) ? as_f4<VEC>(vp + static_cast<size_t>(k0 + r) * dv, 128 * j + 4 * lane, dv) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int h = 0; h < ASA_HEADS; ++h) {
+          if (g4 + h >= G) break;
+          float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float w = __shfl_sync(0xffffffffu, e[h], 2 * r);
+            t.x = fmaf(w, v[r].x, t.x); t.y = fmaf(w, v[r].y, t.y); t.z = fmaf(w, v[r].z, t.z); t.w = fmaf(w, v[r].w, t.w);
+          }
+          float4& c = acc[h][j];
+          c.x = fmaf(c.x, a[h], t.x); c.y = fmaf(c.y, a[h], t.y); c.z = fmaf(c.z, a[h], t.z); c.w = fmaf(c.w, a[h], t.w);
+        }
       }
     }
-    float* mine = part + warp * pitch;
-    if (lane == 0) { mine[dv] = m; mine[dv + 1] = l; }
 #pragma unroll
-    for (int j = 0; j < AS_PER_LANE; ++j)
-      if (lane + 32 * j < dv) mine[lane + 32 * j] = acc[j];
+    for (int h = 0; h < ASA_HEADS; ++h) {
+      float* mine = part + (warp * ASA_HEADS + h) * pitch;
+#pragma unroll
+      for (int j = 0; j < AS_RUNS; ++j)
+        if (128 * j < dv) *reinterpret_cast<float4*>(mine + 128 * j + 4 * lane) = acc[h][j];
+      if (lane == 0) { mine[pitch - 4] = m[h]; mine[pitch - 3] = l[h]; }
+    }
     __syncthreads();
-    float* to = joined + g * pitch;
-    float top = -INFINITY, f[PS_WARPS];
+    for (int i = tid; i < min(ASA_HEADS, G - g4) * (dv + 1); i += PS_THREADS) {      // the last of a head: the sums of its weights
+      const int h = i / (dv + 1), d = i - h * (dv + 1);
+      float top = -INFINITY, v = 0.f;
 #pragma unroll
-    for (int w = 0; w < PS_WARPS; ++w) top = fmaxf(top, part[w * pitch + dv]);
+      for (int w = 0; w < PS_WARPS; ++w) top = fmaxf(top, part[(w * ASA_HEADS + h) * pitch + pitch - 4]);
+      const float use = top == -INFINITY ? 0.f : top;
 #pragma unroll
-    for (int w = 0; w < PS_WARPS; ++w) f[w] = part[w * pitch + dv] == -INFINITY ? 0.f : expf(part[w * pitch + dv] - top);
-    for (int d = tid; d <= dv; d += PS_THREADS) {            // the last: the sums of the weights
-      float v = 0.f;
-#pragma unroll
-      for (int w = 0; w < PS_WARPS; ++w) v = fmaf(f[w], part[w * pitch + d + (d == dv)], v);
-      to[d + (d == dv)] = v;
+      for (int w = 0; w < PS_WARPS; ++w) {
+        const float* x = part + (w * ASA_HEADS + h) * pitch;
+        v = fmaf(expf(x[pitch - 4] - use), d < dv ? x[d] : x[pitch - 3], v);
+      }
+      float* to = joined + (g4 + h) * pitch;
+      if (d < dv) to[d] = v;
+      else { to[pitch - 4] = top; to[pitch - 3] = v; }
     }
-    if (tid == 0) to[dv] = top;
     __syncthreads();
   }
   if (S > 1) cluster_sync_all();
@@ -308,10 +382,10 @@ __global__ void __launch_bounds__(PS_THREADS) attn_sparse_any_kernel(const __gri
     float m = p.s.sink ? p.s.sink[h0 + g] : -INFINITY, l = p.s.sink ? 1.f : 0.f, v = 0.f;
     for (int r = 0; r < S; ++r) {
       const uint32_t base = (S > 1 ? mapa_shared(j_addr, r) : j_addr) + 4u * (g * pitch);
-      const float mr = dw_ld_cluster(base + 4u * dv);
+      const float mr = dw_ld_cluster(base + 4u * (pitch - 4));
       if (mr == -INFINITY) continue;
       const float mn = fmaxf(m, mr), fo = m == -INFINITY ? 0.f : expf(m - mn), fn = expf(mr - mn);
-      l = l * fo + fn * dw_ld_cluster(base + 4u * (dv + 1));
+      l = l * fo + fn * dw_ld_cluster(base + 4u * (pitch - 3));
       v = v * fo + fn * dw_ld_cluster(base + 4u * d);
       m = mn;
     }
@@ -463,13 +537,20 @@ static void fit_scores(SparseParams& p, size_t floats) {
   p.score_cap = static_cast<int>(most < room ? most : room & ~size_t(3));
 }
 
-template <typename T>
-static int launch_sparse_any(SparseParams p, cudaStream_t stream) {
-  const size_t floats = static_cast<size_t>(PS_WARPS + 16) * (p.c.dv + 2) + 16 * static_cast<size_t>(p.c.dk);
+template <typename T, bool VEC>
+static int launch_sparse_any_as(SparseParams p, cudaStream_t stream) {
+  const size_t wide = (static_cast<size_t>(p.c.dk) + 127) & ~size_t(127), pitch = ((static_cast<size_t>(p.c.dv) + 127) & ~size_t(127)) + 4;
+  const size_t floats = (PS_WARPS * ASA_HEADS + 16) * pitch + 16 * wide;
   fit_scores(p, floats);
   const dim3 grid((p.c.max_pages + SCA_PAGES - 1) / SCA_PAGES, p.c.kv_heads, p.M);
-  return launch_sparse_pair<page_scores_any_kernel<T>, attn_sparse_any_kernel<T>>(grid, 4 * static_cast<size_t>(p.hq / p.c.kv_heads) * p.c.dk,
-                                                                                 4 * (floats + p.list_cap + p.score_cap), p, stream);
+  return launch_sparse_pair<page_scores_any_kernel<T, VEC>, attn_sparse_any_kernel<T, VEC>>(grid, 4 * static_cast<size_t>(p.hq / p.c.kv_heads) * wide,
+                                                                                           4 * (floats + p.list_cap + p.score_cap), p, stream);
+}
+
+template <typename T>
+static int launch_sparse_any(const SparseParams& p, cudaStream_t stream) {
+  const bool vec = p.c.dk % 4 == 0 && p.c.dv % 4 == 0 && (reinterpret_cast<uintptr_t>(p.c.data) | reinterpret_cast<uintptr_t>(p.bounds)) % (4 * sizeof(T)) == 0;
+  return vec ? launch_sparse_any_as<T, true>(p, stream) : launch_sparse_any_as<T, false>(p, stream);
 }
 
 template <int DK, int DV, int NH, bool FULL>

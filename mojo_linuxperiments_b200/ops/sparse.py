@@ -13,11 +13,11 @@ from .workspace import default_workspace
 MAX_HEAD_DIM = 512
 
 
-def pick_sparse_splits(pairs: int, pages: int, num_sms: int = 148) -> int:
-    """CTAs (one cluster of up to eight) per row and group of heads, which share ``pages`` pages: as many as still make one wave of one per SM, with 16
-    pages, two for a warp, each."""
+def pick_sparse_splits(pairs: int, pages: int, num_sms: int = 148, least: int = 16) -> int:
+    """CTAs (one cluster of up to eight) per row and group of heads, which share ``pages`` pages: as many as still make one wave of one per SM, with
+    ``least`` pages (16: two for a warp) each."""
     s = 1
-    while s < 8 and pairs * s * 2 <= num_sms and pages // (2 * s) >= 16:
+    while s < 8 and pairs * s * 2 <= num_sms and pages // (2 * s) >= least:
         s *= 2
     return s
 
@@ -52,7 +52,8 @@ def attn_paged_sparse(q: torch.Tensor, hq: int, positions: torch.Tensor, seq_ids
     most = page_table.shape[1]
     if splits is None:
         seen = min(most, spec.chunk // cache.page_size + 2) if spec.chunk > 0 else most
-        splits = pick_sparse_splits(M * cache.kv_heads * ((hq // cache.kv_heads + 15) // 16), min(top, seen), _lib.num_sms(q.device.index))
+        splits = pick_sparse_splits(M * cache.kv_heads * ((hq // cache.kv_heads + 15) // 16), min(top, seen), _lib.num_sms(q.device.index),
+                                    16 if q.dtype == torch.bfloat16 else 4)
     scores = torch.empty(M * cache.kv_heads * most, dtype=torch.int32, device=q.device)
     rc = _lib.on_device(
         q.device, _lib.lib().b200_attn_paged_sparse, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), hq, M, positions.data_ptr(), _lib.ptr(seq_ids),
