@@ -31,6 +31,10 @@ class Engine:
         family = family_of(cfg)
         self.cfg = cfg
         self.rt = rt or RuntimeConfig()
+        if self.rt.share_prefix and self.rt.sparse_pages:
+            raise ValueError("decoding reads shared prefixes once or selected pages, not both")
+        if self.rt.sparse_pages < 0 or 0 < self.rt.sparse_pages < 3:
+            raise ValueError(f"{self.rt.sparse_pages} pages: the first and the last two are among those attended to")
         self.comm = comm or Comm.single()
         self.device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
         # where this rank runs (host thread pinned beside its GPU) and where its long-lived buffers live (HBM arena)
@@ -125,7 +129,7 @@ class Engine:
         r = self.runtime.report()
         if self.kv is not None:
             r["kv_pages"] = {"total": self.kv.num_pages - 1, "in_use": self.kv.pages_in_use(), "high_water": self.kv.pages_high_water,
-                             "page_tokens": self.kv.page_size}
+                             "page_tokens": self.kv.page_size, "shared": len(self.kv._sharers)}
         return r
 
     def prefill(self, prompts, use_graph: bool = True) -> torch.Tensor:
@@ -384,6 +388,35 @@ class Engine:
         self._set_len(slot, S)
         self._host_len = max(self._lens)
         return self.tokens[slot:slot + 1].clone()
+
+    def fork_sequence(self, slot: int, to) -> None:
+        """Between two decode steps: the slots ``to`` (empty, or whose sequences are finished) continue the sequence in ``slot`` from where it is, each on its own
+        from now on.  Full pages are shared, the last one is copied; the next token is the same for all of them until the caller says otherwise (``step``,
+        ``step_from_host``).  With ``rt.share_prefix`` decoding reads what they share once."""
+        to = [int(t) for t in to]
+        if not 0 <= slot < self.batch or any(not 0 <= t < self.batch for t in to):
+            raise IndexError(f"slot {slot} to {to} of a batch of {self.batch}")
+        n = self._lens[slot]
+        if n < 1 or slot in to or len(set(to)) != len(to):
+            raise ValueError(f"a sequence of {n} tokens from slot {slot} to {to}")
+        if not to:
+            return
+        self.kv.fork(slot, to, n)
+        self.kv.flush()
+        at = torch.tensor(to, dtype=torch.int64).to(self.device, non_blocking=True)
+        for t in (self.tokens, self.positions, self.kv.seq_lens):
+            t.index_copy_(0, at, t[slot:slot + 1].repeat(len(to)))
+        self.active.index_fill_(0, at, 1)
+        for t in to:
+            self._active_host[t] = 1
+            self._set_len(t, n)
+        self._host_len = max(self._lens)
+
+    def compact_cache(self) -> int:
+        """Between two decode steps: move the pages in use to the front of the pool (one launch per 64 layers); how many were moved."""
+        n = self.kv.compact()
+        self.kv.flush()
+        return n
 
     def release_sequence(self, slot: int) -> None:
         """The sequence in ``slot`` is finished: its pages go back to the free list, and the slot stays in the batch as

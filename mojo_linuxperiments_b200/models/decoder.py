@@ -14,10 +14,13 @@ import torch
 from ..ops import attention as A
 from ..ops import linear as L
 from ..ops.moe import ExpertSum
+from ..ops.shared import attn_decode_shared
+from ..ops.sparse import attn_paged_sparse
 from ..parallel.comm import Comm
 from ..utils.trace import op_range
 from .config import ModelConfig, RuntimeConfig, kv_heads_per_rank
 from .kvcache import KVState
+from .mixers import portion_spans
 
 
 def own_last_rows(last_idx: torch.Tensor, a: int, b: int):
@@ -89,8 +92,21 @@ class Decoder:
             q = A.rope_kv_write(qkv, positions, self.cos, self.sin, self.hq, self.hkv, k_out=k_rot, cache=cache,
                                 page_table=kv.page_table, seq_ids=seq_ids, q_norm_w=W.get("q_norm"),
                                 k_norm_w=W.get("k_norm"), eps=self.cfg.eps)
+            if kv.bounds[l] is not None:
+                if l == 0:
+                    self._spans = portion_spans(positions, cu_seqlens, seq_ids)
+                kv.note_keys(l, *self._spans, max_len)
             v = qkv.view(M, self.hq + 2 * self.hkv, self.cfg.head_dim)[:, self.hq + self.hkv:]
             return A.attn_prefill(q, k_rot, v, cu_seqlens, max_len, scale=self.scale)
+        if kv.bounds[l] is not None or kv.shared is not None:
+            q = A.rope_kv_write(qkv, positions, self.cos, self.sin, self.hq, self.hkv, cache=cache, page_table=kv.page_table, seq_ids=None,
+                                q_norm_w=W.get("q_norm"), k_norm_w=W.get("k_norm"), eps=self.cfg.eps).view(M, -1)
+            out, spec = torch.empty_like(q), A.attn_spec(self.scale)
+            if kv.bounds[l] is None:
+                return attn_decode_shared(q, self.hq, kv.seq_lens, cache, kv.page_table, kv.shared, spec, out)
+            kv.note_keys(l, positions, kv.seq_lens, None, 1)
+            return attn_paged_sparse(q, self.hq, positions, None, cache, kv.page_table, kv.bounds[l], spec, out, top=self.rt.sparse_pages,
+                                     seq_lens=kv.seq_lens)
         impl = A.decode_impl(cache.page_size, self.hq // self.hkv)
         if impl in ("tc", "tcp"):
             splits = A.pick_decode_splits_tc(M, self.hkv, kv.page_table.shape[1] * cache.page_size,

@@ -74,7 +74,7 @@ class LayeredDecoder:
         and length of every portion on the host (None: whole prompts).  ``last_idx`` may be empty: the call then only fills
         the cache and returns None."""
         cfg = self.cfg
-        call = X.Call(mode, positions, kv, cu_seqlens, max_len, seq_ids, portions)
+        call = X.Call(mode, positions, kv, cu_seqlens, max_len, seq_ids, portions, sparse_pages=self.rt.sparse_pages)
         s = self.stream(self, token_ids, call)
         for r, run in enumerate(self.runs):
             W, mlp = self.w["layers"][run.layer], cfg.layers[run.layer].mlp

@@ -12,6 +12,8 @@ from ..ops import attention as A
 from ..ops import dense as D
 from ..ops import latent as LT
 from ..ops import recurrent as R
+from ..ops.shared import attn_decode_shared
+from ..ops.sparse import attn_paged_sparse
 from .kvcache import KVState
 from .layered_config import AttentionSpec, LatentSpec, MinGRUSpec
 
@@ -26,7 +28,9 @@ class Call:
     max_len: int = 0
     seq_ids: torch.Tensor | None = None
     portions: list | None = None           # host: (first position, tokens) of every portion; None: all start at 0
+    sparse_pages: int = 0                  # pages that decoding attends to; 0: all
     _context: tuple | None = None
+    _spans: tuple | None = None
 
     @property
     def decode(self) -> bool:
@@ -56,6 +60,22 @@ class Call:
         return self._context
 
 
+    @property
+    def spans(self):
+        """First and end position of every portion and its sequence, on the device (made once per call)."""
+        if self.decode:
+            return self.positions, self.kv.seq_lens, None
+        if self._spans is None:
+            self._spans = portion_spans(self.positions, self.cu_seqlens, self.seq_ids)
+        return self._spans
+
+
+def portion_spans(positions: torch.Tensor, cu_seqlens: torch.Tensor, seq_ids: torch.Tensor):
+    first = cu_seqlens[:-1].to(torch.int64)
+    starts = positions.index_select(0, first)
+    return starts, starts + (cu_seqlens[1:] - cu_seqlens[:-1]), seq_ids.index_select(0, first)
+
+
 class Attention:
     """Grouped heads over keys and values: rotary embedding, chunk mask, sink, output gate."""
 
@@ -69,9 +89,16 @@ class Attention:
         g0 = (m.heads + m.kv_heads) * m.dk + m.kv_heads * m.dv
         spec = A.attn_spec(m.scale, chunk=m.chunk, sink=W["sink"], gate=qkvg[:, g0:g0 + m.heads])
         out = D.rows(qkvg.shape[0], m.heads * m.dv, self.dtype, qkvg.device)
-        if c.decode:
+        bounds = c.kv.bounds[run]
+        if c.decode and bounds is None and c.kv.shared is None:
             return A.attn_decode_paged(qkvg, m.heads, c.positions, c.kv.seq_lens, self.cos, self.sin, cache, c.kv.page_table, spec, out)
         A.rotary_paged(qkvg, m.heads, c.positions, c.seq_ids, self.cos, self.sin, cache, c.kv.page_table)
+        if bounds is not None:
+            c.kv.note_keys(run, *c.spans, 1 if c.decode else c.max_len)
+        if c.decode and bounds is not None:
+            return attn_paged_sparse(qkvg, m.heads, c.positions, None, cache, c.kv.page_table, bounds, spec, out, top=c.sparse_pages, seq_lens=c.kv.seq_lens)
+        if c.decode:
+            return attn_decode_shared(qkvg, m.heads, c.kv.seq_lens, cache, c.kv.page_table, c.kv.shared, spec, out)
         return A.attn_prefill_paged(qkvg, m.heads, c.positions, c.seq_ids, c.cu_seqlens, c.max_len, cache, c.kv.page_table, spec, out)
 
 
