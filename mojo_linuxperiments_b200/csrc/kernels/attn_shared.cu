@@ -101,7 +101,9 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
   pdl_launch_dependents();       // what starts now may read all that was written before this kernel
 
   auto wait = [&](int i, uint32_t par, int code) { return mbar_wait(bar(i), par, abort_flag, p.status, code | (26 << 8), p.limit_ns); };
-  auto meet = [&] { named_bar_sync(1, SX_THREADS); };        // all warps, from the two branches that they are in
+  // all warps meet, from the two branches that they are in, where the queries are in place and at the end of a piece
+  enum { M_QUERIES = 1, M_END = 2 };
+  auto meet = [&](int id) { named_bar_sync(id, SX_THREADS); };
   auto piece_of = [&](int item) {
     const int4* at = reinterpret_cast<const int4*>(p.plan + p.pieces_at + (item / hkv) * SP_PIECE);
     const int4 a = at[0], b = at[1];
@@ -128,14 +130,15 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
       if (warp == 0) {
         const int* pt = p.c.page_table + static_cast<size_t>(e.lead) * p.c.max_pages;
         bool ok = true;
-        int page = 0;
-        auto page_of = [&](int j) {
-          const int tok = kv_start + j * SX_BN + (lane & 7) * SX_PS;
+        // the pages of four tiles are in the lanes, those of the next four on their way
+        auto ids_of = [&](int j) {
+          const int tok = kv_start + j * SX_BN + lane * SX_PS;
           const int pg = tok < kv_end ? pt[tok / SX_PS] : p.c.num_pages;       // pages behind the end are filled with zeros
           if (pg >= 0 && pg <= p.c.num_pages) return pg;
           if (p.status) atomicCAS(p.status, 0, static_cast<int>(ST_BAD_ARGUMENT) | (26 << 8));
           return p.c.num_pages;
         };
+        int ids = 0, ids_next = 0;
         auto load = [&](uint32_t dst, const CUtensorMap* m, int b, int chunks, int pg) {
           if (lane == 0) mbar_expect_tx(bar(b), chunks * SX_CHUNK);
           __syncwarp();
@@ -143,7 +146,8 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
             for (int c = 0; c < chunks; ++c) tma_load_3d(dst + c * SX_CHUNK + lane * 2048, m, bar(b), c * 64, kvh * SX_PS, pg);
         };
         auto fetch = [&](int j) {
-          const int next = j + 1 < n ? page_of(j + 1) : 0;
+          if ((j & 3) == 0 && j > 0) { ids = ids_next; ids_next = ids_of(j + 4); }
+          const int page = __shfl_sync(0xffffffffu, ids, (j & 3) * 8 + (lane & 7));
           const int st = (kv + j) & 1;
           const uint32_t ph = (((kv + j) >> 1) & 1u) ^ 1u;
           ok = __all_sync(0xffffffffu, wait(B_KEMPTY + st, ph, ST_TIMEOUT_SMEM_EMPTY)) != 0;
@@ -152,23 +156,15 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
           ok = __all_sync(0xffffffffu, wait(B_VEMPTY + st, ph, ST_TIMEOUT_SMEM_EMPTY)) != 0;
           if (!ok) return;
           load(sV + st * SX_TILE, &tmap_v, B_VFULL + st, vchunks, page);
-          page = next;
         };
-        int j = 0;
-        if (p.chunk <= 0) {                      // the first tiles need not wait for the queries: both stages are free between pieces
-          n = tiles_of(e, turn, kv_start, kv_end);
-          if (n > 0) page = page_of(0);
-          for (; j < min(n, 2) && ok; ++j) fetch(j);
-        }
-        meet();                                  // the queries are in place, and what they see is known
-        if (p.chunk > 0) {
-          n = tiles_of(e, turn, kv_start, kv_end);
-          if (n > 0) page = page_of(0);
-        }
-        for (; j < n && ok; ++j) fetch(j);
+        // without chunks the keys are known before the queries are in place, and nobody waits for this warp
+        if (p.chunk > 0) meet(M_QUERIES); else named_bar_arrive(M_QUERIES, SX_THREADS);
+        n = tiles_of(e, turn, kv_start, kv_end);
+        if (n > 0) { ids = ids_of(0); ids_next = ids_of(4); }
+        for (int j = 0; j < n && ok; ++j) fetch(j);
         if (!ok) { const uint64_t t0 = globaltimer_ns(); while (globaltimer_ns() - t0 < 2000000ull) { } }   // copies in flight land
       } else {
-        meet();
+        meet(M_QUERIES);
         n = tiles_of(e, turn, kv_start, kv_end);
         if (warp == 1) {
           const bool one = elect_one();
@@ -219,7 +215,7 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
         }
       }
       kv += n;
-      meet();
+      meet(M_END);
       if (*abort_flag) break;                    // the same for all: nobody sets it between here and the next meeting
       if (item + static_cast<int>(gridDim.x) < pieces) e = piece_of(item + gridDim.x);
     }
@@ -259,7 +255,7 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
         sx_copies_done();
         fence_proxy_async_smem();
       }
-      meet();
+      meet(M_QUERIES);
       if (threadIdx.x == 128) B200_TRACE(TK_ATTN_SHARED, 2); // queries in place
       int kv_start, kv_end;
       const int n = rows > 0 ? tiles_of(e, turn, kv_start, kv_end) : 0;
@@ -364,7 +360,7 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
           }
       }
       tc_fence_before();
-      meet();
+      meet(M_END);
       if (threadIdx.x == 128) {
         if (!*abort_flag) red_release_gpu_add(reinterpret_cast<uint32_t*>(p.plan + SP_DONE), 1u);
         B200_TRACE(TK_ATTN_SHARED, 6);           // a piece

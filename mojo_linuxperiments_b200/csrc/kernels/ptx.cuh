@@ -298,6 +298,10 @@ template <int N> __device__ __forceinline__ void warpgroup_regs_inc() { asm vola
 __device__ __forceinline__ void named_bar_sync(int id, int nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }
+// counted there, without waiting
+__device__ __forceinline__ void named_bar_arrive(int id, int nthreads) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
+}
 // the same, and true for all threads if it was for one: what decides whether they meet at a barrier again
 __device__ __forceinline__ bool named_bar_or(int id, int nthreads, bool mine) {
   uint32_t any;

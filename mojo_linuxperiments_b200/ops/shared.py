@@ -22,12 +22,13 @@ def room_for(num_seqs: int, per_head: int, kv_heads: int, ctas: int) -> tuple[in
     return num_seqs * per_head // (2 * ROW_TILE) + num_seqs + more, 2 * num_seqs * per_head + 2 * ROW_TILE * more
 
 
-def cut_prefixes(groups, num_seqs: int, per_head: int, kv_heads: int, ctas: int, others: int = 0):
+def cut_prefixes(groups, num_seqs: int, per_head: int, kv_heads: int, ctas: int, others: int = 0, chunk: int = 0):
     """How the prefixes of ``groups`` (slots, tokens) are shared out: (four numbers per slot, pieces, slots in order, rows of partial results).
 
     A piece is up to 256 rows of a group and a run of tiles of 128 keys, for every KV head.  The two units of a CTA have 128 rows each, or, in a group of no
     more than 128, the same rows and every other tile.  Runs are as long as ends soonest: pieces of L steps take L + 4 (their start and end), ``ctas`` of
-    them at a time, and ``others``, the CTAs of the slots' own keys, three of which fit where there is no piece, another 4 if some of them have to wait.  A slot's numbers: first row of its partial results, rows between the parts, parts, tokens."""
+    them at a time, and ``others``, the CTAs of the slots' own keys, three of which fit where there is no piece, another 4 if some of them have to wait.  With ``chunk`` only that many keys of a prefix are seen, so that most
+    runs are over at once.  A slot's numbers: first row of its partial results, rows between the parts, parts, tokens."""
     info, pieces, order, base = [0] * (4 * num_seqs), [], [], 0
     if not groups:
         return info, pieces, order, base
@@ -43,13 +44,15 @@ def cut_prefixes(groups, num_seqs: int, per_head: int, kv_heads: int, ctas: int,
         return (_ONE, 1, 1) if tiles == 1 else (_KEYS, runs, 2 * runs)
 
     def took(steps):
-        longest = count = room = 0
+        longest = count = busy = room = 0
         for rows, tiles in sizes:
             mode, runs, parts = shape(rows, tiles, steps)
-            longest = max(longest, -(-tiles // runs) if mode == _ROWS else -(-tiles // (2 * runs)))
+            seen, run = min(tiles, chunk // KEY_TILE + 2) if chunk else tiles, -(-tiles // runs)
+            longest = max(longest, min(seen, run) if mode == _ROWS else -(-min(seen, run) // 2))
             count += -(-rows // (2 * ROW_TILE)) * runs
+            busy += -(-rows // (2 * ROW_TILE)) * min(runs, -(-seen // run) + (seen < tiles))
             room += rows * parts
-        fits, count = count <= most[0] and room <= most[1], kv_heads * count
+        fits, count = count <= most[0] and room <= most[1], kv_heads * busy
         return not fits, -(-count // ctas) * (longest + 4) + (4 if others > 3 * max(0, ctas - count) else 0)
 
     tried, at = [], max(tiles for _, tiles in sizes)       # one run each always fits
@@ -73,8 +76,8 @@ def cut_prefixes(groups, num_seqs: int, per_head: int, kv_heads: int, ctas: int,
 class _Cut:
     """A plan as the kernels read it, for one number of heads, and room for partial results."""
 
-    def __init__(self, num_seqs: int, per_head: int, kv_heads: int, dv: int, device: torch.device):
-        self.per_head, self.kv_heads, self.sms = per_head, kv_heads, _lib.num_sms(device.index)
+    def __init__(self, num_seqs: int, per_head: int, kv_heads: int, dv: int, chunk: int, device: torch.device):
+        self.per_head, self.kv_heads, self.chunk, self.sms = per_head, kv_heads, chunk, _lib.num_sms(device.index)
         self.max_pieces, self.rows = room_for(num_seqs, per_head, kv_heads, self.sms)
         self.pieces_at = (_INFO + 4 * num_seqs + 7) // 8 * 8
         self.slots_at = self.pieces_at + _PIECE * self.max_pieces
@@ -82,12 +85,12 @@ class _Cut:
         self.plan = torch.zeros(n, dtype=torch.int32, device=device)
         self.part = torch.empty(kv_heads * self.rows * (dv + 2), dtype=torch.float32, device=device)
         # a ring: a copy still queued on the stream never sees an edit that belongs to a later step
-        self.ring = [(torch.zeros(n, dtype=torch.int32).pin_memory(), torch.cuda.Event()) for _ in range(4)]
+        self.ring = [(buf, torch.cuda.Event()) for buf in torch.zeros(4, n, dtype=torch.int32, pin_memory=True)]
         self.turn = 0
 
     def send(self, groups, num_seqs: int) -> None:
         others = num_seqs * self.kv_heads * -(-self.per_head // 16)
-        info, pieces, order, rows = cut_prefixes(groups, num_seqs, self.per_head, self.kv_heads, self.sms, others)
+        info, pieces, order, rows = cut_prefixes(groups, num_seqs, self.per_head, self.kv_heads, self.sms, others, self.chunk)
         assert len(pieces) <= self.max_pieces and rows <= self.rows
         buf, done = self.ring[self.turn]
         self.turn = (self.turn + 1) % len(self.ring)
@@ -124,23 +127,23 @@ class SharedPrefixes:
             raise ValueError(f"slots {sorted(every)} of {self.num_seqs}")
         if any(tokens < 0 or tokens % PAGE for _, tokens in groups):
             raise ValueError(f"prefixes of {[t for _, t in groups]} tokens: whole pages of {PAGE} are shared")
-        self.groups = [(slots, tokens) for slots, tokens in groups if slots and tokens]
+        self.groups = [(slots, tokens) for slots, tokens in groups if len(slots) > 1 and tokens]      # a slot alone shares nothing
         self.longest = max((t for _, t in self.groups), default=0)
         covered = sum(len(slots) for slots, _ in self.groups)
         self.alone = min((t for _, t in self.groups), default=0) if covered == self.num_seqs else 0
         for cut in self._cuts.values():
             cut.send(self.groups, self.num_seqs)
 
-    def cut_for(self, hq: int, cache: PagedKVCache) -> _Cut:
+    def cut_for(self, hq: int, cache: PagedKVCache, chunk: int = 0) -> _Cut:
         device = cache.data.device
-        key = (hq, cache.kv_heads, cache.dv, device.index)
+        key = (hq, cache.kv_heads, cache.dv, chunk, device.index)
         cut = self._cuts.get(key)
         if cut is None:
             if device != self.device and (device.type != self.device.type or self.device.index is not None):
                 raise ValueError(f"a plan for {self.device} and a cache on {device}")
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("the first call with a plan sends it to the device: make one before the capture")
-            cut = self._cuts[key] = _Cut(self.num_seqs, hq // cache.kv_heads, cache.kv_heads, cache.dv, device)
+            cut = self._cuts[key] = _Cut(self.num_seqs, hq // cache.kv_heads, cache.kv_heads, cache.dv, chunk, device)
             cut.send(self.groups, self.num_seqs)
         return cut
 
@@ -165,7 +168,7 @@ def attn_decode_shared(q: torch.Tensor, hq: int, seq_lens: torch.Tensor, cache: 
                             ctypes.byref(desc), ctypes.byref(spec), default_workspace(q.device).status.data_ptr())
         _lib.check(rc, "attn_paged")
         return out
-    cut = shared.cut_for(hq, cache)
+    cut = shared.cut_for(hq, cache, spec.chunk)
     if splits is None:
         keys = min(room - shared.alone, spec.chunk) if spec.chunk > 0 else room - shared.alone
         splits = pick_decode_splits_paged(B, cache.kv_heads * ((hq // cache.kv_heads + 15) // 16), keys, cut.sms)
