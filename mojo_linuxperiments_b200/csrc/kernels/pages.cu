@@ -94,11 +94,12 @@ __global__ void __launch_bounds__(32 * PB_WARPS) page_bounds_kernel(const __grid
   const int lane = threadIdx.x & 31, b = blockIdx.y, ps = p.c.page_size, dk = p.c.dk;
   const int start = p.starts[b], end = p.ends[b], seq = p.seq_ids ? p.seq_ids[b] : b;
   if (end <= start) return;
-  if (start < 0 || seq < 0 || seq >= p.c.num_seqs || (end - 1) / ps >= p.c.max_pages) {
+  const int last = (end - 1) / ps;
+  if (start < 0 || seq < 0 || seq >= p.c.num_seqs || last >= p.c.max_pages || last - start / ps >= static_cast<int>(gridDim.x) * PB_PAGES) {
     if (threadIdx.x == 0 && blockIdx.x == 0 && p.status) atomicCAS(p.status, 0, static_cast<int>(ST_BAD_ARGUMENT) | (24 << 8));
     return;
   }
-  const int place0 = start / ps + blockIdx.x * PB_PAGES, pages = min(PB_PAGES, (end - 1) / ps + 1 - place0);
+  const int place0 = start / ps + blockIdx.x * PB_PAGES, pages = min(PB_PAGES, last + 1 - place0);
   if (pages <= 0) return;
   if (static_cast<int>(threadIdx.x) < pages) {
     const int page = p.c.page_table[static_cast<size_t>(seq) * p.c.max_pages + place0 + threadIdx.x];

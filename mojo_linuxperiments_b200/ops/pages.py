@@ -66,7 +66,8 @@ def page_bounds(cache: PagedKVCache, page_table: torch.Tensor, starts: torch.Ten
                 bounds: torch.Tensor) -> torch.Tensor:
     """Smallest and largest element of the keys of a page, per KV head and dimension, for all pages that hold tokens ``starts[i]`` to
     ``ends[i] - 1`` (int32) of sequence ``seq_ids[i]`` (None: i); all tokens of such a page up to ``ends[i]`` count, nothing behind them is read.
-    ``max_tokens``: the most that a portion has.  A portion of none, as of an empty slot, changes nothing.  Exact; NaN where a key is."""
+    ``max_tokens``: the most that a portion has; one that has more pages than that may is left out, which the status word says.  A page is touched by one
+    portion only.  A portion of no tokens, as of an empty slot, changes nothing.  Exact; NaN where a key is."""
     check_bounds(cache, bounds)
     n = starts.numel()
     assert starts.dtype == ends.dtype == page_table.dtype == torch.int32 and ends.numel() == n and all(t.is_contiguous() for t in (starts, ends, page_table))

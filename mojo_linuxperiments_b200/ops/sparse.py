@@ -11,13 +11,15 @@ from .pages import check_bounds
 from .workspace import default_workspace
 
 MAX_HEAD_DIM = 512
+MAX_ROWS = 65535
+LIST_PER_CTA = 16384           # pages that a CTA may have to read
 
 
 def pick_sparse_splits(pairs: int, pages: int, num_sms: int = 148, least: int = 16) -> int:
     """CTAs (one cluster of up to eight) per row and group of heads, which share ``pages`` pages: as many as still make one wave of one per SM, with
-    ``least`` pages (16: two for a warp) each."""
+    ``least`` pages (16: two for a warp) each, and so many that their lists have room."""
     s = 1
-    while s < 8 and pairs * s * 2 <= num_sms and pages // (2 * s) >= least:
+    while s < 8 and ((pairs * s * 2 <= num_sms and pages // (2 * s) >= least) or pages > s * LIST_PER_CTA):
         s *= 2
     return s
 
@@ -43,8 +45,10 @@ def attn_paged_sparse(q: torch.Tensor, hq: int, positions: torch.Tensor, seq_ids
     assert positions.dtype == page_table.dtype == torch.int32 and page_table.is_contiguous() and positions.is_contiguous()
     for t in (seq_ids, seq_lens):
         assert t is None or (t.dtype == torch.int32 and t.is_contiguous() and t.numel() == M)
-    if max(cache.dk, cache.dv) > MAX_HEAD_DIM or cache.dv == 0:
-        raise ValueError(f"heads of {cache.dk} and {cache.dv}")
+    if max(cache.dk, cache.dv) > MAX_HEAD_DIM or cache.dv == 0 or (hq // cache.kv_heads) * (cache.dk + 127 & ~127) > 50 << 10:
+        raise ValueError(f"{hq} heads of {cache.dk} and {cache.dv} over {cache.kv_heads}")
+    if M > MAX_ROWS or min(top, page_table.shape[1]) > 8 * LIST_PER_CTA:
+        raise ValueError(f"{M} rows and {top} pages in one call")
     if seq_ids is None and M > page_table.shape[0]:
         raise ValueError(f"{M} rows of {page_table.shape[0]} sequences")
     if chosen is not None:

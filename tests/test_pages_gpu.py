@@ -125,3 +125,14 @@ def test_pages_that_do_not_exist_are_told_and_left_out():
     PG.page_bounds(S.cache, S.table, z, z + 49, None, 49, bounds)                  # longer than a row of the table
     with pytest.raises(RuntimeError, match="page_bounds"):
         status_ok()
+
+
+def test_a_portion_longer_than_was_said_is_told_and_left_out():
+    from mojo_linuxperiments_b200.ops import pages as PG
+    S = Sequences([400], 1, 1, 16, 8, "bfloat16")
+    bounds = PG.bounds_for(S.cache).fill_(7.0)
+    z = torch.zeros(1, dtype=torch.int32, device=DEV)
+    PG.page_bounds(S.cache, S.table, z, z + 400, None, 16, bounds)
+    with pytest.raises(RuntimeError, match="page_bounds"):
+        status_ok()
+    assert (bounds == 7.0).all()
