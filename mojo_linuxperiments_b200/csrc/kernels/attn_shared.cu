@@ -16,8 +16,13 @@
 namespace b200 {
 
 // ---- the plan: int32 on the device -------------------------------------------------------------------------------------------------
-// [0] pieces; [4] pieces of this call that are done, [5] CTAs of the second kernel that have seen it (both zero between calls); at SP_INFO four numbers per slot: first row of its partial results, rows between the parts of the prefix, parts, tokens;
-// then the pieces, eight numbers each; then the slots of the groups' members.
+// [0] pieces; [4] pieces of this call that are done, [5] CTAs of the second kernel that have seen it (both zero between calls); at SP_INFO four numbers
+// per slot: first row of its partial results, rows between the parts of the prefix, parts, tokens; then the pieces, eight numbers each; then the slots of the groups'
+// members.
+//
+// A slot takes either all keys of the pieces of its group or none, so that no row meets a value that it does not see: none if it is shorter than the prefix,
+// or if its chunk begins behind it.  A chunk that begins inside the prefix begins at the same key for every other slot, the last multiple of the chunk in front of
+// the prefix's end; the pieces begin at the first page from there on, and what lies in front of that page is each slot's own.
 constexpr int SP_DONE = 4, SP_SEEN = 5, SP_INFO = 16, SP_PIECE = 8;
 // member0: of the group, in the list of slots; rows row0 .. row0 + rows of the group (member x query head); keys key0 .. key1; part: first row of the partial
 // results of the group's rows for this run of keys; lead: slot whose pages are read; mode: what the two units of a CTA do, and above it the group's rows
@@ -78,7 +83,7 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
   auto bar = [&](int i) { return bar0 + 8u * i; };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + B_COUNT);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* spans = reinterpret_cast<int*>(tmem_slot + 2);        // keys that some row of the piece sees: first, end; two pieces in turn
+  volatile int* seen = reinterpret_cast<volatile int*>(tmem_slot + 2);       // with chunks: some row of the piece takes it; two pieces in turn
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int dk = p.c.dk, dv = p.c.dv, hkv = p.c.kv_heads, group = p.hq / hkv;
@@ -86,8 +91,7 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
   if (threadIdx.x == 0) {
     for (int i = 0; i < B_COUNT; ++i) mbar_init(bar(i), (i & ~1) == B_PFULL ? 4 : 1);
     *abort_flag = 0;
-    spans[0] = spans[2] = 0x7fffffff;
-    spans[1] = spans[3] = 0;
+    seen[0] = seen[1] = 0;
     mbar_fence_init();
   }
   if (warp == 1) { tmem_alloc(smem_u32(tmem_slot), 512); tmem_relinquish(); }
@@ -110,12 +114,10 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
     return SharedPiece{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w & 3, b.w >> 2};
   };
   const int room = p.c.max_pages * SX_PS;
-  // Tiles of 128 keys.  Without chunks they are the piece's; a sequence that ends within it sees less of them.  With chunks: from the page of the
-  // first key that counts for somebody, known when the queries are in place.
-  auto tiles_of = [&](const SharedPiece& e, int turn, int& kv_start, int& kv_end) {
-    kv_start = p.chunk > 0 ? spans[2 * turn] & ~(SX_PS - 1) : e.key0;
-    kv_end = p.chunk > 0 ? spans[2 * turn + 1] : min(e.key1, room);
-    return kv_end > kv_start ? (kv_end - kv_start + SX_BN - 1) / SX_BN : 0;
+  // tiles of 128 keys; with chunks known when the queries are in place
+  auto tiles_of = [&](const SharedPiece& e, int turn) {
+    const int end = min(e.key1, room);
+    return end > e.key0 && (p.chunk <= 0 || seen[turn]) ? (end - e.key0 + SX_BN - 1) / SX_BN : 0;
   };
   auto units_of = [&](const SharedPiece& e) { return e.mode == SM_KEYS || (e.mode == SM_ROWS && e.rows > 128) ? 2 : 1; };
   SharedPiece e = piece_of(blockIdx.x);          // there is room for as many pieces as there are CTAs
@@ -126,13 +128,14 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
     uint32_t kv = 0, p_par = 0;                  // tiles so far; bit u: parity of unit u's P
     for (int item = blockIdx.x; item < pieces; item += gridDim.x, turn ^= 1) {
       const int kvh = item % hkv;
-      int kv_start = 0, kv_end = 0, n = 0;
+      int n = 0;
       if (warp == 0) {
+        const int kv_end = min(e.key1, room);
         const int* pt = p.c.page_table + static_cast<size_t>(e.lead) * p.c.max_pages;
         bool ok = true;
         // the pages of four tiles are in the lanes, those of the next four on their way
         auto ids_of = [&](int j) {
-          const int tok = kv_start + j * SX_BN + lane * SX_PS;
+          const int tok = e.key0 + j * SX_BN + lane * SX_PS;
           const int pg = tok < kv_end ? pt[tok / SX_PS] : p.c.num_pages;       // pages behind the end are filled with zeros
           if (pg >= 0 && pg <= p.c.num_pages) return pg;
           if (p.status) atomicCAS(p.status, 0, static_cast<int>(ST_BAD_ARGUMENT) | (26 << 8));
@@ -159,13 +162,13 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
         };
         // without chunks the keys are known before the queries are in place, and nobody waits for this warp
         if (p.chunk > 0) meet(M_QUERIES); else named_bar_arrive(M_QUERIES, SX_THREADS);
-        n = tiles_of(e, turn, kv_start, kv_end);
+        n = tiles_of(e, turn);
         if (n > 0) { ids = ids_of(0); ids_next = ids_of(4); }
         for (int j = 0; j < n && ok; ++j) fetch(j);
         if (!ok) { const uint64_t t0 = globaltimer_ns(); while (globaltimer_ns() - t0 < 2000000ull) { } }   // copies in flight land
       } else {
         meet(M_QUERIES);
-        n = tiles_of(e, turn, kv_start, kv_end);
+        n = tiles_of(e, turn);
         if (warp == 1) {
           const bool one = elect_one();
           constexpr uint32_t IDESC_S = umma_idesc_bf16(128, 128, 0, 0);
@@ -209,9 +212,8 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
             }
           }
           __syncwarp();
-        } else if (threadIdx.x == 64) {          // the other piece's, of which nobody reads any more
-          spans[2 * (turn ^ 1)] = 0x7fffffff;
-          spans[2 * (turn ^ 1) + 1] = 0;
+        } else if (threadIdx.x == 64) {
+          seen[turn ^ 1] = 0;                    // the other piece's, at which nobody looks any more
         }
       }
       kv += n;
@@ -229,22 +231,20 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
       const int kvh = item % hkv;
       const int row0 = e.row0 + (e.mode == SM_ROWS ? 128 * u : 0), rows = u < units_of(e) ? min(128, e.rows - (row0 - e.row0)) : 0;
       const bool idle = (warp & 3) * 32 >= rows;             // rows that nobody asked for: their weights are never looked at
-      int low = 0, end = 0;                      // keys that the row sees of this piece
       if (!idle) {
         const int row = row0 + r, member = row / group;
         const bool on = r < rows;
         const int slot = on ? p.plan[p.slots_at + e.member0 + member] : 0;
-        const int len = on ? p.seq_lens[slot] : 0;
         const long long from = on ? slot * p.ldq + static_cast<long long>(kvh * group + row - member * group) * dk : -1;
-        if (len > 0) {
-          low = max(e.key0, p.chunk > 0 ? (len - 1) - (len - 1) % p.chunk : 0);
-          end = min(min(e.key1, len), room);
-          if (low >= end) end = 0;
+        bool any = true;
+        if (p.chunk > 0) {
+          const int len = on ? p.seq_lens[slot] : 0, tokens = on ? p.plan[SP_INFO + 4 * slot + 3] : 0;
+          any = __any_sync(0xffffffffu, on && len >= tokens && (len - 1) - (len - 1) % p.chunk < tokens);
+          if (any && lane == 0) seen[turn] = 1;
         }
-        if (end > 0 && p.chunk > 0) { atomicMin(&spans[2 * turn], low); atomicMax(&spans[2 * turn + 1], end); }
         // half a warp per row: 256 neighbouring bytes at a time
         const int col = lane & 15;
-        if (p.chunk <= 0 || __any_sync(0xffffffffu, end > 0))      // with chunks: nobody may see anything
+        if (any)
 #pragma unroll 2
         for (int i = 0; i < 16; ++i) {
           const long long at = __shfl_sync(0xffffffffu, from, 2 * i + (lane >> 4));
@@ -257,8 +257,7 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
       }
       meet(M_QUERIES);
       if (threadIdx.x == 128) B200_TRACE(TK_ATTN_SHARED, 2); // queries in place
-      int kv_start, kv_end;
-      const int n = rows > 0 ? tiles_of(e, turn, kv_start, kv_end) : 0;
+      const int n = rows > 0 ? tiles_of(e, turn) : 0, keys = min(e.key1, room) - e.key0;
       const int j0 = e.mode == SM_KEYS ? u : 0, step = e.mode == SM_KEYS ? 2 : 1;
       float m_ref = -INFINITY, l = 0.f;
       bool ok = true;
@@ -272,12 +271,12 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
 #pragma unroll
           for (int c = 0; c < 4; ++c) tmem_ld_x32(t_s + c * 32, v[c]);
           tmem_ld_wait();
-          const int kv0 = kv_start + j * SX_BN, a = low - kv0, b = end - kv0;
-          if (__any_sync(0xffffffffu, a > 0 || b < SX_BN)) {
+          const int here = keys - j * SX_BN;     // behind them the tile is zeros
+          if (here < SX_BN) {
 #pragma unroll
             for (int c = 0; c < 4; ++c)
 #pragma unroll
-              for (int i = 0; i < 32; ++i) if (c * 32 + i < a || c * 32 + i >= b) v[c][i] = 0xff800000u;      // -inf
+              for (int i = 0; i < 32; ++i) if (c * 32 + i >= here) v[c][i] = 0xff800000u;      // -inf
           }
           float mx[4];
 #pragma unroll
@@ -422,8 +421,12 @@ __global__ void __launch_bounds__(SO_THREADS, NH == 1 ? 3 : 2) attn_shared_own_k
     so_leave(p);
     return;
   }
-  const int low = max(p.chunk > 0 ? (len - 1) - (len - 1) % p.chunk : 0, min(info.w, len));      // first key that is this kernel's
-  const int t0 = low / SX_PS, tiles = low < len ? (len - 1) / SX_PS - t0 + 1 : 0;
+  const int low = p.chunk > 0 ? (len - 1) - (len - 1) % p.chunk : 0;
+  const bool shares = info.z > 0 && len >= info.w && low < info.w;
+  // pages of the keys that are this kernel's: from the first seen, or those behind the prefix and, in front of them, the one that a chunk begins in
+  const bool head = shares && low % SX_PS != 0;
+  const int t0 = shares ? info.w / SX_PS - head : low / SX_PS, tiles = (len + SX_PS - 1) / SX_PS - t0;
+  auto place = [&](int t) { return head && t == t0 ? low / SX_PS : t; };
   const int ta = t0 + static_cast<int>(static_cast<long long>(tiles) * rank / S), tb = t0 + static_cast<int>(static_cast<long long>(tiles) * (rank + 1) / S);
   const int mine = tb - ta > warp ? (tb - ta - warp + SO_WARPS - 1) / SO_WARPS : 0;
   const int* pt = p.c.page_table + static_cast<size_t>(b) * p.c.max_pages;
@@ -438,12 +441,12 @@ __global__ void __launch_bounds__(SO_THREADS, NH == 1 ? 3 : 2) attn_shared_own_k
   w.template walk<false>(mine, [&](int i) {
     if (i >= ids_from + 32) {
       ids_from = i;
-      ids = i + lane < mine ? pt[ta + warp + (i + lane) * SO_WARPS] : -1;
+      ids = i + lane < mine ? pt[place(ta + warp + (i + lane) * SO_WARPS)] : -1;
       if (lane > 0 && lane < SO_AHEAD) dw_prefetch(kbase, vbase, ids, rec, dk, dv, p.c.num_pages);
     } else if (lane == i - ids_from + SO_AHEAD - 1) {
       dw_prefetch(kbase, vbase, ids, rec, dk, dv, p.c.num_pages);
     }
-    const int page = __shfl_sync(0xffffffffu, ids, i - ids_from), first = (ta + warp + i * SO_WARPS) * SX_PS;
+    const int page = __shfl_sync(0xffffffffu, ids, i - ids_from), first = place(ta + warp + i * SO_WARPS) * SX_PS;
     const bool there = page >= 0 && page < p.c.num_pages;
     if (!there && lane == 0 && p.status) atomicCAS(p.status, 0, static_cast<int>(ST_BAD_ARGUMENT) | (26 << 8));
     const size_t at = there ? page * rec : 0;
@@ -456,7 +459,7 @@ __global__ void __launch_bounds__(SO_THREADS, NH == 1 ? 3 : 2) attn_shared_own_k
   float* share = own + Sh::SIZE;                 // [16][8 + SO_PARTS]: what each part counts in the end
   dw_join<SO_WARPS, SO_THREADS>(so_smem, Sh::SIZE, Sh::PITCH, G, dv, own);
   // The parts of the prefix.  All CTAs of the first kernel run when this one starts, so their pieces may be waited for; the wait for its end takes 2 us longer.
-  if (tid == 0 && info.z > 0) {
+  if (tid == 0 && shares) {
     const uint32_t pieces = static_cast<uint32_t>(min(p.plan[0], p.max_pieces)) * p.c.kv_heads;
     wait_count_gpu(reinterpret_cast<const uint32_t*>(p.plan + SP_DONE), pieces, p.status, static_cast<int>(ST_TIMEOUT_PEER_FLAG) | (26 << 8), p.limit_ns);
   }
@@ -465,7 +468,7 @@ __global__ void __launch_bounds__(SO_THREADS, NH == 1 ? 3 : 2) attn_shared_own_k
   const uint32_t own_addr = smem_u32(own);
   const float4* parts = reinterpret_cast<const float4*>(p.part) + static_cast<size_t>(kvh) * (dv >> 2) * p.part_rows + info.x + g0;
   const float* ml = p.part + static_cast<size_t>(p.c.kv_heads) * p.part_rows * dv + 2 * (static_cast<size_t>(kvh) * p.part_rows + info.x + g0);
-  const int n_parts = min(info.z, SO_PARTS), all = S + n_parts;
+  const int n_parts = shares ? min(info.z, SO_PARTS) : 0, all = S + n_parts;
   // a warp per row: lanes take the parts
   for (int g = warp; g < G; g += SO_WARPS) {
     float m[2], l[2];
@@ -511,7 +514,7 @@ __global__ void __launch_bounds__(SO_THREADS, NH == 1 ? 3 : 2) attn_shared_own_k
     }
 #pragma unroll 8
     for (int s = 0; s < n_parts; ++s) {
-      const float fs = f[S + s];                 // zero: a part without keys, which has left no numbers
+      const float fs = f[S + s];                 // zero: perhaps a part without keys, which has left no numbers
       const float4 x = fs != 0.f ? __ldcg(parts + static_cast<size_t>(d >> 2) * p.part_rows + static_cast<size_t>(s) * info.y + g) : make_float4(0.f, 0.f, 0.f, 0.f);
       v.x += fs * x.x; v.y += fs * x.y; v.z += fs * x.z; v.w += fs * x.w;
     }

@@ -27,12 +27,14 @@ def cut_prefixes(groups, num_seqs: int, per_head: int, kv_heads: int, ctas: int,
 
     A piece is up to 256 rows of a group and a run of tiles of 128 keys, for every KV head.  The two units of a CTA have 128 rows each, or, in a group of no
     more than 128, the same rows and every other tile.  Runs are as long as ends soonest: pieces of L steps take L + 4 (their start and end), ``ctas`` of
-    them at a time, and ``others``, the CTAs of the slots' own keys, three of which fit where there is no piece, another 4 if some of them have to wait.  With ``chunk`` only that many keys of a prefix are seen, so that most
-    runs are over at once.  A slot's numbers: first row of its partial results, rows between the parts, parts, tokens."""
+    them at a time, and ``others``, the CTAs of the slots' own keys, three of which fit where there is no piece, another 4 if some of them have to wait.  With ``chunk`` only the keys from the last multiple of it are seen, and
+    shared from the next page on.  A slot's numbers: first row of its partial results, rows between the parts, parts (none: it shares nothing), tokens."""
     info, pieces, order, base = [0] * (4 * num_seqs), [], [], 0
+    begins = [-(-((tokens - 1) // chunk * chunk) // PAGE) * PAGE if chunk else 0 for _, tokens in groups]
+    groups, begins = [g for g, a in zip(groups, begins) if a < g[1]], [a for (_, tokens), a in zip(groups, begins) if a < tokens]
     if not groups:
         return info, pieces, order, base
-    sizes = [(len(slots) * per_head, -(-tokens // KEY_TILE)) for slots, tokens in groups]
+    sizes = [(len(slots) * per_head, -(-(tokens - begin) // KEY_TILE)) for (slots, tokens), begin in zip(groups, begins)]
     most = room_for(num_seqs, per_head, kv_heads, ctas)
 
     def shape(rows, tiles, steps):
@@ -44,15 +46,14 @@ def cut_prefixes(groups, num_seqs: int, per_head: int, kv_heads: int, ctas: int,
         return (_ONE, 1, 1) if tiles == 1 else (_KEYS, runs, 2 * runs)
 
     def took(steps):
-        longest = count = busy = room = 0
+        longest = count = room = 0
         for rows, tiles in sizes:
             mode, runs, parts = shape(rows, tiles, steps)
-            seen, run = min(tiles, chunk // KEY_TILE + 2) if chunk else tiles, -(-tiles // runs)
-            longest = max(longest, min(seen, run) if mode == _ROWS else -(-min(seen, run) // 2))
+            run = -(-tiles // runs)
+            longest = max(longest, run if mode == _ROWS else -(-run // 2))
             count += -(-rows // (2 * ROW_TILE)) * runs
-            busy += -(-rows // (2 * ROW_TILE)) * min(runs, -(-seen // run) + (seen < tiles))
             room += rows * parts
-        fits, count = count <= most[0] and room <= most[1], kv_heads * busy
+        fits, count = count <= most[0] and room <= most[1], kv_heads * count
         return not fits, -(-count // ctas) * (longest + 4) + (4 if others > 3 * max(0, ctas - count) else 0)
 
     tried, at = [], max(tiles for _, tiles in sizes)       # one run each always fits
@@ -60,12 +61,12 @@ def cut_prefixes(groups, num_seqs: int, per_head: int, kv_heads: int, ctas: int,
         tried.append(at)
         at = min(at - 1, int(at / 1.06))
     steps = min(tried, key=took)
-    for (slots, tokens), (rows, tiles) in zip(groups, sizes):
+    for (slots, tokens), begin, (rows, tiles) in zip(groups, begins, sizes):
         mode, runs, parts = shape(rows, tiles, steps)
         for i, s in enumerate(slots):
             info[4 * s:4 * s + 4] = [base + i * per_head, rows, parts, tokens]
         for k in range(runs):
-            a, b = tiles * k // runs * KEY_TILE, min(tokens, tiles * (k + 1) // runs * KEY_TILE)
+            a, b = begin + tiles * k // runs * KEY_TILE, min(tokens, begin + tiles * (k + 1) // runs * KEY_TILE)
             for row0 in range(0, rows, 2 * ROW_TILE):
                 pieces.append([len(order), row0, min(2 * ROW_TILE, rows - row0), a, b, base + k * (parts // runs) * rows, slots[0], mode + 4 * rows])
         base += rows * parts
@@ -120,13 +121,16 @@ class SharedPrefixes:
         self._cuts: dict[tuple, _Cut] = {}
 
     def set(self, groups) -> None:
-        """``groups``: (slots, tokens) each.  Stream-ordered, like ``KVState.flush``."""
+        """``groups``: (slots, tokens) each.  Stream-ordered, like ``KVState.flush``, and not part of a captured call.  The pages of a prefix are read by the
+        row that the group's first slot has in the page table: a group is set anew before that slot lets go of them."""
         groups = [([int(s) for s in slots], int(tokens)) for slots, tokens in groups]
         every = [s for slots, _ in groups for s in slots]
         if len(set(every)) != len(every) or any(not 0 <= s < self.num_seqs for s in every):
             raise ValueError(f"slots {sorted(every)} of {self.num_seqs}")
         if any(tokens < 0 or tokens % PAGE for _, tokens in groups):
             raise ValueError(f"prefixes of {[t for _, t in groups]} tokens: whole pages of {PAGE} are shared")
+        if self._cuts and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("groups are set between captured calls, which follow them")
         self.groups = [(slots, tokens) for slots, tokens in groups if len(slots) > 1 and tokens]      # a slot alone shares nothing
         self.longest = max((t for _, t in self.groups), default=0)
         covered = sum(len(slots) for slots, _ in self.groups)
@@ -152,7 +156,8 @@ def attn_decode_shared(q: torch.Tensor, hq: int, seq_lens: torch.Tensor, cache: 
                        out: torch.Tensor, *, splits: int | None = None) -> torch.Tensor:
     """The last token of every slot (row b of q, already rotated, [B, hq dk], row stride free; its key is in the cache) against the first
     ``seq_lens[b]`` cached tokens of slot b.  Slots of a group of ``shared`` have the same pages in front, which are read once for all of them (bf16 heads of up
-    to 128, pages of 16; otherwise every slot reads its own way through ``attn_paged``).  An empty slot (length 0) gets zeros.
+    to 128, pages of 16; otherwise every slot reads its own way through ``attn_paged``); a slot that does not see the prefix up to its end, being shorter or in a later
+    chunk, reads alone.  An empty slot (length 0) gets zeros.
 
     ``splits``: CTAs that share a slot's own keys."""
     B = seq_lens.numel()

@@ -44,7 +44,7 @@ def _sparse(**kw):
 
 
 @pytest.mark.parametrize("kw", [dict(top=2), dict(last=0), dict(first=-1), dict(scale=0.0), dict(scale=-1.0), dict(table=torch.zeros(2, 40, dtype=torch.int32)),
-                                dict(cache=_cache(dk=520)), dict(cache=_cache(dv=0)), dict(bounds=torch.zeros(6, 2, 2, 32))])
+                                dict(cache=_cache(dk=520)), dict(cache=_cache(dv=0)), dict(top=140000, table=torch.zeros(3, 150000, dtype=torch.int32)), dict(bounds=torch.zeros(6, 2, 2, 32))])
 def test_selections_that_make_no_sense_are_refused(kw):
     with pytest.raises(ValueError):
         _sparse(**kw)
@@ -56,7 +56,7 @@ def test_groups_that_make_no_sense_are_refused(groups):
         SH.SharedPrefixes(4, "cpu").set(groups)
 
 
-@pytest.mark.parametrize("pairs,pages,want", [(8, 128, 8), (64, 64, 2), (512, 256, 1), (20, 100, 4), (2, 31, 1), (1, 32, 2)])
+@pytest.mark.parametrize("pairs,pages,want", [(8, 128, 8), (64, 64, 2), (512, 256, 1), (20, 100, 4), (2, 31, 1), (1, 32, 2), (4000, 65536, 4), (300, 16384, 1)])
 def test_clusters_for_selections(pairs, pages, want):
     assert SP.pick_sparse_splits(pairs, pages) == want
 
@@ -97,3 +97,18 @@ def test_pieces_of_prefixes_cover_every_row_and_key_once(per_head, kv_heads, gro
                 assert sorted(k for tiles, _ in runs for k in tiles) == list(range(0, tokens, 128))
                 assert sorted(at for _, at in runs) == [first + h + k * step for k in range(parts)]
     assert not seen and all(info[4 * s + 2] == 0 for s in range(n) if s not in set(order))
+
+
+@pytest.mark.parametrize("chunk", [1, 16, 50, 128, 300, 4096])
+def test_pieces_begin_where_the_chunk_of_a_prefix_does(chunk):
+    """From the first page behind the last multiple of the chunk: what every slot sees that is as long and whose own chunk begins in front of the prefix's end."""
+    groups = [([2 * i, 2 * i + 1], 16 * (1 + 3 * i)) for i in range(20)]
+    info, pieces, order, rows = SH.cut_prefixes(groups, 40, 4, 2, 148, 0, chunk)
+    for slots, tokens in groups:
+        begin = min(tokens, -(-((tokens - 1) // chunk * chunk) // 16) * 16)
+        mine = sorted((p[3], p[4]) for p in pieces if p[6] == slots[0])
+        assert all(info[4 * s + 2] == 0 for s in slots) if begin == tokens else all(info[4 * s + 3] == tokens for s in slots)
+        assert [a for a, _ in mine] + [tokens] == [begin] + [b for _, b in mine]
+        for n in range(tokens, tokens + 2 * chunk, max(1, chunk // 7)):
+            low = (n - 1) - (n - 1) % chunk
+            assert low >= tokens or begin - 16 < low <= begin

@@ -154,3 +154,83 @@ def test_the_same_call_gives_the_same_bits():
     first = _check(S, q, S.lens, groups, 0.09).clone()
     for _ in range(5):
         assert torch.equal(_check(S, q, S.lens, groups, 0.09), first)
+
+
+@pytest.mark.parametrize("hq,hkv,dk,dv,n", [(16, 4, 128, 128, 170), (8, 8, 40, 64, 90), (40, 2, 64, 64, 120), (48, 4, 128, 96, 80)])
+def test_more_slots_than_ctas(hq, hkv, dk, dv, n):
+    """Empty slots, slots that share nothing and sequences of any length among them, in several waves; twice, and the same bits."""
+    groups = [(list(range(0, n, 2)), 272), ([1, 3, 5, 7], 128)]
+    lens = [0] * n
+    for i in range(n):
+        base = 272 if i % 2 == 0 else 128 if i in (1, 3, 5, 7) else 0
+        lens[i] = 0 if i % 11 == 10 and base == 0 else base + (i * 37) % 200
+    S = Sequences([max(1, x) for x in lens], hq, hkv, dk, dv, "bfloat16", groups=groups, seed=n)
+    q = S.rows_of(n, 8)
+    s, g = S.heads_of(n)
+    first = _check(S, q, lens, groups, dk ** -0.5, s, g).clone()
+    assert torch.equal(_check(S, q, lens, groups, dk ** -0.5, s, g), first)
+    _check(S, q, lens, groups, dk ** -0.5, s, g, chunk=150)
+
+
+@pytest.mark.parametrize("chunk", [None, 40, 100])
+@pytest.mark.parametrize("hq,hkv,dk,dv", [(16, 4, 128, 128), (96, 4, 64, 80)])
+def test_more_pieces_than_ctas(hq, hkv, dk, dv, chunk):
+    """A CTA takes several pieces one after the other: of groups with one, two or some tiles, with rows for one unit or for both, seen in full, in part or not at all."""
+    groups, lens, at = [], [], 0
+    for i in range(70):
+        members, tokens = 2 + (i % 7 == 3) * (12 if hq == 96 else 40), 16 * (1 + (i * 5) % 23)
+        groups.append((list(range(at, at + members)), tokens))
+        lens += [tokens + (i + j * 3) % 50 for j in range(members)]
+        at += members
+    S = Sequences(lens, hq, hkv, dk, dv, "bfloat16", groups=groups, seed=7)
+    q = S.rows_of(len(lens))
+    s, g = S.heads_of(len(lens))
+    first = _check(S, q, lens, groups, dk ** -0.5, s, g, chunk).clone()
+    assert torch.equal(_check(S, q, lens, groups, dk ** -0.5, s, g, chunk), first)
+
+
+def test_groups_are_not_set_inside_a_capture():
+    from mojo_linuxperiments_b200.ops import shared as SH
+    groups = [([0, 1], 32)]
+    S = Sequences([40, 40], 4, 2, 64, 64, "bfloat16", groups=groups)
+    plan = SH.SharedPrefixes(2, DEV)
+    q = S.rows_of(2)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            with pytest.raises(RuntimeError, match="capture"):
+                _run(S, q, [40, 40], plan, 0.1, None, None)            # the plan is not on the device yet
+            torch.zeros(1, device=DEV).add_(1)
+        _run(S, q, [40, 40], plan, 0.1, None, None)
+        with torch.cuda.graph(g := torch.cuda.CUDAGraph(), stream=side):
+            with pytest.raises(RuntimeError, match="captured"):
+                plan.set(groups)
+            torch.zeros(1, device=DEV).add_(1)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("chunk,lens,right", [(None, [320, 500, 100, 16, 0, 99], [2, 3, 4, 5]), (50, [320, 700, 321, 100, 319, 0], range(6)),
+                                              (304, [320, 700, 321, 319, 100, 0], range(6)), (128, [320, 400, 500, 321, 50, 0], [1, 2, 4, 5])])
+@pytest.mark.parametrize("hq", [8, 120])
+def test_what_a_slot_does_not_see_may_be_anything(chunk, lens, right, hq, bad):
+    """Positions 100 .. 299 of the prefix are not finite: rows that see none of them are as they would be without."""
+    groups = [([2, 0, 1, 3, 4, 5], 320)]
+    S = Sequences(lens, hq, 2, 64, 64, "bfloat16", groups=groups, seed=3)
+    for at in range(100, 300):
+        S.cache.keys()[S.rows[0][at // 16], :, at % 16] = bad
+        S.cache.values()[S.rows[0][at // 16], :, at % 16] = bad
+    q = S.rows_of(6)
+    from mojo_linuxperiments_b200.ops import shared as SH
+    plan = SH.SharedPrefixes(6, DEV)
+    plan.set(groups)
+    out = _run(S, q, lens, plan, 0.1, None, None, chunk)
+    status_ok()
+    for i in right:
+        n = lens[i]
+        low = (n - 1) - (n - 1) % chunk if chunk and n else 0
+        assert not set(range(100, 300)) & set(range(low, n))
+        want, tol = S.want(q, i, i, list(range(low, n)), 0.1, None, None)
+        assert worst(out[i], want, tol) <= 1, (i, worst(out[i], want, tol))
