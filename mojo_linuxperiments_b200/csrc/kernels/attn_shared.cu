@@ -68,6 +68,7 @@ constexpr int SX_THREADS = 384, SX_BN = 128, SX_PS = 16;
 // registers: 384 x 168 at launch, 128 x (72 + 216 + 216) afterwards, which is as many
 constexpr int SX_REGS_FEW = 72, SX_REGS_MANY = 216;
 constexpr int SX_CHUNK = 128 * 128, SX_TILE = 2 * SX_CHUNK;
+constexpr float SX_LAZY = 8.f;
 constexpr int SX_SMEM = 6 * SX_TILE + 1024 + 256;
 
 __global__ void __launch_bounds__(SX_THREADS, 1)
@@ -287,7 +288,8 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
             mx[c] = fmaxf(mx[c], __uint_as_float(v[c][31]));
           }
           const float m_new = fmaxf(m_ref, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2);
-          if (__any_sync(0xffffffffu, m_new > m_ref)) {
+          // weights are taken against an older maximum until one would pass 2^8: they are relative numbers, and O is seldom scaled
+          if (__any_sync(0xffffffffu, m_new > m_ref + SX_LAZY)) {
             const float alpha = m_ref == -INFINITY ? 0.f : dw_exp2(m_ref - m_new);
             l *= alpha;
             m_ref = m_new;
