@@ -60,8 +60,8 @@ __device__ __forceinline__ void sx_copy16(uint32_t dst, const void* src, bool on
 __device__ __forceinline__ void sx_copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // ---- prefixes -----------------------------------------------------------------------------------------------------------------------
-// One CTA per SM with two units, which take turns on the tensor cores: warp 0 fetches pages by TMA (lane <-> page) into two-stage rings, warp 1 issues the
-// MMAs, warps 4..7 and 8..11 gather the queries of a unit, take its softmax (thread <-> row) and keep O in tensor memory.  Where a group has more than 128 rows
+// One CTA per SM with two units, which take turns on the tensor cores: warp 0 fetches pages by TMA (lane <-> page; one box for a page of rows of 128,
+// whose requests take half the time of two) into two-stage rings, warp 1 issues the MMAs, warps 4..7 and 8..11 gather the queries of a unit, take its softmax (thread <-> row) and keep O in tensor memory.  Where a group has more than 128 rows
 // the units share the keys, otherwise each has every other tile.  Results are stored with the rows of a tile next to each other, so that a warp's stores and the loads of
 // a slot's heads are whole sectors.
 constexpr int SX_THREADS = 384, SX_BN = 128, SX_PS = 16;
@@ -80,7 +80,7 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
   const uint32_t sQ = smem_u32(smem), sK = sQ + 2 * SX_TILE, sV = sK + 2 * SX_TILE;        // two units, two stages, two stages
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 6 * SX_TILE);
   const uint32_t bar0 = smem_u32(bars);
-  enum { B_KFULL = 0, B_KEMPTY = 2, B_VFULL = 4, B_VEMPTY = 6, B_SFULL = 8, B_PFULL = 10, B_OFULL = 12, B_COUNT = 14 };      // two of each: stages or units
+  enum { B_KFULL = 0, B_KEMPTY = 2, B_VFULL = 4, B_VEMPTY = 6, B_SFULL = 8, B_PFULL = 10, B_OFULL = 14, B_COUNT = 16 };      // two of each: stages or units; P in two halves
   auto bar = [&](int i) { return bar0 + 8u * i; };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + B_COUNT);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -89,8 +89,9 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int dk = p.c.dk, dv = p.c.dv, hkv = p.c.kv_heads, group = p.hq / hkv;
   const int kchunks = (dk + 63) >> 6, vchunks = (dv + 63) >> 6, ksteps = (dk + 15) >> 4, dv16 = (dv + 15) & ~15;
+  const bool kwhole = dk == 128, vwhole = dv == 128;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < B_COUNT; ++i) mbar_init(bar(i), (i & ~1) == B_PFULL ? 4 : 1);
+    for (int i = 0; i < B_COUNT; ++i) mbar_init(bar(i), i >= B_PFULL && i < B_OFULL ? 4 : 1);
     *abort_flag = 0;
     seen[0] = seen[1] = 0;
     mbar_fence_init();
@@ -143,10 +144,11 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
           return p.c.num_pages;
         };
         int ids = 0, ids_next = 0;
-        auto load = [&](uint32_t dst, const CUtensorMap* m, int b, int chunks, int pg) {
+        auto load = [&](uint32_t dst, const CUtensorMap* m, int b, int chunks, bool whole, int pg) {
           if (lane == 0) mbar_expect_tx(bar(b), chunks * SX_CHUNK);
           __syncwarp();
-          if (lane < 8)
+          if (lane < 8 && whole) tma_load_5d(dst + lane * 4096, m, bar(b), 0, 0, 0, 2 * kvh, pg);
+          else if (lane < 8)
             for (int c = 0; c < chunks; ++c) tma_load_3d(dst + c * SX_CHUNK + lane * 2048, m, bar(b), c * 64, kvh * SX_PS, pg);
         };
         auto fetch = [&](int j) {
@@ -156,10 +158,10 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
           const uint32_t ph = (((kv + j) >> 1) & 1u) ^ 1u;
           ok = __all_sync(0xffffffffu, wait(B_KEMPTY + st, ph, ST_TIMEOUT_SMEM_EMPTY)) != 0;
           if (!ok) return;
-          load(sK + st * SX_TILE, &tmap_k, B_KFULL + st, kchunks, page);
+          load(sK + st * SX_TILE, &tmap_k, B_KFULL + st, kchunks, kwhole, page);
           ok = __all_sync(0xffffffffu, wait(B_VEMPTY + st, ph, ST_TIMEOUT_SMEM_EMPTY)) != 0;
           if (!ok) return;
-          load(sV + st * SX_TILE, &tmap_v, B_VFULL + st, vchunks, page);
+          load(sV + st * SX_TILE, &tmap_v, B_VFULL + st, vchunks, vwhole, page);
         };
         // without chunks the keys are known before the queries are in place, and nobody waits for this warp
         if (p.chunk > 0) meet(M_QUERIES); else named_bar_arrive(M_QUERIES, SX_THREADS);
@@ -174,7 +176,9 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
           const bool one = elect_one();
           constexpr uint32_t IDESC_S = umma_idesc_bf16(128, 128, 0, 0);
           const uint32_t idesc_pv = umma_idesc_bf16(128, dv16, 0, 1);
-          const uint64_t q_desc = umma_desc_k_sw128(sQ), k_desc = umma_desc_k_sw128(sK), v_desc = umma_desc_mn_sw128(sV, SX_CHUNK, 1024);
+          const uint64_t q_desc = umma_desc_k_sw128(sQ), k_desc = umma_desc_mn_sw128(sK, 16, kwhole ? 2048 : 1024);
+          const uint64_t v_desc = umma_desc_mn_sw128(sV, vwhole ? 1024 : SX_CHUNK, vwhole ? 2048 : 1024);
+          const uint32_t k_chunk = (kwhole ? 1024 : SX_CHUNK) >> 4, v_step = (vwhole ? 4096 : 2048) >> 4;
           const int units = units_of(e), lag = e.mode == SM_KEYS ? 2 : 1;      // tiles between two of a unit
           bool ok = true;
           // the product of tile j - lag and the scores of tile j, which go to where its weights were
@@ -186,14 +190,18 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
 #pragma unroll 1
             for (int u = e.mode == SM_KEYS ? j & 1 : 0; u < (e.mode == SM_KEYS ? (j & 1) + 1 : units) && ok; ++u) {
               if (past >= 0) {
-                ok = wait(B_PFULL + u, (p_par >> u) & 1u, ST_TIMEOUT_TMEM_EMPTY);
-                if (!ok) break;
-                p_par ^= 1u << u;
-                tc_fence_after();
                 const uint64_t bd = v_desc + vs * (SX_TILE >> 4);
 #pragma unroll
-                for (int kk = 0; kk < 8; ++kk)
-                  if (one) umma_f16_ts(tmem + 256 + u * 128, tmem + u * 128 + kk * 8, bd + kk * (2048 >> 4), idesc_pv, (past >= lag || kk > 0) ? 1u : 0u);
+                for (int half = 0; half < 2; ++half) {
+                  ok = wait(B_PFULL + 2 * u + half, (p_par >> u) & 1u, ST_TIMEOUT_TMEM_EMPTY);
+                  if (!ok) break;
+                  tc_fence_after();
+#pragma unroll
+                  for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
+                    if (one) umma_f16_ts(tmem + 256 + u * 128, tmem + u * 128 + kk * 8, bd + kk * v_step, idesc_pv, (past >= lag || kk > 0) ? 1u : 0u);
+                }
+                if (!ok) break;
+                p_par ^= 1u << u;
                 if (one && past + lag >= n) umma_commit(bar(B_OFULL + u));
               }
               if (j < n) {
@@ -201,8 +209,8 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
                 const uint64_t ad = q_desc + static_cast<uint32_t>(u * (SX_TILE >> 4)), bd = k_desc + ks * (SX_TILE >> 4);
 #pragma unroll
                 for (int kk = 0; kk < 8; ++kk) {
-                  const uint32_t off = (kk >> 2) * (SX_CHUNK >> 4) + 2 * (kk & 3);
-                  if (one && kk < ksteps) umma_f16_ss(tmem + u * 128, ad + off, bd + off, IDESC_S, kk > 0 ? 1u : 0u);
+                  const uint32_t at_q = (kk >> 2) * (SX_CHUNK >> 4) + 2 * (kk & 3), at_k = (kk >> 2) * k_chunk + 2 * (kk & 3);
+                  if (one && kk < ksteps) umma_f16_ss(tmem + u * 128, ad + at_q, bd + at_k, IDESC_S, kk > 0 ? 1u : 0u);
                 }
                 if (one) umma_commit(bar(B_SFULL + u));
               }
@@ -322,6 +330,12 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
               sum[i & 1] = sx_add2(sum[i & 1], sx_pair(e0, e1));
             }
             tmem_st_x16(t_s + c * 16, pk);
+            if (c == 1) {                        // the product of the first half may begin
+              tmem_st_wait();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(bar(B_PFULL + 2 * u));
+            }
           }
           float l0, l1, l2, l3;
           sx_split(sum[0], l0, l1);
@@ -331,7 +345,10 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(B_PFULL + u));
+        if (lane == 0) {
+          if (idle) mbar_arrive(bar(B_PFULL + 2 * u));
+          mbar_arrive(bar(B_PFULL + 2 * u + 1));
+        }
       }
       if (threadIdx.x == 128) B200_TRACE(TK_ATTN_SHARED, 4); // last weights
       const bool some = j0 < n;
@@ -565,9 +582,16 @@ extern "C" int b200_attn_decode_shared(const void* q, long long ldq, void* out, 
       (reinterpret_cast<uintptr_t>(part) & 15)) return -4;
   const uint64_t rec = static_cast<uint64_t>(c->kv_heads) * SX_PS * (c->dk + c->dv) * 2, kbytes = static_cast<uint64_t>(c->kv_heads) * SX_PS * c->dk * 2;
   CUtensorMap tk, tv;
-  if (make_tmap_3d_bf16(&tk, c->data, c->dk, static_cast<uint64_t>(c->kv_heads) * SX_PS, c->num_pages, static_cast<uint64_t>(c->dk) * 2, rec, SX_PS, 1)) return -12;
-  if (make_tmap_3d_bf16(&tv, static_cast<const uint8_t*>(c->data) + kbytes, c->dv, static_cast<uint64_t>(c->kv_heads) * SX_PS, c->num_pages,
-                        static_cast<uint64_t>(c->dv) * 2, rec, SX_PS, 1)) return -13;
+  // rows of 128 numbers: a page at once, its two groups of eight keys, in each the two halves of their rows
+  auto whole = [&](CUtensorMap* m, const void* base) {
+    const uint64_t row = 256, n[5] = {64, 8, 2, static_cast<uint64_t>(c->kv_heads) * 2, static_cast<uint64_t>(c->num_pages)}, pitch[4] = {row, 128, 8 * row, rec};
+    const uint32_t box[5] = {64, 8, 2, 2, 1};
+    return make_tmap_5d_bf16(m, base, n, pitch, box);
+  };
+  const uint8_t* values = static_cast<const uint8_t*>(c->data) + kbytes;
+  const uint64_t keys = static_cast<uint64_t>(c->kv_heads) * SX_PS;
+  if (c->dk == 128 ? whole(&tk, c->data) : make_tmap_3d_bf16(&tk, c->data, c->dk, keys, c->num_pages, static_cast<uint64_t>(c->dk) * 2, rec, SX_PS, 1)) return -12;
+  if (c->dv == 128 ? whole(&tv, values) : make_tmap_3d_bf16(&tv, values, c->dv, keys, c->num_pages, static_cast<uint64_t>(c->dv) * 2, rec, SX_PS, 1)) return -13;
   SharedParams p = {};
   p.q = static_cast<const __nv_bfloat16*>(q); p.ldq = ldq; p.out = static_cast<__nv_bfloat16*>(out); p.ldo = ldo; p.hq = hq; p.B = B; p.seq_lens = seq_lens;
   p.plan = plan; p.pieces_at = pieces_at; p.slots_at = slots_at; p.max_pieces = max_pieces; p.part = part; p.part_rows = part_rows; p.c = *c; p.chunk = s->chunk;

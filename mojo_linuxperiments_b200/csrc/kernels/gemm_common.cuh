@@ -16,5 +16,7 @@ int make_tmap_2d_u8(CUtensorMap* out, const void* base, uint64_t cols, uint64_t 
 // bf16 [n2][n1][n0] with pitches in bytes; box = 64 columns x rows1 x rows2, 128-byte swizzle, zero fill outside.
 int make_tmap_3d_bf16(CUtensorMap* out, const void* base, uint64_t n0, uint64_t n1, uint64_t n2, uint64_t pitch1,
                       uint64_t pitch2, uint32_t rows1, uint32_t rows2);
+// any five dimensions (sizes in elements, pitches in bytes), box rows[0..4], rows[0] = 64 elements, 128-byte swizzle
+int make_tmap_5d_bf16(CUtensorMap* out, const void* base, const uint64_t (&n)[5], const uint64_t (&pitch)[4], const uint32_t (&rows)[5]);
 
 }  // namespace b200

@@ -49,4 +49,17 @@ int make_tmap_3d_bf16(CUtensorMap* out, const void* base, uint64_t n0, uint64_t 
   return r == CUDA_SUCCESS ? 0 : -static_cast<int>(r);
 }
 
+int make_tmap_5d_bf16(CUtensorMap* out, const void* base, const uint64_t (&n)[5], const uint64_t (&pitch)[4], const uint32_t (&rows)[5]) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (!fn) return -1;
+  cuuint64_t dims[5], strides[4];
+  cuuint32_t box[5], estr[5];
+  for (int i = 0; i < 5; ++i) { dims[i] = n[i]; box[i] = rows[i]; estr[i] = 1; }
+  for (int i = 0; i < 4; ++i) strides[i] = pitch[i];
+  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -static_cast<int>(r);
+}
+
 }  // namespace b200
