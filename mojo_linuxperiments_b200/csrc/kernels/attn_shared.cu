@@ -526,16 +526,28 @@ __global__ void __launch_bounds__(SO_THREADS, NH == 1 ? 3 : 2) attn_shared_own_k
     const int d = i / G * 4, g = i - i / G * G;              // heads side by side, as the parts of the prefix have them
     const float* f = share + g * (8 + SO_PARTS);
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int s = 0; s < S; ++s) {
-      const float4 x = dw_ld_cluster4(own_addr + 4u * (g * Sh::PITCH + d), s, S > 1);
-      v.x += f[s] * x.x; v.y += f[s] * x.y; v.z += f[s] * x.z; v.w += f[s] * x.w;
+    // (in batches of which none is cut short: what is left of a loop would wait for each of its loads)
+    auto take = [&](float w, const float4& x) { v.x += w * x.x; v.y += w * x.y; v.z += w * x.z; v.w += w * x.w; };
+    const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int s = 0; s < S; s += 4) {
+      float4 x[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = s + k < S ? dw_ld_cluster4(own_addr + 4u * (g * Sh::PITCH + d), s + k, S > 1) : none;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) if (s + k < S) take(f[s + k], x[k]);
     }
-#pragma unroll 8
-    for (int s = 0; s < n_parts; ++s) {
-      const float fs = f[S + s];                 // zero: perhaps a part without keys, which has left no numbers
-      const float4 x = fs != 0.f ? __ldcg(parts + static_cast<size_t>(d >> 2) * p.part_rows + static_cast<size_t>(s) * info.y + g) : make_float4(0.f, 0.f, 0.f, 0.f);
-      v.x += fs * x.x; v.y += fs * x.y; v.z += fs * x.z; v.w += fs * x.w;
+#pragma unroll 1
+    for (int s = 0; s < n_parts; s += 8) {
+      float4 x[8];
+      float fs[8];                               // zero: perhaps a part without keys, which has left no numbers
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        fs[k] = s + k < n_parts ? f[S + s + k] : 0.f;
+        x[k] = fs[k] != 0.f ? __ldcg(parts + static_cast<size_t>(d >> 2) * p.part_rows + static_cast<size_t>(s + k) * info.y + g) : none;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) take(fs[k], x[k]);
     }
     const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), c = __floats2bfloat162_rn(v.z, v.w);
     *reinterpret_cast<uint2*>(p.out + static_cast<size_t>(b) * p.ldo + static_cast<size_t>(h0 + g) * dv + d) =
