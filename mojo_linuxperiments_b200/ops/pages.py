@@ -57,8 +57,9 @@ def bounds_for(cache: PagedKVCache) -> torch.Tensor:
 
 
 def check_bounds(cache: PagedKVCache, bounds: torch.Tensor) -> None:
-    if bounds.shape != (cache.num_pages, cache.kv_heads, 2, cache.dk) or bounds.dtype != cache.data.dtype or not bounds.is_contiguous() \
-            or bounds.get_device() != cache.data.get_device():
+    data = cache.data
+    if bounds.shape != (cache.num_pages, cache.kv_heads, 2, cache.dk) or bounds.dtype != data.dtype or not bounds.is_contiguous() \
+            or bounds.get_device() != data.get_device():
         raise ValueError(f"bounds {tuple(bounds.shape)} {bounds.dtype} of a cache of {cache.num_pages} pages, {cache.kv_heads} heads of {cache.dk}, {cache.data.dtype}")
 
 
@@ -70,7 +71,7 @@ def page_bounds(cache: PagedKVCache, page_table: torch.Tensor, starts: torch.Ten
     portion only.  A portion of no tokens, as of an empty slot, changes nothing.  Exact; NaN where a key is."""
     check_bounds(cache, bounds)
     n = starts.numel()
-    assert starts.dtype == ends.dtype == page_table.dtype == torch.int32 and ends.numel() == n and all(t.is_contiguous() for t in (starts, ends, page_table))
+    assert starts.dtype == ends.dtype == page_table.dtype == torch.int32 and ends.numel() == n and starts.is_contiguous() and ends.is_contiguous() and page_table.is_contiguous()
     if seq_ids is None:
         if n > page_table.shape[0]:
             raise ValueError(f"{n} portions of {page_table.shape[0]} sequences")

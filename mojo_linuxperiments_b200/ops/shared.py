@@ -160,27 +160,30 @@ def attn_decode_shared(q: torch.Tensor, hq: int, seq_lens: torch.Tensor, cache: 
     chunk, reads alone.  An empty slot (length 0) gets zeros.
 
     ``splits``: CTAs that share a slot's own keys."""
-    B = seq_lens.numel()
-    assert q.dtype == cache.data.dtype == out.dtype and q.stride(1) == 1 and out.stride(1) == 1 and q.shape[0] == out.shape[0] == B
-    assert q.shape[1] >= hq * cache.dk and out.shape[1] >= hq * cache.dv and hq % cache.kv_heads == 0
+    B, dk, dv, kv_heads, data = seq_lens.numel(), cache.dk, cache.dv, cache.kv_heads, cache.data
+    (rows, width), (out_rows, out_width), (seqs, pages) = q.shape, out.shape, page_table.shape
+    (ldq, q_step), (ldo, out_step), dtype, device = q.stride(), out.stride(), data.dtype, q.device
+    assert q.dtype == dtype == out.dtype and q_step == 1 and out_step == 1 and rows == out_rows == B
+    assert width >= hq * dk and out_width >= hq * dv and hq % kv_heads == 0
     assert seq_lens.dtype == page_table.dtype == torch.int32 and page_table.is_contiguous() and seq_lens.is_contiguous()
-    room = page_table.shape[1] * cache.page_size
-    if B > page_table.shape[0] or B != shared.num_seqs or shared.longest > room:
-        raise ValueError(f"{B} rows, {page_table.shape[0]} sequences of up to {room} tokens, a plan for {shared.num_seqs} with prefixes of up to {shared.longest}")
-    L, desc = _lib.lib(), cache.desc(page_table)
-    if not L.b200_attn_decode_shared_takes(ctypes.byref(desc), hq, q.stride(0), out.stride(0)) or q.data_ptr() % 16 or out.data_ptr() % 8:
-        rc = _lib.on_device(q.device, L.b200_attn_paged, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), hq, B, None, None, seq_lens.data_ptr(),
-                            ctypes.byref(desc), ctypes.byref(spec), default_workspace(q.device).status.data_ptr())
+    room = pages * cache.page_size
+    if B > seqs or B != shared.num_seqs or shared.longest > room:
+        raise ValueError(f"{B} rows, {seqs} sequences of up to {room} tokens, a plan for {shared.num_seqs} with prefixes of up to {shared.longest}")
+    if not q.get_device() == out.get_device() == data.get_device() == page_table.get_device() == seq_lens.get_device() >= 0:
+        raise ValueError("tensors on one GPU")
+    L, desc, q_at, out_at, status = _lib.lib(), cache.desc(page_table), q.data_ptr(), out.data_ptr(), default_workspace(device).status.data_ptr()
+    if dtype != torch.bfloat16 or cache.page_size != PAGE or dk > 128 or dv > 128 or (dk | dv | ldq) % 8 or ldo % 4 or q_at % 16 or out_at % 8 or data.data_ptr() % 16:
+        rc = _lib.on_device(device, L.b200_attn_paged, q_at, ldq, out_at, ldo, hq, B, None, None, seq_lens.data_ptr(), ctypes.byref(desc), ctypes.byref(spec), status)
         _lib.check(rc, "attn_paged")
         return out
     cut = shared.cut_for(hq, cache, spec.chunk)
     if splits is None:
         keys = min(room - shared.alone, spec.chunk) if spec.chunk > 0 else room - shared.alone
-        splits = pick_decode_splits_paged(B, cache.kv_heads * ((hq // cache.kv_heads + 15) // 16), keys, cut.sms)
+        splits = pick_decode_splits_paged(B, kv_heads * ((hq // kv_heads + 15) // 16), keys, cut.sms)
     rc = _lib.on_device(
-        q.device, L.b200_attn_decode_shared, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), hq, B, seq_lens.data_ptr(), ctypes.byref(desc),
+        device, L.b200_attn_decode_shared, q_at, ldq, out_at, ldo, hq, B, seq_lens.data_ptr(), ctypes.byref(desc),
         ctypes.byref(spec), cut.plan.data_ptr(), cut.pieces_at, cut.slots_at, cut.max_pieces, cut.part.data_ptr(), cut.rows, splits, cut.sms,
-        default_workspace(q.device).status.data_ptr())
+        status)
     _lib.check(rc, "attn_decode_shared")
     _lib.LAUNCHES[0] += 1                        # two kernels
     return out

@@ -12,6 +12,7 @@ from .workspace import default_workspace
 
 MAX_HEAD_DIM = 512
 MAX_ROWS = 65535
+MAX_QUERIES = 50 << 10         # numbers of a group's queries, heads padded to 128, that shared memory holds
 LIST_PER_CTA = 16384           # pages that a CTA may have to read
 
 
@@ -40,29 +41,33 @@ def attn_paged_sparse(q: torch.Tensor, hq: int, positions: torch.Tensor, seq_ids
     if not spec.scale > 0:
         raise ValueError("scores bound products with a positive scale")
     check_bounds(cache, bounds)
-    assert q.dtype == cache.data.dtype == out.dtype and q.stride(1) == 1 and out.stride(1) == 1 and q.shape[0] == out.shape[0] == M
-    assert q.shape[1] >= hq * cache.dk and out.shape[1] >= hq * cache.dv and hq % cache.kv_heads == 0
+    dk, dv, kv_heads, dtype, device = cache.dk, cache.dv, cache.kv_heads, cache.data.dtype, q.device
+    (rows, width), (out_rows, out_width), (seqs, most) = q.shape, out.shape, page_table.shape
+    (ldq, q_step), (ldo, out_step) = q.stride(), out.stride()
+    assert q.dtype == dtype == out.dtype and q_step == 1 and out_step == 1 and rows == out_rows == M
+    assert width >= hq * dk and out_width >= hq * dv and hq % kv_heads == 0
     assert positions.dtype == page_table.dtype == torch.int32 and page_table.is_contiguous() and positions.is_contiguous()
     for t in (seq_ids, seq_lens):
         assert t is None or (t.dtype == torch.int32 and t.is_contiguous() and t.numel() == M)
-    if max(cache.dk, cache.dv) > MAX_HEAD_DIM or cache.dv == 0 or (hq // cache.kv_heads) * (cache.dk + 127 & ~127) > 50 << 10:
-        raise ValueError(f"{hq} heads of {cache.dk} and {cache.dv} over {cache.kv_heads}")
-    if M > MAX_ROWS or min(top, page_table.shape[1]) > 8 * LIST_PER_CTA:
+    group = hq // kv_heads
+    if dk > MAX_HEAD_DIM or dv > MAX_HEAD_DIM or dv == 0 or group * (dk + 127 & ~127) > MAX_QUERIES:
+        raise ValueError(f"{hq} heads of {dk} and {dv} over {kv_heads}")
+    if M > MAX_ROWS or min(top, most) > 8 * LIST_PER_CTA:
         raise ValueError(f"{M} rows and {top} pages in one call")
-    if seq_ids is None and M > page_table.shape[0]:
-        raise ValueError(f"{M} rows of {page_table.shape[0]} sequences")
+    if seq_ids is None and M > seqs:
+        raise ValueError(f"{M} rows of {seqs} sequences")
+    if not q.get_device() == out.get_device() == bounds.get_device() == page_table.get_device() == positions.get_device() >= 0:
+        raise ValueError("tensors on one GPU")
     if chosen is not None:
-        assert chosen.dtype == torch.int32 and tuple(chosen.shape) == (M, cache.kv_heads, top) and chosen.is_contiguous()
-    most = page_table.shape[1]
+        assert chosen.dtype == torch.int32 and tuple(chosen.shape) == (M, kv_heads, top) and chosen.is_contiguous()
     if splits is None:
         seen = min(most, spec.chunk // cache.page_size + 2) if spec.chunk > 0 else most
-        splits = pick_sparse_splits(M * cache.kv_heads * ((hq // cache.kv_heads + 15) // 16), min(top, seen), _lib.num_sms(q.device.index),
-                                    16 if q.dtype == torch.bfloat16 else 4)
-    scores = torch.empty(M * cache.kv_heads * most, dtype=torch.int32, device=q.device)
+        splits = pick_sparse_splits(M * kv_heads * ((group + 15) // 16), min(top, seen), _lib.num_sms(device.index), 16 if dtype == torch.bfloat16 else 4)
+    scores = torch.empty(M * kv_heads * most, dtype=torch.int32, device=device)
     rc = _lib.on_device(
-        q.device, _lib.lib().b200_attn_paged_sparse, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), hq, M, positions.data_ptr(), _lib.ptr(seq_ids),
+        device, _lib.lib().b200_attn_paged_sparse, q.data_ptr(), ldq, out.data_ptr(), ldo, hq, M, positions.data_ptr(), _lib.ptr(seq_ids),
         _lib.ptr(seq_lens), ctypes.byref(cache.desc(page_table)), bounds.data_ptr(), ctypes.byref(spec), int(top), int(first), int(last), splits,
-        scores.data_ptr(), _lib.ptr(chosen), default_workspace(q.device).status.data_ptr())
+        scores.data_ptr(), _lib.ptr(chosen), default_workspace(device).status.data_ptr())
     _lib.check(rc, "attn_paged_sparse")
     _lib.LAUNCHES[0] += 1                        # two kernels
     return out
