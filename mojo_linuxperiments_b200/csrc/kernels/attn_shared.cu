@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(SO_THREADS, NH == 1 ? 3 : 2) attn_shared_own_k
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     if (p.sink) total += dw_exp2(sink2 - use);
-    float f = total > 0.f ? 1.f / total : 0.f;
+    float f = total > 0.f ? 1.f / total : total;      // nothing, or not a number
     if (p.gate) f *= 1.f / (1.f + __expf(-__bfloat162float(p.gate[static_cast<size_t>(b) * p.ldg + h0 + g])));
     if (lane < all) share[g * (8 + SO_PARTS) + lane] = f0 * f;
     if (lane + 32 < all) share[g * (8 + SO_PARTS) + lane + 32] = f1 * f;

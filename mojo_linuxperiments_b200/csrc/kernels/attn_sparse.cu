@@ -383,13 +383,12 @@ __global__ void __launch_bounds__(PS_THREADS) attn_sparse_any_kernel(const __gri
     for (int r = 0; r < S; ++r) {
       const uint32_t base = (S > 1 ? mapa_shared(j_addr, r) : j_addr) + 4u * (g * pitch);
       const float mr = dw_ld_cluster(base + 4u * (pitch - 4));
-      if (mr == -INFINITY) continue;
-      const float mn = fmaxf(m, mr), fo = m == -INFINITY ? 0.f : expf(m - mn), fn = expf(mr - mn);
+      const float mn = fmaxf(m, mr), use = mn == -INFINITY ? 0.f : mn, fo = expf(m - use), fn = expf(mr - use);
       l = l * fo + fn * dw_ld_cluster(base + 4u * (pitch - 3));
       v = v * fo + fn * dw_ld_cluster(base + 4u * d);
       m = mn;
     }
-    float f = l > 0.f ? 1.f / l : 0.f;
+    float f = l > 0.f ? 1.f / l : l;             // nothing, or not a number
     if (p.s.gate) f *= 1.f / (1.f + expf(-as_f(static_cast<const T*>(p.s.gate)[static_cast<size_t>(tok) * p.s.ldg + h0 + g])));
     o[i] = T(v * f);
   }
@@ -509,7 +508,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) attn_sparse_kernel(const __grid
       v.x += f * y.x; v.y += f * y.y; v.z += f * y.z; v.w += f * y.w;
       l += f * ml[32 * r + 16 + g];
     }
-    float f = l > 0.f ? 1.f / l : 0.f;
+    float f = l > 0.f ? 1.f / l : l;             // nothing, or not a number
     if (p.s.gate) f *= 1.f / (1.f + __expf(-__bfloat162float(static_cast<const bf16*>(p.s.gate)[static_cast<size_t>(tok) * p.s.ldg + h0 + g])));
     *reinterpret_cast<uint2*>(out + g * dv + d) = make_uint2(dw_pack(v.x * f, v.y * f), dw_pack(v.z * f, v.w * f));
   }

@@ -248,11 +248,11 @@ __device__ __forceinline__ void dw_join(const float* parts, int size, int pitch,
     float mw[WARPS], m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) { mw[w] = parts[w * size + 16 * pitch + g]; m = fmaxf(m, mw[w]); }
+    const float use = m == -INFINITY ? 0.f : m;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      if (mw[w] == -INFINITY) continue;          // its numbers are nobody's
-      const float f = dw_exp2(mw[w] - m);
+    for (int w = 0; w < WARPS; ++w) {            // a warp without pages has left zeros
+      const float f = dw_exp2(mw[w] - use);
       const float4 x = *reinterpret_cast<const float4*>(parts + w * size + g * pitch + d);
       v.x += f * x.x; v.y += f * x.y; v.z += f * x.z; v.w += f * x.w;
       l += f * parts[w * size + 16 * pitch + 16 + g];

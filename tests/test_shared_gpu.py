@@ -234,3 +234,20 @@ def test_what_a_slot_does_not_see_may_be_anything(chunk, lens, right, hq, bad):
         assert not set(range(100, 300)) & set(range(low, n))
         want, tol = S.want(q, i, i, list(range(low, n)), 0.1, None, None)
         assert worst(out[i], want, tol) <= 1, (i, worst(out[i], want, tol))
+
+
+@pytest.mark.parametrize("sink", [True, False])
+@pytest.mark.parametrize("hq,hkv,dk,dv", [(4, 2, 64, 64), (160, 1, 64, 32), (40, 2, 128, 128), (6, 2, 40, 56)])
+def test_queries_that_are_not_numbers_give_none(hq, hkv, dk, dv, sink):
+    from mojo_linuxperiments_b200.ops import shared as SH
+    lens, groups = [320, 400, 260, 272], [([0, 1, 2, 3], 256)]
+    S = Sequences(lens, hq, hkv, dk, dv, "bfloat16", groups=groups, seed=2)
+    q = S.rows_of(4)
+    q[0, :dk] = float("nan")
+    q[1, :hq * dk] = float("nan")
+    s, _ = S.heads_of(4, sink, False)
+    plan = SH.SharedPrefixes(4, DEV)
+    plan.set(groups)
+    out = _run(S, q, lens, plan, 0.1, s, None)
+    status_ok()
+    assert torch.isnan(out[0, :dv]).all() and torch.isnan(out[1]).all() and torch.isfinite(out[0, dv:]).all() and torch.isfinite(out[2:]).all()

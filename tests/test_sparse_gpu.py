@@ -223,3 +223,21 @@ def test_more_pages_than_a_selection_holds_at_once(dtype):
             score[0], score[k - 2:] = 1e9, 1e9
             want = torch.sort(score, descending=True, stable=True).indices[:top].sort().values
             assert torch.equal(chosen[i, 0].long(), want), (top, i)
+
+
+@pytest.mark.parametrize("sink", [True, False])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("hq,hkv,dk,dv", [(4, 2, 64, 64), (20, 1, 128, 128), (6, 2, 40, 56)])
+def test_queries_that_are_not_numbers_give_none(hq, hkv, dk, dv, dtype, sink):
+    from mojo_linuxperiments_b200.ops import attention as A
+    from mojo_linuxperiments_b200.ops import sparse as SP
+    S = Sequences([500, 40, 300], hq, hkv, dk, dv, dtype, seed=2)
+    q = S.rows_of(3)
+    q[0, :dk] = float("nan")
+    q[1] = float("nan")
+    s, _ = S.heads_of(3, sink, False)
+    pos = torch.tensor([499, 39, 299], dtype=torch.int32, device=DEV)
+    out = torch.empty((3, hq * dv), dtype=S.dtype, device=DEV)
+    SP.attn_paged_sparse(q, hq, pos, None, S.cache, S.table, _bounds(S), A.attn_spec(0.1, sink=s), out, top=8)
+    status_ok()
+    assert torch.isnan(out[0, :dv]).all() and torch.isnan(out[1]).all() and torch.isfinite(out[0, dv:]).all() and torch.isfinite(out[2]).all()
