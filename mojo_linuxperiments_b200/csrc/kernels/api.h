@@ -347,10 +347,9 @@ int b200_attn_paged(const void* q, long long ldq, void* out, long long ldo, int 
 int b200_attn_paged_sparse(const void* q, long long ldq, void* out, long long ldo, int hq, int M, const int* positions, const int* seq_ids,
                            const int* seq_lens, const b200_paged_cache* cache, const void* bounds, const b200_attn_spec* spec, int top, int first,
                            int last, int splits, unsigned* scores, int* chosen, int* status, cudaStream_t stream);
-// Last tokens of sequences of which some share the pages of a prefix (attn_shared.cu; bf16, dk and dv up to 128, page size 16: _takes says which).  plan: which
+// Last tokens of sequences of which some share the pages of a prefix (attn_shared.cu; bf16, dk and dv up to 128, page size 16; -2 otherwise).  plan: which
 // pieces of which prefixes there are, on the device; part: room for their results, part_rows rows per KV head of dv + 2 floats.  splits: CTAs (a cluster)
 // per slot and KV head for the slot's own keys.
-int b200_attn_decode_shared_takes(const b200_paged_cache* cache, int hq, long long ldq, long long ldo);
 int b200_attn_decode_shared(const void* q, long long ldq, void* out, long long ldo, int hq, int B, const int* seq_lens, const b200_paged_cache* cache,
                             const b200_attn_spec* spec, int* plan, int pieces_at, int slots_at, int max_pieces, float* part, int part_rows,
                             int splits, int num_sms, int* status, cudaStream_t stream);

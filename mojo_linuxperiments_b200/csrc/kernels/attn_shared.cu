@@ -7,6 +7,11 @@
 // up to 256 rows and of some tiles, which leave (m, l, O) in fp32.  Which pieces there are is a list on the device, made when groups change, so that a captured call
 // follows them.  The second takes each sequence's own keys (decode_warp.cuh) while the first still runs, joins the pieces of the prefix, adds sink
 // and gate and writes the output; it waits for the first only there.
+//
+// 4 sequences behind 512 tokens (32 heads over 8, rows of 128): 10.3 us, a chain of latencies: start 0.5, plan and queries 2, tiles 2.5, results 2.5, join 2.
+// 32 behind 2,048 tokens with up to 300 of their own: 17 us.  128 behind 32,768 with up to 1,000 of their own: 125 us, 71 for the prefix, then 54 for the own
+// keys, whose CTAs find no place beside the pieces.  (In one kernel's registers beside the pieces: 166 us and more.  Own keys by as many CTAs as there are places,
+// one slot after the other and the joins shared out at the end: 135 us.)
 #include "ptx.cuh"
 #include "api.h"
 #include "launch.cuh"
@@ -16,14 +21,14 @@
 namespace b200 {
 
 // ---- the plan: int32 on the device -------------------------------------------------------------------------------------------------
-// [0] pieces; [4] pieces of this call that are done, [5] CTAs of the second kernel that have seen it (both zero between calls); at SP_INFO four numbers
+// [0] pieces; [4] pieces of this call that are done, [5] CTAs of the second kernel that have left (both zero between calls); at SP_INFO four numbers
 // per slot: first row of its partial results, rows between the parts of the prefix, parts, tokens; then the pieces, eight numbers each; then the slots of the groups'
 // members.
 //
 // A slot takes either all keys of the pieces of its group or none, so that no row meets a value that it does not see: none if it is shorter than the prefix,
 // or if its chunk begins behind it.  A chunk that begins inside the prefix begins at the same key for every other slot, the last multiple of the chunk in front of
 // the prefix's end; the pieces begin at the first page from there on, and what lies in front of that page is each slot's own.
-constexpr int SP_DONE = 4, SP_SEEN = 5, SP_INFO = 16, SP_PIECE = 8;
+constexpr int SP_DONE = 4, SP_LEFT = 5, SP_INFO = 16, SP_PIECE = 8;
 // member0: of the group, in the list of slots; rows row0 .. row0 + rows of the group (member x query head); keys key0 .. key1; part: first row of the partial
 // results of the group's rows for this run of keys; lead: slot whose pages are read; mode: what the two units of a CTA do, and above it the group's rows
 struct SharedPiece { int member0, row0, rows, key0, key1, part, lead, mode, group_rows; };
@@ -60,15 +65,21 @@ __device__ __forceinline__ void sx_copy16(uint32_t dst, const void* src, bool on
 __device__ __forceinline__ void sx_copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // ---- prefixes -----------------------------------------------------------------------------------------------------------------------
-// One CTA per SM with two units, which take turns on the tensor cores: warp 0 fetches pages by TMA (lane <-> page; one box for a page of rows of 128,
-// whose requests take half the time of two) into two-stage rings, warp 1 issues the MMAs, warps 4..7 and 8..11 gather the queries of a unit, take its softmax (thread <-> row) and keep O in tensor memory.  Where a group has more than 128 rows
-// the units share the keys, otherwise each has every other tile.  Results are stored with the rows of a tile next to each other, so that a warp's stores and the loads of
-// a slot's heads are whole sectors.
+// One CTA per SM with two units, which take turns on the tensor cores: warp 0 fetches pages by TMA (lane <-> page; one box for a page of rows of 128, whose
+// requests take half the time of two) into two-stage rings, warp 1 issues the MMAs, warps 4..7 and 8..11 gather the queries of a unit, take its softmax
+// (thread <-> row) and keep O in tensor memory.  Where a group has more than 128 rows the units share the keys, otherwise each has every other tile.  Results are
+// stored with the rows of a tile next to each other, so that a warp's stores and the loads of a slot's heads are whole sectors.
+//
+// A step of both units, 2 x 128 x 128 scores and their products, takes 2.25 us at the 1.5 GHz that this load leaves; the tensor cores, the exponentials and the reads of
+// shared memory would take 1.4 each.  The rest is the way of one unit from its scores to its weights and back, which the other unit covers in part.  Measured on 128
+// sequences behind 32,768 tokens and not kept: scores of 64 keys at a time, two ahead (144 us for 127: MMAs 64 wide read their rows as often as wide ones), two
+// warpgroups per unit (156 for 136), a quarter or half of the exponentials as polynomials (125, 128 for 125), columns reread in short loops (130 for 125), pages asked for
+// into L2 two or three tiles ahead (135 for 126).
 constexpr int SX_THREADS = 384, SX_BN = 128, SX_PS = 16;
 // registers: 384 x 168 at launch, 128 x (72 + 216 + 216) afterwards, which is as many
 constexpr int SX_REGS_FEW = 72, SX_REGS_MANY = 216;
 constexpr int SX_CHUNK = 128 * 128, SX_TILE = 2 * SX_CHUNK;
-constexpr float SX_LAZY = 8.f;
+constexpr float SX_LAZY = 8.f;           // 137 -> 127 us there
 constexpr int SX_SMEM = 6 * SX_TILE + 1024 + 256;
 
 __global__ void __launch_bounds__(SX_THREADS, 1)
@@ -408,10 +419,10 @@ template <int DV> struct SoShape {
 __device__ __forceinline__ void so_leave(const SharedParams& p) {
   if (threadIdx.x == 0) {
     const unsigned all = gridDim.x * gridDim.y * gridDim.z;
-    if (atomicAdd(reinterpret_cast<unsigned*>(p.plan + SP_SEEN), 1u) == all - 1u) {
+    if (atomicAdd(reinterpret_cast<unsigned*>(p.plan + SP_LEFT), 1u) == all - 1u) {
       pdl_wait();                                // no piece is still to be counted, not even one that was given up
       p.plan[SP_DONE] = 0;
-      p.plan[SP_SEEN] = 0;
+      p.plan[SP_LEFT] = 0;
     }
   }
   pdl_wait();
@@ -457,7 +468,7 @@ __global__ void __launch_bounds__(SO_THREADS, NH == 1 ? 3 : 2) attn_shared_own_k
   w.begin(dk, dv, p.scale);
   // the ids of this warp's next 32 pages are in its lanes
   int ids = 0, ids_from = -32;
-  w.template walk<false>(mine, [&](int i) {
+  w.walk(mine, [&](int i) {
     if (i >= ids_from + 32) {
       ids_from = i;
       ids = i + lane < mine ? pt[place(ta + warp + (i + lane) * SO_WARPS)] : -1;
@@ -578,8 +589,8 @@ static int launch_shared_own(const SharedParams& p, cudaStream_t stream) {
 
 using namespace b200;
 
-extern "C" int b200_attn_decode_shared_takes(const b200_paged_cache* c, int hq, long long ldq, long long ldo) {
-  return c && !c->f32 && c->page_size == SX_PS && c->dk > 0 && c->dv > 0 && c->dk <= 128 && c->dv <= 128 && c->dk % 8 == 0 && c->dv % 8 == 0 && c->kv_heads > 0 &&
+static bool shared_takes(const b200_paged_cache* c, int hq, long long ldq, long long ldo) {
+  return !c->f32 && c->page_size == SX_PS && c->dk > 0 && c->dv > 0 && c->dk <= 128 && c->dv <= 128 && c->dk % 8 == 0 && c->dv % 8 == 0 && c->kv_heads > 0 &&
          hq % c->kv_heads == 0 && ldq % 8 == 0 && ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(c->data) & 15) == 0;
 }
 
@@ -588,7 +599,7 @@ extern "C" int b200_attn_decode_shared(const void* q, long long ldq, void* out, 
                                        int splits, int num_sms, int* status, cudaStream_t stream) {
   if (B <= 0) return 0;
   if (!q || !out || !seq_lens || !c || !c->data || !c->page_table || !s || !plan || !part) return -1;
-  if (!b200_attn_decode_shared_takes(c, hq, ldq, ldo) || hq <= 0 || c->num_pages <= 0) return -2;
+  if (!shared_takes(c, hq, ldq, ldo) || hq <= 0 || c->num_pages <= 0) return -2;
   if (B > c->num_seqs || B > 65535 || splits < 1 || splits > 8 || max_pieces < 0 || part_rows <= 0 || num_sms <= 0) return -3;
   if ((reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(out) & 7) || (reinterpret_cast<uintptr_t>(plan) & 15) ||
       (reinterpret_cast<uintptr_t>(part) & 15)) return -4;

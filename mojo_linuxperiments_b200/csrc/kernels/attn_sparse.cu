@@ -7,7 +7,10 @@
 // Two launches.  The first scores all pages of all rows, spread over the whole chip; bound by the bytes of the bounds, 2 dk per page.  The second has a
 // cluster of CTAs per row and group of heads: each selects (page_select.cuh), reads its share of the pages taken, and the sums are joined
 // through distributed shared memory, every CTA joining a slice of the dimensions.  (One launch of clusters that scored, selected and read took 32 us where these
-// two take 18, 131,071 keys and 8 KV heads: eight clusters keep 64 of 148 SMs busy with the scores, and clusters of 16 do not all run at once.)
+// two take 20, 131,071 keys and 8 KV heads: eight clusters keep 64 of 148 SMs busy with the scores, and clusters of 16 do not all run at once.)
+//
+// One row behind 131,071 keys, 128 of 8,192 pages taken, 8 KV heads of 128: 7.5 us for the scores (33.5 MB of bounds, 4.5 TB/s), 1.7 between the launches, 5 for the
+// selection, 4 for 8.4 MB of pages, 2 for the join.  16 rows behind 8,000 to 16,001 keys, 64 pages each, 4 KV heads: 22 us for 59 MB.
 #include "ptx.cuh"
 #include "api.h"
 #include "launch.cuh"
@@ -445,7 +448,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) attn_sparse_kernel(const __grid
   // the places and pages of this warp's next 32 entries are in its lanes
   int ids = 0, places = 0, ids_from = -32;
   const int mine = share > warp ? (share - warp + PS_WARPS - 1) / PS_WARPS : 0;
-  w.template walk<false>(mine, [&](int i) {
+  w.walk(mine, [&](int i) {
     if (i >= ids_from + 32) {
       ids_from = i;
       places = i + lane < mine ? list[warp + (i + lane) * PS_WARPS] : 0;

@@ -6,8 +6,10 @@
 // its share of two MMA steps (the queries are read in the same order).  Of the values a lane takes eight neighbouring dimensions of four keys and pairs
 // them up key by key; P^T is P through two 8 x 8 transpositions in registers.
 //
-// A page's keys are requested anew as soon as its scores are issued and its values after the last MMA; up to eight heads leave registers for two
-// pages, so that one is on its way while the other is used: 16 KiB per warp.  45 KiB per SM in flight are the full rate of the memory.
+// The next page's keys are requested into the same registers as soon as the scores are issued, its values after the last MMA: 8 KiB on the way per warp of heads
+// of 128, 96 KiB per SM with twelve warps, where 45 KiB are the full rate of the memory.  (Two pages in registers, one on its way while the other is used: no
+// faster, with half the warps.)  128 sequences with 500 own keys each, 8 heads of 128, take 54 us for 267 MB behind their prefix: 4.9 TB/s, with the waits for
+// places and the joins in it.
 #pragma once
 #include "ptx.cuh"
 
@@ -183,26 +185,15 @@ struct DecodeWarp {
     if (more) load_v(p, at);
   }
   // pages 0 .. n - 1; page(i) is asked for in this order.  start() runs once the first requests are out.
-  // DEEP: two pages at a time
-  template <bool DEEP, typename Page, typename Start>
+  template <typename Page, typename Start>
   __device__ __forceinline__ void walk(int n, Page&& page, Start&& start) {
     if (n <= 0) return;
     Held x;
     DwPage at = page(0);
     load_k(x, at);
     load_v(x, at);
-    if constexpr (DEEP) {
-      Held y;
-      if (n > 1) { at = page(1); load_k(y, at); load_v(y, at); }
-      start();
-      for (int i = 0; i < n; i += 2) {
-        step(x, i + 2 < n, [&] { return page(i + 2); });
-        if (i + 1 < n) step(y, i + 3 < n, [&] { return page(i + 3); });
-      }
-    } else {
-      start();
-      for (int i = 0; i < n; ++i) step(x, i + 1 < n, [&] { return page(i + 1); });
-    }
+    start();
+    for (int i = 0; i < n; ++i) step(x, i + 1 < n, [&] { return page(i + 1); });
   }
   // O and (m, l) of the first G heads to shared memory, rows `pitch` floats apart: [16][pitch], then m [16], l [16]
   __device__ __forceinline__ void put(float* to, int pitch, int G) {
@@ -262,7 +253,7 @@ __device__ __forceinline__ void dw_join(const float* parts, int size, int pitch,
   }
 }
 
-// four numbers of shared memory of CTA r of the cluster (addr: this CTA's address of the same place)
+// four numbers of shared memory of CTA r of the cluster, if there is one (addr: this CTA's address of the same place)
 __device__ __forceinline__ float4 dw_ld_cluster4(uint32_t addr, int r, bool cluster) {
   const uint32_t a = cluster ? mapa_shared(addr, r) : addr;
   float4 v;
