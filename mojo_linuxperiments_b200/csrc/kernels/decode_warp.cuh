@@ -7,8 +7,8 @@
 // them up key by key; P^T is P through two 8 x 8 transpositions in registers.
 //
 // The next page's keys are requested into the same registers as soon as the scores are issued, its values after the last MMA: 8 KiB on the way per warp of heads
-// of 128, 96 KiB per SM with twelve warps, where 45 KiB are the full rate of the memory.  (Two pages in registers, one on its way while the other is used: no
-// faster, with half the warps.)  128 sequences with 500 own keys each, 8 heads of 128, take 54 us for 267 MB behind their prefix: 4.9 TB/s, with the waits for
+// of 128, 96 KiB per SM with twelve warps, where 45 KiB are the full rate of the memory.  (Two pages in registers, one on its way while the other is used, or two in a
+// ring in shared memory, brought by bulk copies: no faster.)  128 sequences with 500 own keys each, 8 heads of 128, take 54 us for 267 MB behind their prefix: 4.9 TB/s, with the waits for
 // places and the joins in it.
 #pragma once
 #include "ptx.cuh"

@@ -2,8 +2,8 @@
 //
 // copy_pages: y[dst_i] = y[src_i] for every array y of records.  The page numbers come from the host, which has handed the pages out,
 // and travel in the kernel's parameters: no copy to the device in front of the launch, no look-up behind a load.  Bound by the bytes, read once and
-// written once; a CTA takes 16 KiB of one record, four loads of 16 bytes per thread in flight.  1,500 pages in each of 16 layers, 3.1 GB, take 482 us, 6.5 TB/s, the rate of a plain
-// copy; one page in each of 32 layers 1.6 us.
+// written once; a CTA takes 16 KiB of one record, four loads of 16 bytes per thread in flight.  1,500 pages in each of 16 layers, 3.1 GB, take 482 us, 6.5 TB/s,
+// the rate of a plain copy; one page in each of 32 layers 1.6 us.
 //
 // page_bounds: lo[d] = min_t k[t][d], hi[d] = max_t k[t][d] over the tokens of a page that a sequence has, per KV head.  Both are values of the
 // keys' own type, so nothing is rounded.  Bound by the bytes of the keys.  A CTA takes eight pages, whose numbers it looks up at once, and a warp one head of one of
