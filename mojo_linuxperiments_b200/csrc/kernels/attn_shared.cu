@@ -415,17 +415,16 @@ template <int DV> struct SoShape {
   static constexpr int SMEM = ((SO_WARPS + 1) * SIZE + 16 * (8 + SO_PARTS)) * 4;
 };
 
-// The last CTA to leave clears the counters for the next call, which starts behind this kernel; every CTA leaves behind the first kernel.
-__device__ __forceinline__ void so_leave(const SharedParams& p) {
-  if (threadIdx.x == 0) {
-    const unsigned all = gridDim.x * gridDim.y * gridDim.z;
-    if (atomicAdd(reinterpret_cast<unsigned*>(p.plan + SP_LEFT), 1u) == all - 1u) {
-      pdl_wait();                                // no piece is still to be counted, not even one that was given up
-      p.plan[SP_DONE] = 0;
-      p.plan[SP_LEFT] = 0;
-    }
-  }
-  pdl_wait();
+// The last CTA that has looked at the counters clears them for the next call, which starts behind this kernel, and this kernel ends behind the first one.  Which
+// that is, thread 0 asks early: the answer comes meanwhile.
+__device__ __forceinline__ unsigned so_looked(const SharedParams& p) {
+  return threadIdx.x == 0 ? atomicAdd(reinterpret_cast<unsigned*>(p.plan + SP_LEFT), 1u) : 0u;
+}
+__device__ __forceinline__ void so_leave(const SharedParams& p, unsigned before) {
+  if (threadIdx.x != 0 || before != gridDim.x * gridDim.y * gridDim.z - 1u) return;
+  pdl_wait();                                    // no piece is still to be counted, not even one that was given up
+  p.plan[SP_DONE] = 0;
+  p.plan[SP_LEFT] = 0;
 }
 
 template <int DK, int DV, int NH, bool FULL>
@@ -448,7 +447,7 @@ __global__ void __launch_bounds__(SO_THREADS, NH == 1 ? 3 : 2) attn_shared_own_k
     if (bad && tid == 0 && p.status) atomicCAS(p.status, 0, static_cast<int>(ST_BAD_ARGUMENT) | (26 << 8));
     if (rank == 0)
       for (int i = tid; i < G * dv; i += SO_THREADS) p.out[static_cast<size_t>(b) * p.ldo + static_cast<size_t>(h0) * dv + i] = __float2bfloat16(0.f);
-    so_leave(p);
+    so_leave(p, so_looked(p));
     return;
   }
   const int low = p.chunk > 0 ? (len - 1) - (len - 1) % p.chunk : 0;
@@ -493,6 +492,7 @@ __global__ void __launch_bounds__(SO_THREADS, NH == 1 ? 3 : 2) attn_shared_own_k
     const uint32_t pieces = static_cast<uint32_t>(min(p.plan[0], p.max_pieces)) * p.c.kv_heads;
     wait_count_gpu(reinterpret_cast<const uint32_t*>(p.plan + SP_DONE), pieces, p.status, static_cast<int>(ST_TIMEOUT_PEER_FLAG) | (26 << 8), p.limit_ns);
   }
+  const unsigned before = so_looked(p);
   if (S > 1) cluster_sync_all(); else __syncthreads();
   if (tid == 0) B200_TRACE(TK_ATTN_OWN, TP_DEPS);
   const uint32_t own_addr = smem_u32(own);
@@ -565,7 +565,7 @@ __global__ void __launch_bounds__(SO_THREADS, NH == 1 ? 3 : 2) attn_shared_own_k
         make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&c));
   }
   if (S > 1) cluster_sync_all(); else __syncthreads();       // no CTA leaves while a peer may still read its part
-  so_leave(p);
+  so_leave(p, before);
   if (tid == 0) B200_TRACE(TK_ATTN_OWN, TP_EXIT);
   B200_TRACE_FLUSH(TK_ATTN_OWN);
 }
