@@ -27,8 +27,9 @@ def cut_prefixes(groups, num_seqs: int, per_head: int, kv_heads: int, ctas: int,
 
     A piece is up to 256 rows of a group and a run of tiles of 128 keys, for every KV head.  The two units of a CTA have 128 rows each, or, in a group of no
     more than 128, the same rows and every other tile.  Runs are as long as ends soonest: pieces of L steps take L + 4 (their start and end), ``ctas`` of
-    them at a time, and ``others``, the CTAs of the slots' own keys, three of which fit where there is no piece, another 4 if some of them have to wait.  With ``chunk`` only the keys from the last multiple of it are seen, and
-    shared from the next page on.  A slot's numbers: first row of its partial results, rows between the parts, parts (none: it shares nothing), tokens."""
+    them at a time, and ``others``, the CTAs of the slots' own keys, three of which fit where there is no piece, another 4 if some of
+    them have to wait.  Where that is the same, fewer pieces if they wait and shorter runs if not (25 slots behind 1,657 tokens: 13.6 us in six, 14.9 in four).  With
+    ``chunk`` only the keys from the last multiple of it are seen, and shared from the next page on.  A slot's numbers: first row of its partial results, rows between the parts, parts (none: it shares nothing), tokens."""
     info, pieces, order, base = [0] * (4 * num_seqs), [], [], 0
     begins = [-(-((tokens - 1) // chunk * chunk) // PAGE) * PAGE if chunk else 0 for _, tokens in groups]
     groups, begins = [g for g, a in zip(groups, begins) if a < g[1]], [a for (_, tokens), a in zip(groups, begins) if a < tokens]
@@ -54,7 +55,8 @@ def cut_prefixes(groups, num_seqs: int, per_head: int, kv_heads: int, ctas: int,
             count += -(-rows // (2 * ROW_TILE)) * runs
             room += rows * parts
         fits, count = count <= most[0] and room <= most[1], kv_heads * count
-        return not fits, -(-count // ctas) * (longest + 4) + (4 if others > 3 * max(0, ctas - count) else 0)
+        wait = others > 3 * max(0, ctas - count)
+        return not fits, -(-count // ctas) * (longest + 4) + 4 * wait, wait, count if wait else steps
 
     tried, at = [], max(tiles for _, tiles in sizes)       # one run each always fits
     while at >= 1:
@@ -77,8 +79,9 @@ def cut_prefixes(groups, num_seqs: int, per_head: int, kv_heads: int, ctas: int,
 class _Cut:
     """A plan as the kernels read it, for one number of heads, and room for partial results."""
 
-    def __init__(self, num_seqs: int, per_head: int, kv_heads: int, dv: int, chunk: int, device: torch.device):
-        self.per_head, self.kv_heads, self.chunk, self.sms = per_head, kv_heads, chunk, _lib.num_sms(device.index)
+    def __init__(self, num_seqs: int, per_head: int, kv_heads: int, dv: int, chunk: int, room: int, device: torch.device):
+        self.per_head, self.kv_heads, self.chunk, self.room, self.sms = per_head, kv_heads, chunk, room, _lib.num_sms(device.index)
+        self.splits = 1                          # CTAs that share a slot's own keys
         self.max_pieces, self.rows = room_for(num_seqs, per_head, kv_heads, self.sms)
         self.pieces_at = (_INFO + 4 * num_seqs + 7) // 8 * 8
         self.slots_at = self.pieces_at + _PIECE * self.max_pieces
@@ -89,9 +92,11 @@ class _Cut:
         self.ring = [(buf, torch.cuda.Event()) for buf in torch.zeros(4, n, dtype=torch.int32, pin_memory=True)]
         self.turn = 0
 
-    def send(self, groups, num_seqs: int) -> None:
-        others = num_seqs * self.kv_heads * -(-self.per_head // 16)
-        info, pieces, order, rows = cut_prefixes(groups, num_seqs, self.per_head, self.kv_heads, self.sms, others, self.chunk)
+    def send(self, groups, num_seqs: int, alone: int) -> None:
+        heads, keys = self.kv_heads * -(-self.per_head // 16), self.room - alone
+        # at least 128 keys each: 16 slots with up to 150 take 8.9 us, 9.8 in two; 28 with up to 698 take 10.5 in four, 11.3 in eight
+        self.splits = pick_decode_splits_paged(num_seqs, heads, (min(keys, self.chunk) if self.chunk else keys) // 2, self.sms)
+        info, pieces, order, rows = cut_prefixes(groups, num_seqs, self.per_head, self.kv_heads, self.sms, num_seqs * heads * self.splits, self.chunk)
         assert len(pieces) <= self.max_pieces and rows <= self.rows
         buf, done = self.ring[self.turn]
         self.turn = (self.turn + 1) % len(self.ring)
@@ -136,19 +141,19 @@ class SharedPrefixes:
         covered = sum(len(slots) for slots, _ in self.groups)
         self.alone = min((t for _, t in self.groups), default=0) if covered == self.num_seqs else 0
         for cut in self._cuts.values():
-            cut.send(self.groups, self.num_seqs)
+            cut.send(self.groups, self.num_seqs, self.alone)
 
-    def cut_for(self, hq: int, cache: PagedKVCache, chunk: int = 0) -> _Cut:
+    def cut_for(self, hq: int, cache: PagedKVCache, room: int, chunk: int = 0) -> _Cut:
         device = cache.data.device
-        key = (hq, cache.kv_heads, cache.dv, chunk, device.index)
+        key = (hq, cache.kv_heads, cache.dv, chunk, room, device.index)
         cut = self._cuts.get(key)
         if cut is None:
             if device != self.device and (device.type != self.device.type or self.device.index is not None):
                 raise ValueError(f"a plan for {self.device} and a cache on {device}")
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("the first call with a plan sends it to the device: make one before the capture")
-            cut = self._cuts[key] = _Cut(self.num_seqs, hq // cache.kv_heads, cache.kv_heads, cache.dv, chunk, device)
-            cut.send(self.groups, self.num_seqs)
+            cut = self._cuts[key] = _Cut(self.num_seqs, hq // cache.kv_heads, cache.kv_heads, cache.dv, chunk, room, device)
+            cut.send(self.groups, self.num_seqs, self.alone)
         return cut
 
 
@@ -176,13 +181,10 @@ def attn_decode_shared(q: torch.Tensor, hq: int, seq_lens: torch.Tensor, cache: 
         rc = _lib.on_device(device, L.b200_attn_paged, q_at, ldq, out_at, ldo, hq, B, None, None, seq_lens.data_ptr(), ctypes.byref(desc), ctypes.byref(spec), status)
         _lib.check(rc, "attn_paged")
         return out
-    cut = shared.cut_for(hq, cache, spec.chunk)
-    if splits is None:
-        keys = min(room - shared.alone, spec.chunk) if spec.chunk > 0 else room - shared.alone
-        splits = pick_decode_splits_paged(B, kv_heads * ((hq // kv_heads + 15) // 16), keys, cut.sms)
+    cut = shared.cut_for(hq, cache, room, spec.chunk)
     rc = _lib.on_device(
         device, L.b200_attn_decode_shared, q_at, ldq, out_at, ldo, hq, B, seq_lens.data_ptr(), ctypes.byref(desc),
-        ctypes.byref(spec), cut.plan.data_ptr(), cut.pieces_at, cut.slots_at, cut.max_pieces, cut.part.data_ptr(), cut.rows, splits, cut.sms,
+        ctypes.byref(spec), cut.plan.data_ptr(), cut.pieces_at, cut.slots_at, cut.max_pieces, cut.part.data_ptr(), cut.rows, splits or cut.splits, cut.sms,
         status)
     _lib.check(rc, "attn_decode_shared")
     _lib.LAUNCHES[0] += 1                        # two kernels
