@@ -33,19 +33,22 @@ def copy_pages(caches, src, dst) -> None:
     if lo < 0:
         raise IndexError(f"page {lo}")
     at, sizes = array("Q"), array("q")
+    shape = dtype = None                          # of the array before: a model's layers are alike, and there are many
     for a in arrays:
-        if a.get_device() != index or index < 0 or not a.is_contiguous() or a.dim() < 2:
+        if a.shape != shape or a.dtype != dtype:
+            shape, dtype = a.shape, a.dtype
+            records = shape[0] if len(shape) > 1 else 0
+            if hi >= records:
+                raise IndexError(f"pages {lo} to {hi} of {records}")
+            size = a.nbytes // records
+        start = a.data_ptr()
+        if a.get_device() != index or index < 0 or not a.is_contiguous():
             raise ValueError("records lie in contiguous tensors on one GPU")
-        records = a.shape[0]
-        if hi >= records:
-            raise IndexError(f"pages {lo} to {hi} of {records}")
-        start, size = a.data_ptr(), a.nbytes // records
-        if size == 0:
-            continue
         if size % 16 or start % 16:
             raise ValueError("records are whole pieces of 16 bytes")
-        at.append(start)
-        sizes.append(size)
+        if size:
+            at.append(start)
+            sizes.append(size)
     rc = _lib.on_device(arrays[0].device, _lib.lib().b200_copy_pages, at.buffer_info()[0], sizes.buffer_info()[0], len(at), src.buffer_info()[0],
                         dst.buffer_info()[0], n)
     _lib.check(rc, "copy_pages")
