@@ -6,9 +6,9 @@
 // the rate of a plain copy; one page in each of 32 layers 1.6 us.
 //
 // page_bounds: lo[d] = min_t k[t][d], hi[d] = max_t k[t][d] over the tokens of a page that a sequence has, per KV head.  Both are values of the
-// keys' own type, so nothing is rounded.  Bound by the bytes of the keys.  A CTA takes eight pages, whose numbers it looks up at once, and a warp one head of one of
+// keys' own type, so nothing is rounded.  Bound by the bytes of the keys.  A CTA takes some pages, whose numbers it looks up at once, and a warp one head of one of
 // them after the other; lanes lie along the row of 16-byte pieces and, where a row has fewer than 32 of them, along the tokens.
-// 382 MB of prompts take 68 us (5.6 TB/s), the pages of a step's tokens 2.6 us.
+// 382 MB of prompts take 62 us (6.1 TB/s), the pages of a step's tokens 2.6 us.
 #include "ptx.cuh"
 #include "api.h"
 #include "launch.cuh"
@@ -60,12 +60,13 @@ static int copy_pages_some(void* const* arrays, const long long* records, int n_
 }
 
 // ---- bounds ------------------------------------------------------------------------------------------------------------------
-constexpr int PB_WARPS = 8, PB_PAGES = 8;
+constexpr int PB_WARPS = 8, PB_MOST = 32, PB_UNITS = 6, PB_CTAS = 592;
 
 struct PageBoundsParams {
   b200_paged_cache c;
   const int* starts; const int* ends; const int* seq_ids;
   void* out;                             // [pages][kv_heads][2][dk]
+  int each;                              // pages of a CTA
   int* status;
 };
 
@@ -92,16 +93,16 @@ __global__ void __launch_bounds__(32 * PB_WARPS) page_bounds_kernel(const __grid
   constexpr int N = VEC ? 16 / static_cast<int>(sizeof(T)) : 1, WORDS = VEC ? 4 : 1, BATCH = 8;
   pdl_launch_dependents();
   pdl_wait();
-  __shared__ int ids[PB_PAGES];
+  __shared__ int ids[PB_MOST];
   const int lane = threadIdx.x & 31, b = blockIdx.y, ps = p.c.page_size, dk = p.c.dk;
   const int start = p.starts[b], end = p.ends[b], seq = p.seq_ids ? p.seq_ids[b] : b;
   if (end <= start) return;
   const int last = (end - 1) / ps;
-  if (start < 0 || seq < 0 || seq >= p.c.num_seqs || last >= p.c.max_pages || last - start / ps >= static_cast<int>(gridDim.x) * PB_PAGES) {
+  if (start < 0 || seq < 0 || seq >= p.c.num_seqs || last >= p.c.max_pages || last - start / ps >= static_cast<int>(gridDim.x) * p.each) {
     if (threadIdx.x == 0 && blockIdx.x == 0 && p.status) atomicCAS(p.status, 0, static_cast<int>(ST_BAD_ARGUMENT) | (24 << 8));
     return;
   }
-  const int place0 = start / ps + blockIdx.x * PB_PAGES, pages = min(PB_PAGES, last + 1 - place0);
+  const int place0 = start / ps + blockIdx.x * p.each, pages = min(p.each, last + 1 - place0);
   if (pages <= 0) return;
   if (static_cast<int>(threadIdx.x) < pages) {
     const int page = p.c.page_table[static_cast<size_t>(seq) * p.c.max_pages + place0 + threadIdx.x];
@@ -200,10 +201,13 @@ extern "C" int b200_page_bounds(const b200_paged_cache* c, const int* starts, co
   if (portions <= 0 || max_tokens <= 0) return 0;
   if (!c || !c->data || !c->page_table || !starts || !ends || !out) return -1;
   if (c->kv_heads <= 0 || c->dk <= 0 || c->dv < 0 || c->page_size <= 0 || c->num_pages <= 0 || portions > 65535) return -2;
-  PageBoundsParams p{*c, starts, ends, seq_ids, out, status};
   const long long pages = (static_cast<long long>(max_tokens) + 2 * c->page_size - 2) / c->page_size;
   const long long most = pages < c->max_pages ? pages : c->max_pages;
-  const dim3 grid(static_cast<unsigned>((most + PB_PAGES - 1) / PB_PAGES), portions);
+  // Pages of a CTA: so many that a warp has six heads, one after the other, and no more than leave four CTAs per SM (8 heads of 128, 240,000 tokens: 62 us with 6
+  // pages, 68 with 8; 8 heads of 64, 32,000 tokens: 8.5 us with 3 pages, 16 with 8; one head, 144,000 tokens: 10.6 with 3, 7.1 with 8)
+  const long long heads = PB_UNITS * PB_WARPS / c->kv_heads, share = most * portions / PB_CTAS, each = heads < share ? heads : share;
+  PageBoundsParams p{*c, starts, ends, seq_ids, out, static_cast<int>(each < 1 ? 1 : each > PB_MOST ? PB_MOST : each), status};
+  const dim3 grid(static_cast<unsigned>((most + p.each - 1) / p.each), portions);
   const size_t size = c->f32 ? 4 : 2;
   const bool vec = c->dk * size % 16 == 0 && static_cast<size_t>(c->kv_heads) * c->page_size * (c->dk + c->dv) * size % 16 == 0 &&
                    ((reinterpret_cast<uintptr_t>(c->data) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
