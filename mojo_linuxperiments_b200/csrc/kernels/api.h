@@ -344,6 +344,7 @@ int b200_attn_paged(const void* q, long long ldq, void* out, long long ldo, int 
 // Attention of single rows over the pages that always count and those whose keys' bounds promise most (attn_sparse.cu): `top` pages per KV head, the
 // `first` pages and the `last` up to the row's own among them.  bounds [pages][kv_heads][2][dk] as b200_page_bounds leaves them.  splits: CTAs (a
 // cluster) per row and KV head.  scores [M][kv_heads][max_pages]: room.  chosen [M][kv_heads][top] or NULL: the pages read, ascending, -1 behind them.
+int b200_sparse_clusters(int size);          // clusters of that size that run at once, one CTA per SM; 0: unknown
 int b200_attn_paged_sparse(const void* q, long long ldq, void* out, long long ldo, int hq, int M, const int* positions, const int* seq_ids,
                            const int* seq_lens, const b200_paged_cache* cache, const void* bounds, const b200_attn_spec* spec, int top, int first,
                            int last, int splits, unsigned* scores, int* chosen, int* status, cudaStream_t stream);

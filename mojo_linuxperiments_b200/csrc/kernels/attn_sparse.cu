@@ -579,6 +579,20 @@ static int launch_sparse_heads(const SparseParams& p, cudaStream_t stream) {
 
 using namespace b200;
 
+// Clusters of so many CTAs, one per SM, that run at once on the current device (which of a GPU's SMs make up a cluster depends on how many of them each part of it has);
+// 0 where that cannot be told
+extern "C" int b200_sparse_clusters(int size) {
+  if (size < 1 || size > 8) return 0;
+  if (allow_smem<attn_sparse_kernel<128, 128, 1, true>>(static_cast<int>(SPARSE_MAX_SMEM)) != cudaSuccess) return 0;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = size; attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(size); cfg.blockDim = dim3(PS_THREADS); cfg.dynamicSmemBytes = SPARSE_MAX_SMEM; cfg.attrs = &attr; cfg.numAttrs = 1;
+  int n = 0;
+  return cudaOccupancyMaxActiveClusters(&n, attn_sparse_kernel<128, 128, 1, true>, &cfg) == cudaSuccess ? n : (static_cast<void>(cudaGetLastError()), 0);
+}
+
 extern "C" int b200_attn_paged_sparse(const void* q, long long ldq, void* out, long long ldo, int hq, int M, const int* positions, const int* seq_ids,
                                       const int* seq_lens, const b200_paged_cache* c, const void* bounds, const b200_attn_spec* s, int top, int first,
                                       int last, int splits, unsigned* scores, int* chosen, int* status, cudaStream_t stream) {

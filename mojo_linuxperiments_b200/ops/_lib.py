@@ -129,6 +129,7 @@ class _Sig:
     b200_embed_norm = (I, [P, P, LL, I, I, F, I, I, P, P, P, P])
     b200_attn_paged = (I, [P, LL, P, LL, I, I, P, P, P, P, P, P, P])
     b200_attn_paged_sparse = (I, [P, LL, P, LL, I, I, P, P, P, P, P, P, I, I, I, I, P, P, P, P])
+    b200_sparse_clusters = (I, [I])
     b200_attn_decode_shared = (I, [P, LL, P, LL, I, I, P, P, P, P, I, I, I, P, I, I, I, P, P])
     b200_page_bounds = (I, [P, P, P, P, I, I, P, P, P])
     b200_copy_pages = (I, [P, P, I, P, P, I, P])

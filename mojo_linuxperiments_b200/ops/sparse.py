@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 
 import torch
 
@@ -16,11 +17,19 @@ MAX_QUERIES = 50 << 10         # numbers of a group's queries, heads padded to 1
 LIST_PER_CTA = 16384           # pages that a CTA may have to read
 
 
-def pick_sparse_splits(pairs: int, pages: int, num_sms: int = 148, least: int = 16) -> int:
-    """CTAs (one cluster of up to eight) per row and group of heads, which share ``pages`` pages: as many as still make one wave of one per SM, with
-    ``least`` pages (16: two for a warp) each, and so many that their lists have room."""
+@lru_cache(maxsize=None)
+def clusters_at_once(device_index: int) -> dict[int, int]:
+    """Clusters of 2, 4 and 8 CTAs, one per SM, that run at once."""
+    with torch.cuda.device(device_index):
+        return {s: _lib.lib().b200_sparse_clusters(s) or _lib.num_sms(device_index) // (2 * s) for s in (2, 4, 8)}
+
+
+def pick_sparse_splits(pairs: int, pages: int, at_once: dict[int, int]) -> int:
+    """CTAs (one cluster of up to eight) per row and group of heads, which share ``pages`` pages: as many as still run at once (16 clusters of eight, of which 15 do,
+    take 21.4 us where clusters of four take 14.6), with four pages each (one row, 64 pages, 8 KV heads: 12.2 us in eight, 13.2 in four; 16 pages, one KV head:
+    11.1 in four, 12.5 in one), and so many that their lists have room."""
     s = 1
-    while s < 8 and ((pairs * s * 2 <= num_sms and pages // (2 * s) >= least) or pages > s * LIST_PER_CTA):
+    while s < 8 and ((pairs <= at_once[2 * s] and pages // (2 * s) >= 4) or pages > s * LIST_PER_CTA):
         s *= 2
     return s
 
@@ -62,7 +71,7 @@ def attn_paged_sparse(q: torch.Tensor, hq: int, positions: torch.Tensor, seq_ids
         assert chosen.dtype == torch.int32 and tuple(chosen.shape) == (M, kv_heads, top) and chosen.is_contiguous()
     if splits is None:
         seen = min(most, spec.chunk // cache.page_size + 2) if spec.chunk > 0 else most
-        splits = pick_sparse_splits(M * kv_heads * ((group + 15) // 16), min(top, seen), _lib.num_sms(device.index), 16 if dtype == torch.bfloat16 else 4)
+        splits = pick_sparse_splits(M * kv_heads * ((group + 15) // 16), min(top, seen), clusters_at_once(device.index))
     scores = torch.empty(M * kv_heads * most, dtype=torch.int32, device=device)
     rc = _lib.on_device(
         device, _lib.lib().b200_attn_paged_sparse, q.data_ptr(), ldq, out.data_ptr(), ldo, hq, M, positions.data_ptr(), _lib.ptr(seq_ids),

@@ -56,9 +56,9 @@ def test_groups_that_make_no_sense_are_refused(groups):
         SH.SharedPrefixes(4, "cpu").set(groups)
 
 
-@pytest.mark.parametrize("pairs,pages,want", [(8, 128, 8), (64, 64, 2), (512, 256, 1), (20, 100, 4), (2, 31, 1), (1, 32, 2), (4000, 65536, 4), (300, 16384, 1)])
+@pytest.mark.parametrize("pairs,pages,want", [(8, 128, 8), (15, 128, 8), (16, 128, 4), (33, 64, 4), (34, 64, 2), (74, 64, 2), (75, 64, 1), (2, 31, 4), (1, 32, 8), (3, 7, 1), (4000, 65536, 4), (300, 16384, 1)])
 def test_clusters_for_selections(pairs, pages, want):
-    assert SP.pick_sparse_splits(pairs, pages) == want
+    assert SP.pick_sparse_splits(pairs, pages, {2: 74, 4: 33, 8: 15}) == want
 
 
 @pytest.mark.parametrize("per_head,kv_heads,groups", [
