@@ -6,7 +6,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .attention import PAGE, PagedKVCache, pick_decode_splits_paged
+from .attention import PAGE, PagedKVCache
 from .workspace import default_workspace
 
 KEY_TILE = 128                 # keys of a step of the kernel
@@ -76,6 +76,16 @@ def cut_prefixes(groups, num_seqs: int, per_head: int, kv_heads: int, ctas: int,
     return info, pieces, order, base
 
 
+def pick_own_splits(pairs: int, keys: int, per_head: int, num_sms: int) -> int:
+    """CTAs (one cluster) that share a slot's own keys, up to ``keys``, for a group of heads: as many as find a place at once with some left for the prefix, and at
+    least 128 keys each.  Up to eight heads leave places for three CTAs per SM (80 pairs with up to 2,000 keys: 22.5 us in four, 29.2 in two; 60: 20.2 in four, 25.5
+    in eight), more for two (34: 19.2 in four, 26.3 in eight).  16 slots with up to 150 keys take 8.9 us, 9.8 in two; 28 with up to 698 take 10.5 in four, 11.3 in eight."""
+    s, most = 1, (4 * (3 if per_head <= 8 else 2) - 1) * num_sms // 4
+    while s < 8 and pairs * 2 * s <= most and keys // (2 * s) >= KEY_TILE:
+        s *= 2
+    return s
+
+
 class _Cut:
     """A plan as the kernels read it, for one number of heads, and room for partial results."""
 
@@ -94,8 +104,7 @@ class _Cut:
 
     def send(self, groups, num_seqs: int, alone: int) -> None:
         heads, keys = self.kv_heads * -(-self.per_head // 16), self.room - alone
-        # at least 128 keys each: 16 slots with up to 150 take 8.9 us, 9.8 in two; 28 with up to 698 take 10.5 in four, 11.3 in eight
-        self.splits = pick_decode_splits_paged(num_seqs, heads, (min(keys, self.chunk) if self.chunk else keys) // 2, self.sms)
+        self.splits = pick_own_splits(num_seqs * heads, min(keys, self.chunk) if self.chunk else keys, self.per_head, self.sms)
         info, pieces, order, rows = cut_prefixes(groups, num_seqs, self.per_head, self.kv_heads, self.sms, num_seqs * heads * self.splits, self.chunk)
         assert len(pieces) <= self.max_pieces and rows <= self.rows
         buf, done = self.ring[self.turn]

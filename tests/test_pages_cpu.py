@@ -61,6 +61,12 @@ def test_clusters_for_selections(pairs, pages, want):
     assert SP.pick_sparse_splits(pairs, pages, {2: 74, 4: 33, 8: 15}) == want
 
 
+@pytest.mark.parametrize("pairs,keys,per_head,want", [(1, 100, 4, 1), (16, 150, 4, 1), (28, 698, 8, 4), (80, 2000, 4, 4), (80, 2000, 16, 2), (74, 2000, 9, 2), (64, 2000, 16, 4), (34, 2000, 16, 4), (60, 2000, 4, 4),
+                                                      (50, 2000, 4, 8), (1024, 1000, 4, 1), (4, -100, 4, 1)])
+def test_clusters_for_own_keys(pairs, keys, per_head, want):
+    assert SH.pick_own_splits(pairs, keys, per_head, 148) == want
+
+
 @pytest.mark.parametrize("per_head,kv_heads,groups", [
     (4, 8, [(list(range(32)), 2048)]), (4, 8, [(list(range(128)), 32768)]), (20, 1, [([3, 1, 2], 16), ([0, 7], 160), ([5], 4096)]),
     (160, 1, [([1, 0, 2], 272)]), (1, 1, [(list(range(200)), 16)]), (7, 3, [([i, 199 - i], 16 * (1 + i)) for i in range(90)]), (4, 8, []),
