@@ -325,7 +325,8 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
             }
           }
           const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
-          // two at a time; rounded to bf16 for the MMA, the denominator adds what was rounded (which is off by as much to either side)
+          // two at a time; rounded to bf16 for the MMA, the denominator adds what the MMA sees, so that the rounding of a weight that outweighs all others
+          // has no part in the result
           const uint64_t scale2 = sx_pair(scale_log2, scale_log2), shift2 = sx_pair(-m_use, -m_use);
           uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
@@ -338,7 +339,7 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
               e0 = dw_exp2(e0);
               e1 = dw_exp2(e1);
               pk[i] = dw_pack(e0, e1);
-              sum[i & 1] = sx_add2(sum[i & 1], sx_pair(e0, e1));
+              sum[i & 1] = sx_add2(sum[i & 1], sx_pair(__uint_as_float(pk[i] << 16), __uint_as_float(pk[i] & 0xffff0000u)));
             }
             tmem_st_x16(t_s + c * 16, pk);
             if (c == 1) {                        // the product of the first half may begin

@@ -251,3 +251,19 @@ def test_queries_that_are_not_numbers_give_none(hq, hkv, dk, dv, sink):
     out = _run(S, q, lens, plan, 0.1, s, None)
     status_ok()
     assert torch.isnan(out[0, :dv]).all() and torch.isnan(out[1]).all() and torch.isfinite(out[0, dv:]).all() and torch.isfinite(out[2:]).all()
+
+
+@pytest.mark.parametrize("hq,hkv,dk,dv,n,tokens", [(32, 8, 128, 128, 24, 4096), (40, 2, 64, 64, 12, 2048), (6, 2, 104, 56, 30, 1024)])
+def test_weights_add_up_to_the_denominator(hq, hkv, dk, dv, n, tokens):
+    """All values are one, so every result is the sum of the weights over the denominator: exactly one, whatever the weights are rounded to.  Between
+    the two stand fp32 sums of some thousand terms and a reciprocal, 2^-10 at most, where the bf16 number below one is 2^-8 away and what lies within half of that rounds to one."""
+    groups = [(list(range(n)), tokens)]
+    lens = [tokens + 1 + 5 * i for i in range(n)]
+    S = Sequences(lens, hq, hkv, dk, dv, "bfloat16", groups=groups, seed=tokens, spread=3.0)
+    S.cache.values().fill_(1.0)
+    from mojo_linuxperiments_b200.ops import shared as SH
+    plan = SH.SharedPrefixes(n, DEV)
+    plan.set(groups)
+    out = _run(S, S.rows_of(n), lens, plan, dk ** -0.5, None, None)
+    status_ok()
+    assert torch.equal(out, torch.ones_like(out)), (float(out.min()), float(out.max()))
