@@ -267,3 +267,33 @@ def test_weights_add_up_to_the_denominator(hq, hkv, dk, dv, n, tokens):
     out = _run(S, S.rows_of(n), lens, plan, dk ** -0.5, None, None)
     status_ok()
     assert torch.equal(out, torch.ones_like(out)), (float(out.min()), float(out.max()))
+
+
+def test_no_further_from_exact_than_decoding_alone():
+    """A few keys decide each softmax (scores of a standard deviation of 3): the errors against 64 bits are those of the decode kernel that reads every
+    sequence's keys by itself, whose weights are rounded as well, relative to the largest so far.  Errors of 4,096 independent rows: their mean square is known to
+    sqrt(2 / 4096) = 2.2 %, its root to 1.1 %; 5 % are allowed.  (Weights relative to an older maximum: 12 % and more.)"""
+    from mojo_linuxperiments_b200.ops import attention as A
+    from mojo_linuxperiments_b200.ops import shared as SH
+    n, hq, hkv, d, tokens, own = 128, 32, 8, 128, 4096, 16
+    groups = [(list(range(n)), tokens)]
+    S = Sequences([tokens + own] * n, hq, hkv, d, d, "bfloat16", groups=groups, seed=4, spread=3.0)
+    q, per = S.rows_of(n), hq // hkv
+    plan = SH.SharedPrefixes(n, DEV)
+    plan.set(groups)
+    got = _run(S, q, S.lens, plan, d ** -0.5, None, None)
+    # the new token's key and value are in the cache already and are written there once more
+    last = torch.tensor([r[-1] for r in S.rows], device=DEV)
+    k, v = S.cache.keys()[last, :, own - 1].reshape(n, -1), S.cache.values()[last, :, own - 1].reshape(n, -1)
+    lens = torch.tensor(S.lens, dtype=torch.int32, device=DEV)
+    alone = torch.empty((n, hq * d), dtype=S.dtype, device=DEV)
+    A.attn_decode_paged(torch.cat([q, k, v], 1), hq, lens - 1, lens, None, None, S.cache, S.table, A.attn_spec(d ** -0.5), alone)
+    status_ok()
+    want = torch.empty((n, hkv, per, d), dtype=torch.float64, device=DEV)
+    for h in range(hkv):
+        for i in range(0, n, 16):
+            page = S.table[i:i + 16].long()
+            K, V = (x()[page][:, :, h].flatten(1, 2).double() for x in (S.cache.keys, S.cache.values))
+            want[i:i + 16, h] = torch.softmax(q[i:i + 16].view(-1, hkv, per, d)[:, h].double() @ K.transpose(1, 2) * d ** -0.5, -1) @ V
+    off = [float((x.view_as(want).double() - want).norm() / want.norm()) for x in (got, alone)]
+    assert off[0] <= 1.05 * off[1], off
