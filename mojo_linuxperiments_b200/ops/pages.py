@@ -66,6 +66,13 @@ def check_bounds(cache: PagedKVCache, bounds: torch.Tensor) -> None:
         raise ValueError(f"bounds {tuple(bounds.shape)} {bounds.dtype} of a cache of {cache.num_pages} pages, {cache.kv_heads} heads of {cache.dk}, {cache.data.dtype}")
 
 
+def on_one_gpu(*tensors: torch.Tensor | None) -> None:
+    """Kernels are given addresses: those of one GPU's memory."""
+    index = tensors[0].get_device()
+    if index < 0 or any(t is not None and t.get_device() != index for t in tensors):
+        raise ValueError("tensors on one GPU")
+
+
 def page_bounds(cache: PagedKVCache, page_table: torch.Tensor, starts: torch.Tensor, ends: torch.Tensor, seq_ids: torch.Tensor | None, max_tokens: int,
                 bounds: torch.Tensor) -> torch.Tensor:
     """Smallest and largest element of the keys of a page, per KV head and dimension, for all pages that hold tokens ``starts[i]`` to
@@ -73,6 +80,7 @@ def page_bounds(cache: PagedKVCache, page_table: torch.Tensor, starts: torch.Ten
     ``max_tokens``: the most that a portion has; one that has more pages than that may is left out, which the status word says.  A page is touched by one
     portion only.  A portion of no tokens, as of an empty slot, changes nothing.  Exact; NaN where a key is."""
     check_bounds(cache, bounds)
+    on_one_gpu(bounds, page_table, starts, ends, seq_ids)
     n = starts.numel()
     assert starts.dtype == ends.dtype == page_table.dtype == torch.int32 and ends.numel() == n and starts.is_contiguous() and ends.is_contiguous() and page_table.is_contiguous()
     if seq_ids is None:

@@ -7,6 +7,7 @@ import torch
 
 from . import _lib
 from .attention import PAGE, PagedKVCache
+from .pages import on_one_gpu
 from .workspace import default_workspace
 
 KEY_TILE = 128                 # keys of a step of the kernel
@@ -183,8 +184,7 @@ def attn_decode_shared(q: torch.Tensor, hq: int, seq_lens: torch.Tensor, cache: 
     room = pages * cache.page_size
     if B > seqs or B != shared.num_seqs or shared.longest > room:
         raise ValueError(f"{B} rows, {seqs} sequences of up to {room} tokens, a plan for {shared.num_seqs} with prefixes of up to {shared.longest}")
-    if not q.get_device() == out.get_device() == data.get_device() == page_table.get_device() == seq_lens.get_device() >= 0:
-        raise ValueError("tensors on one GPU")
+    on_one_gpu(q, out, data, page_table, seq_lens)
     L, desc, q_at, out_at, status = _lib.lib(), cache.desc(page_table), q.data_ptr(), out.data_ptr(), default_workspace(device).status.data_ptr()
     if dtype != torch.bfloat16 or cache.page_size != PAGE or dk > 128 or dv > 128 or (dk | dv | ldq) % 8 or ldo % 4 or q_at % 16 or out_at % 8 or data.data_ptr() % 16:
         rc = _lib.on_device(device, L.b200_attn_paged, q_at, ldq, out_at, ldo, hq, B, None, None, seq_lens.data_ptr(), ctypes.byref(desc), ctypes.byref(spec), status)

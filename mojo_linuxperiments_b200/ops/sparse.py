@@ -8,7 +8,7 @@ import torch
 
 from . import _lib
 from .attention import PagedKVCache
-from .pages import check_bounds
+from .pages import check_bounds, on_one_gpu
 from .workspace import default_workspace
 
 MAX_HEAD_DIM = 512
@@ -65,8 +65,7 @@ def attn_paged_sparse(q: torch.Tensor, hq: int, positions: torch.Tensor, seq_ids
         raise ValueError(f"{M} rows and {top} pages in one call")
     if seq_ids is None and M > seqs:
         raise ValueError(f"{M} rows of {seqs} sequences")
-    if not q.get_device() == out.get_device() == bounds.get_device() == page_table.get_device() == positions.get_device() >= 0:
-        raise ValueError("tensors on one GPU")
+    on_one_gpu(q, out, bounds, page_table, positions, seq_ids, seq_lens, chosen)
     if chosen is not None:
         assert chosen.dtype == torch.int32 and tuple(chosen.shape) == (M, kv_heads, top) and chosen.is_contiguous()
     if splits is None:

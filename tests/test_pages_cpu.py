@@ -118,3 +118,65 @@ def test_pieces_begin_where_the_chunk_of_a_prefix_does(chunk):
         for n in range(tokens, tokens + 2 * chunk, max(1, chunk // 7)):
             low = (n - 1) - (n - 1) % chunk
             assert low >= tokens or begin - 16 < low <= begin
+
+
+class _OnGpu(torch.Tensor):
+    """A tensor that says it is on the GPU"""
+
+    def get_device(self):
+        return 0
+
+
+def _gpu(t):
+    return t.as_subclass(_OnGpu)
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """Stands in for the library: what would have been launched"""
+    from types import SimpleNamespace
+    calls = []
+    for m in (PG, SP, SH):
+        monkeypatch.setattr(m._lib, "lib", lambda: SimpleNamespace(b200_page_bounds="page_bounds", b200_attn_paged_sparse="attn_paged_sparse"))
+        monkeypatch.setattr(m._lib, "on_device", lambda device, fn, *args: calls.append((fn, args)) or 0)
+        monkeypatch.setattr(m, "default_workspace", lambda device: SimpleNamespace(status=torch.zeros(4, dtype=torch.int32)))
+    return calls
+
+
+def _i32(*shape):
+    return torch.zeros(shape, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("host", ["all", "bounds", "page_table", "starts", "ends", "seq_ids", None])
+def test_bounds_of_tensors_on_the_host_are_refused(host, launches):
+    c = _cache()
+    t = {"page_table": _i32(3, 2), "starts": _i32(3), "ends": _i32(3), "seq_ids": _i32(3), "bounds": PG.bounds_for(c)}
+    c.data = c.data if host == "all" else _gpu(c.data)
+    t = {k: x if host in ("all", k) else _gpu(x) for k, x in t.items()}
+    if host is None:
+        PG.page_bounds(c, t["page_table"], t["starts"], t["ends"], t["seq_ids"], 1, t["bounds"])
+        assert len(launches) == 1
+        return
+    with pytest.raises(ValueError):
+        PG.page_bounds(c, t["page_table"], t["starts"], t["ends"], t["seq_ids"], 1, t["bounds"])
+    assert not launches
+
+
+@pytest.mark.parametrize("host", ["q", "page_table", "positions", "seq_ids", "seq_lens", "chosen", "out", None])
+def test_selections_by_tensors_on_the_host_are_refused(host, launches):
+    c = _cache()
+    c.data = _gpu(c.data)
+    t = {"q": torch.zeros(3, 4 * c.dk, dtype=torch.bfloat16), "out": torch.zeros(3, 4 * c.dv, dtype=torch.bfloat16), "page_table": _i32(3, 40), "positions": _i32(3),
+         "seq_ids": _i32(3), "seq_lens": _i32(3), "chosen": _i32(3, 2, 8)}
+    t = {k: x if k == host else _gpu(x) for k, x in t.items()}
+
+    def call():
+        SP.attn_paged_sparse(t["q"], 4, t["positions"], t["seq_ids"], c, t["page_table"], _gpu(PG.bounds_for(c)), A.attn_spec(0.1), t["out"],
+                             top=8, seq_lens=t["seq_lens"], chosen=t["chosen"], splits=1)
+    if host is None:
+        call()
+        assert len(launches) == 1
+        return
+    with pytest.raises(ValueError):
+        call()
+    assert not launches
