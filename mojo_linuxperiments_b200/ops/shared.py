@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 
 import torch
 
@@ -13,6 +14,7 @@ from .workspace import default_workspace
 KEY_TILE = 128                 # keys of a step of the kernel
 ROW_TILE = 128                 # rows (member x query head) of one of its two units
 MAX_PARTS = 32                 # parts of a prefix
+MAX_SPLITS = 8                 # CTAs of a cluster
 _INFO, _PIECE = 16, 8          # where the numbers per slot start, numbers per piece
 _ROWS, _KEYS, _ONE = 0, 1, 2   # two tiles of rows; one, and every other tile of keys for each unit; one unit
 
@@ -77,22 +79,23 @@ def cut_prefixes(groups, num_seqs: int, per_head: int, kv_heads: int, ctas: int,
     return info, pieces, order, base
 
 
+@lru_cache(maxsize=1024)
 def pick_own_splits(pairs: int, keys: int, per_head: int, num_sms: int) -> int:
-    """CTAs (one cluster) that share a slot's own keys, up to ``keys``, for a group of heads: as many as find a place at once with some left for the prefix, and at
-    least 128 keys each.  Up to eight heads leave places for three CTAs per SM (80 pairs with up to 2,000 keys: 22.5 us in four, 29.2 in two; 60: 20.2 in four, 25.5
+    """CTAs (one cluster) that share a slot's own keys, up to ``keys`` where it shares none, for a group of heads: as many as find a place at once with some left for the
+    prefix, and at least 128 keys each.  Not by what slots share at the moment: a captured call keeps its clusters while groups change.
+    Up to eight heads leave places for three CTAs per SM (80 pairs with up to 2,000 keys: 22.5 us in four, 29.2 in two; 60: 20.2 in four, 25.5
     in eight), more for two (34: 19.2 in four, 26.3 in eight).  16 slots with up to 150 keys take 8.9 us, 9.8 in two; 28 with up to 698 take 10.5 in four, 11.3 in eight."""
     s, most = 1, (4 * (3 if per_head <= 8 else 2) - 1) * num_sms // 4
-    while s < 8 and pairs * 2 * s <= most and keys // (2 * s) >= KEY_TILE:
+    while s < MAX_SPLITS and pairs * 2 * s <= most and keys // (2 * s) >= KEY_TILE:
         s *= 2
     return s
 
 
 class _Cut:
-    """A plan as the kernels read it, for one number of heads, and room for partial results."""
+    """A plan as the kernels read it, for one number of heads and of CTAs that share a slot's own keys, and room for partial results."""
 
-    def __init__(self, num_seqs: int, per_head: int, kv_heads: int, dv: int, chunk: int, room: int, device: torch.device):
-        self.per_head, self.kv_heads, self.chunk, self.room, self.sms = per_head, kv_heads, chunk, room, _lib.num_sms(device.index)
-        self.splits = 1                          # CTAs that share a slot's own keys
+    def __init__(self, num_seqs: int, per_head: int, kv_heads: int, dv: int, chunk: int, splits: int, device: torch.device):
+        self.per_head, self.kv_heads, self.chunk, self.splits, self.sms = per_head, kv_heads, chunk, splits, _lib.num_sms(device.index)
         self.max_pieces, self.rows = room_for(num_seqs, per_head, kv_heads, self.sms)
         self.pieces_at = (_INFO + 4 * num_seqs + 7) // 8 * 8
         self.slots_at = self.pieces_at + _PIECE * self.max_pieces
@@ -103,10 +106,9 @@ class _Cut:
         self.ring = [(buf, torch.cuda.Event()) for buf in torch.zeros(4, n, dtype=torch.int32, pin_memory=True)]
         self.turn = 0
 
-    def send(self, groups, num_seqs: int, alone: int) -> None:
-        heads, keys = self.kv_heads * -(-self.per_head // 16), self.room - alone
-        self.splits = pick_own_splits(num_seqs * heads, min(keys, self.chunk) if self.chunk else keys, self.per_head, self.sms)
-        info, pieces, order, rows = cut_prefixes(groups, num_seqs, self.per_head, self.kv_heads, self.sms, num_seqs * heads * self.splits, self.chunk)
+    def send(self, groups, num_seqs: int) -> None:
+        others = num_seqs * self.kv_heads * -(-self.per_head // 16) * self.splits
+        info, pieces, order, rows = cut_prefixes(groups, num_seqs, self.per_head, self.kv_heads, self.sms, others, self.chunk)
         assert len(pieces) <= self.max_pieces and rows <= self.rows
         buf, done = self.ring[self.turn]
         self.turn = (self.turn + 1) % len(self.ring)
@@ -132,7 +134,6 @@ class SharedPrefixes:
         self.num_seqs, self.device = int(num_seqs), torch.device(device)
         self.groups: list[tuple[list[int], int]] = []
         self.longest = 0                          # tokens of the longest prefix
-        self.alone = 0                            # tokens that every slot shares at least
         self._cuts: dict[tuple, _Cut] = {}
 
     def set(self, groups) -> None:
@@ -148,22 +149,22 @@ class SharedPrefixes:
             raise RuntimeError("groups are set between captured calls, which follow them")
         self.groups = [(slots, tokens) for slots, tokens in groups if len(slots) > 1 and tokens]      # a slot alone shares nothing
         self.longest = max((t for _, t in self.groups), default=0)
-        covered = sum(len(slots) for slots, _ in self.groups)
-        self.alone = min((t for _, t in self.groups), default=0) if covered == self.num_seqs else 0
         for cut in self._cuts.values():
-            cut.send(self.groups, self.num_seqs, self.alone)
+            cut.send(self.groups, self.num_seqs)
 
-    def cut_for(self, hq: int, cache: PagedKVCache, room: int, chunk: int = 0) -> _Cut:
-        device = cache.data.device
-        key = (hq, cache.kv_heads, cache.dv, chunk, room, device.index)
+    def cut_for(self, hq: int, cache: PagedKVCache, room: int, chunk: int = 0, splits: int | None = None) -> _Cut:
+        device, per_head = cache.data.device, hq // cache.kv_heads
+        if not splits:
+            splits = pick_own_splits(self.num_seqs * cache.kv_heads * -(-per_head // 16), min(room, chunk) if chunk > 0 else room, per_head, _lib.num_sms(device.index))
+        key = (hq, cache.kv_heads, cache.dv, chunk, splits, device.index)
         cut = self._cuts.get(key)
         if cut is None:
             if device != self.device and (device.type != self.device.type or self.device.index is not None):
                 raise ValueError(f"a plan for {self.device} and a cache on {device}")
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("the first call with a plan sends it to the device: make one before the capture")
-            cut = self._cuts[key] = _Cut(self.num_seqs, hq // cache.kv_heads, cache.kv_heads, cache.dv, chunk, room, device)
-            cut.send(self.groups, self.num_seqs, self.alone)
+            cut = self._cuts[key] = _Cut(self.num_seqs, per_head, cache.kv_heads, cache.dv, chunk, splits, device)
+            cut.send(self.groups, self.num_seqs)
         return cut
 
 
@@ -182,6 +183,8 @@ def attn_decode_shared(q: torch.Tensor, hq: int, seq_lens: torch.Tensor, cache: 
     assert width >= hq * dk and out_width >= hq * dv and hq % kv_heads == 0
     assert seq_lens.dtype == page_table.dtype == torch.int32 and page_table.is_contiguous() and seq_lens.is_contiguous()
     room = pages * cache.page_size
+    if splits and not 1 <= splits <= MAX_SPLITS:
+        raise ValueError(f"{splits} CTAs in a cluster of up to {MAX_SPLITS}")
     if B > seqs or B != shared.num_seqs or shared.longest > room:
         raise ValueError(f"{B} rows, {seqs} sequences of up to {room} tokens, a plan for {shared.num_seqs} with prefixes of up to {shared.longest}")
     on_one_gpu(q, out, data, page_table, seq_lens)
@@ -190,10 +193,10 @@ def attn_decode_shared(q: torch.Tensor, hq: int, seq_lens: torch.Tensor, cache: 
         rc = _lib.on_device(device, L.b200_attn_paged, q_at, ldq, out_at, ldo, hq, B, None, None, seq_lens.data_ptr(), ctypes.byref(desc), ctypes.byref(spec), status)
         _lib.check(rc, "attn_paged")
         return out
-    cut = shared.cut_for(hq, cache, room, spec.chunk)
+    cut = shared.cut_for(hq, cache, room, spec.chunk, splits)
     rc = _lib.on_device(
         device, L.b200_attn_decode_shared, q_at, ldq, out_at, ldo, hq, B, seq_lens.data_ptr(), ctypes.byref(desc),
-        ctypes.byref(spec), cut.plan.data_ptr(), cut.pieces_at, cut.slots_at, cut.max_pieces, cut.part.data_ptr(), cut.rows, splits or cut.splits, cut.sms,
+        ctypes.byref(spec), cut.plan.data_ptr(), cut.pieces_at, cut.slots_at, cut.max_pieces, cut.part.data_ptr(), cut.rows, cut.splits, cut.sms,
         status)
     _lib.check(rc, "attn_decode_shared")
     _lib.LAUNCHES[0] += 1                        # two kernels

@@ -297,3 +297,50 @@ def test_no_further_from_exact_than_decoding_alone():
             want[i:i + 16, h] = torch.softmax(q[i:i + 16].view(-1, hkv, per, d)[:, h].double() @ K.transpose(1, 2) * d ** -0.5, -1) @ V
     off = [float((x.view_as(want).double() - want).norm() / want.norm()) for x in (got, alone)]
     assert off[0] <= 1.05 * off[1], off
+
+
+def test_a_captured_call_has_the_clusters_that_sequences_without_groups_need(monkeypatch):
+    """Captured while all share most of what they hold, replayed when none shares anything: as many CTAs per slot as a plan without groups would have had,
+    and the same for page tables of any width that asks for as many."""
+    from mojo_linuxperiments_b200.ops import attention as A
+    from mojo_linuxperiments_b200.ops import shared as SH
+    lens, groups = [4100, 4200, 4097, 4150], [([0, 1, 2, 3], 4096)]
+    S = Sequences(lens, 8, 2, 128, 128, "bfloat16", groups=groups, seed=6)
+    q, seq_lens, spec = S.rows_of(4), torch.tensor(lens, dtype=torch.int32, device=DEV), A.attn_spec(0.1)
+    out, launched, run = torch.empty((4, 1024), dtype=S.dtype, device=DEV), [], SH._lib.on_device
+
+    def on_device(device, fn, *args):
+        launched.append(args[-3])
+        return run(device, fn, *args)
+    monkeypatch.setattr(SH._lib, "on_device", on_device)
+
+    def call(plan, table=S.table):
+        SH.attn_decode_shared(q, 8, seq_lens, S.cache, table, plan, spec, out)
+    plan, other = SH.SharedPrefixes(4, DEV), SH.SharedPrefixes(4, DEV)
+    plan.set(groups)
+    call(other)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(plan)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            call(plan)
+    torch.cuda.current_stream().wait_stream(side)
+    plan.set([])
+    call(plan)
+    assert len(set(launched)) == 1 and launched[0] > 1, launched
+    assert all(c.splits == launched[0] for c in plan._cuts.values())
+    for groups in ([], [([0, 1, 2, 3], 4096)], [([3, 1], 64)]):
+        plan.set(groups)
+        out.fill_(float("nan"))
+        g.replay()
+        status_ok()
+        for i, k in enumerate(lens):
+            want, tol = S.want(q, i, i, list(range(k)), 0.1, None, None)
+            assert worst(out[i], want, tol) <= 1
+    for more in range(20):
+        call(plan, torch.cat([S.table, S.table[:, :1].expand(-1, more)], 1).contiguous())
+    assert len(plan._cuts) == 1
+    with pytest.raises(ValueError):
+        SH.attn_decode_shared(q, 8, seq_lens, S.cache, S.table, plan, spec, out, splits=9)
