@@ -100,6 +100,7 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + B_COUNT);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* seen = reinterpret_cast<volatile int*>(tmem_slot + 2);       // with chunks: some row of the piece takes it; two pieces in turn
+  volatile int* gaps = reinterpret_cast<volatile int*>(tmem_slot + 4);       // some page of the piece does not exist; two pieces in turn
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int dk = p.c.dk, dv = p.c.dv, hkv = p.c.kv_heads, group = p.hq / hkv;
@@ -108,7 +109,7 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
   if (threadIdx.x == 0) {
     for (int i = 0; i < B_COUNT; ++i) mbar_init(bar(i), i >= B_PFULL && i < B_OFULL ? 4 : 1);
     *abort_flag = 0;
-    seen[0] = seen[1] = 0;
+    seen[0] = seen[1] = gaps[0] = gaps[1] = 0;
     mbar_fence_init();
   }
   if (warp == 1) { tmem_alloc(smem_u32(tmem_slot), 512); tmem_relinquish(); }
@@ -153,8 +154,9 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
         // the pages of four tiles are in the lanes, those of the next four on their way
         auto ids_of = [&](int j) {
           const int tok = e.key0 + j * SX_BN + lane * SX_PS;
-          const int pg = tok < kv_end ? pt[tok / SX_PS] : p.c.num_pages;       // pages behind the end are filled with zeros
-          if (pg >= 0 && pg <= p.c.num_pages) return pg;
+          if (tok >= kv_end) return p.c.num_pages;       // pages behind the end are filled with zeros, and so are those that do not exist
+          const int pg = pt[tok / SX_PS];
+          if (pg >= 0 && pg < p.c.num_pages) return pg;
           if (p.status) atomicCAS(p.status, 0, static_cast<int>(ST_BAD_ARGUMENT) | (26 << 8));
           return p.c.num_pages;
         };
@@ -237,7 +239,7 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
           }
           __syncwarp();
         } else if (threadIdx.x == 64) {
-          seen[turn ^ 1] = 0;                    // the other piece's, at which nobody looks any more
+          seen[turn ^ 1] = gaps[turn ^ 1] = 0;   // the other piece's, at which nobody looks any more
         }
       }
       kv += n;
@@ -255,6 +257,11 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
       const int kvh = item % hkv;
       const int row0 = e.row0 + (e.mode == SM_ROWS ? 128 * u : 0), rows = u < units_of(e) ? min(128, e.rows - (row0 - e.row0)) : 0;
       const bool idle = (warp & 3) * 32 >= rows;             // rows that nobody asked for: their weights are never looked at
+      const int keys = min(e.key1, room) - e.key0;
+      const int* pt = p.c.page_table + static_cast<size_t>(e.lead) * p.c.max_pages + e.key0 / SX_PS;
+      auto exists = [&](int t) { const int pg = pt[t]; return pg >= 0 && pg < p.c.num_pages; };
+      bool gap = false;
+      for (int t = threadIdx.x - 128; t * SX_PS < keys; t += 256) gap = gap || !exists(t);
       if (!idle) {
         const int row = row0 + r, member = row / group;
         const bool on = r < rows;
@@ -279,9 +286,11 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
         sx_copies_done();
         fence_proxy_async_smem();
       }
+      if (gap) gaps[turn] = 1;
       meet(M_QUERIES);
       if (threadIdx.x == 128) B200_TRACE(TK_ATTN_SHARED, 2); // queries in place
-      const int n = rows > 0 ? tiles_of(e, turn) : 0, keys = min(e.key1, room) - e.key0;
+      const int n = rows > 0 ? tiles_of(e, turn) : 0;
+      const bool gapped = gaps[turn] != 0;
       const int j0 = e.mode == SM_KEYS ? u : 0, step = e.mode == SM_KEYS ? 2 : 1;
       float m_ref = -INFINITY, l = 0.f;
       bool ok = true;
@@ -296,11 +305,14 @@ attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
           for (int c = 0; c < 4; ++c) tmem_ld_x32(t_s + c * 32, v[c]);
           tmem_ld_wait();
           const int here = keys - j * SX_BN;     // behind them the tile is zeros
-          if (here < SX_BN) {
+          if (here < SX_BN || gapped) {
+            unsigned on = 0xffu;                 // pages of the tile that exist
+            if (gapped) on = __ballot_sync(0xffffffffu, lane < 8 && lane * SX_PS < here && exists(j * (SX_BN / SX_PS) + lane));
 #pragma unroll
             for (int c = 0; c < 4; ++c)
 #pragma unroll
-              for (int i = 0; i < 32; ++i) if (c * 32 + i >= here) v[c][i] = 0xff800000u;      // -inf
+              for (int i = 0; i < 32; ++i)
+                if (c * 32 + i >= here || !(on >> ((c * 32 + i) / SX_PS) & 1u)) v[c][i] = 0xff800000u;      // -inf
           }
           float mx[4];
 #pragma unroll

@@ -344,3 +344,30 @@ def test_a_captured_call_has_the_clusters_that_sequences_without_groups_need(mon
     assert len(plan._cuts) == 1
     with pytest.raises(ValueError):
         SH.attn_decode_shared(q, 8, seq_lens, S.cache, S.table, plan, spec, out, splits=9)
+
+
+@pytest.mark.parametrize("bad", [-1, 1 << 30, "behind the last"])
+@pytest.mark.parametrize("hq,hkv,dk,chunk", [(8, 2, 128, None), (160, 1, 64, None), (6, 2, 40, 300), (8, 2, 128, 1000)])
+def test_pages_that_do_not_exist_are_left_out_and_told(hq, hkv, dk, chunk, bad):
+    """In a prefix (single pages, a whole tile of eight, the last one) and among a sequence's own keys: as if the sequences did not have these tokens."""
+    from mojo_linuxperiments_b200.ops import shared as SH
+    lens, groups = [700, 641, 640, 655], [([2, 0, 1, 3], 640)]
+    S = Sequences(lens, hq, hkv, dk, 64, "bfloat16", groups=groups, seed=5)
+    q, (s, g) = S.rows_of(4), S.heads_of(4)
+    plan = SH.SharedPrefixes(4, DEV)
+    plan.set(groups)
+    held = S.table.clone()
+    for gone, slots in (([3], range(4)), ([0, 17, 39], range(4)), (list(range(16, 24)) + [31], range(4)), (list(range(40)), range(4)), ([40, 42], [0]), ([], [])):
+        S.table.copy_(held)
+        for t in gone:
+            for i in slots:
+                S.table[i, t] = S.cache.num_pages if bad == "behind the last" else bad
+        out = _run(S, q, lens, plan, 0.2, s, g, chunk)
+        low = [(n - 1) - (n - 1) % chunk if chunk else 0 for n in lens]
+        if any(low[i] // 16 <= t <= (lens[i] - 1) // 16 for i in slots for t in gone):
+            with pytest.raises(RuntimeError, match="bad argument|status 6"):
+                status_ok()
+        status_ok()
+        for i, n in enumerate(lens):
+            want, tol = S.want(q, i, i, [t for t in range(low[i], n) if i not in slots or t // 16 not in gone], 0.2, s, g)
+            assert worst(out[i], want, tol) <= 1, (gone, i, worst(out[i], want, tol))
