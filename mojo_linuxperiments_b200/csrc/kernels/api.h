@@ -348,7 +348,7 @@ int b200_sparse_clusters(int size);          // clusters of that size that run a
 int b200_attn_paged_sparse(const void* q, long long ldq, void* out, long long ldo, int hq, int M, const int* positions, const int* seq_ids,
                            const int* seq_lens, const b200_paged_cache* cache, const void* bounds, const b200_attn_spec* spec, int top, int first,
                            int last, int splits, unsigned* scores, int* chosen, int* status, cudaStream_t stream);
-// Last tokens of sequences of which some share the pages of a prefix (attn_shared.cu; bf16, dk and dv up to 128, page size 16; -2 otherwise).  plan: which
+// Last tokens of sequences of which some share the pages of a prefix (attn_shared.cu; bf16, dk and dv up to 128, page size 16; -2 otherwise; scale > 0).  plan: which
 // pieces of which prefixes there are, on the device; part: room for their results, part_rows rows per KV head of dv + 2 floats.  splits: CTAs (a cluster)
 // per slot and KV head for the slot's own keys.
 int b200_attn_decode_shared(const void* q, long long ldq, void* out, long long ldo, int hq, int B, const int* seq_lens, const b200_paged_cache* cache,

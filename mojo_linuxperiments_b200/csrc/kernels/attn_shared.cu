@@ -616,7 +616,7 @@ extern "C" int b200_attn_decode_shared(const void* q, long long ldq, void* out, 
   if (B <= 0) return 0;
   if (!q || !out || !seq_lens || !c || !c->data || !c->page_table || !s || !plan || !part) return -1;
   if (!shared_takes(c, hq, ldq, ldo) || hq <= 0 || c->num_pages <= 0) return -2;
-  if (B > c->num_seqs || B > 65535 || splits < 1 || splits > 8 || max_pieces < 0 || part_rows <= 0 || num_sms <= 0) return -3;
+  if (B > c->num_seqs || B > 65535 || splits < 1 || splits > 8 || max_pieces < 0 || part_rows <= 0 || num_sms <= 0 || !(s->scale > 0.f)) return -3;
   if ((reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(out) & 7) || (reinterpret_cast<uintptr_t>(plan) & 15) ||
       (reinterpret_cast<uintptr_t>(part) & 15)) return -4;
   const uint64_t rec = static_cast<uint64_t>(c->kv_heads) * SX_PS * (c->dk + c->dv) * 2, kbytes = static_cast<uint64_t>(c->kv_heads) * SX_PS * c->dk * 2;

@@ -172,7 +172,7 @@ def attn_decode_shared(q: torch.Tensor, hq: int, seq_lens: torch.Tensor, cache: 
                        out: torch.Tensor, *, splits: int | None = None) -> torch.Tensor:
     """The last token of every slot (row b of q, already rotated, [B, hq dk], row stride free; its key is in the cache) against the first
     ``seq_lens[b]`` cached tokens of slot b.  Slots of a group of ``shared`` have the same pages in front, which are read once for all of them (bf16 heads of up
-    to 128, pages of 16; otherwise every slot reads its own way through ``attn_paged``); a slot that does not see the prefix up to its end, being shorter or in a later
+    to 128, pages of 16, a positive scale; otherwise every slot reads its own way through ``attn_paged``); a slot that does not see the prefix up to its end, being shorter or in a later
     chunk, reads alone.  An empty slot (length 0) gets zeros.
 
     ``splits``: CTAs that share a slot's own keys."""
@@ -189,7 +189,8 @@ def attn_decode_shared(q: torch.Tensor, hq: int, seq_lens: torch.Tensor, cache: 
         raise ValueError(f"{B} rows, {seqs} sequences of up to {room} tokens, a plan for {shared.num_seqs} with prefixes of up to {shared.longest}")
     on_one_gpu(q, out, data, page_table, seq_lens)
     L, desc, q_at, out_at, status = _lib.lib(), cache.desc(page_table), q.data_ptr(), out.data_ptr(), default_workspace(device).status.data_ptr()
-    if dtype != torch.bfloat16 or cache.page_size != PAGE or dk > 128 or dv > 128 or (dk | dv | ldq) % 8 or ldo % 4 or q_at % 16 or out_at % 8 or data.data_ptr() % 16:
+    # (the kernels of prefixes take maxima before they scale)
+    if not spec.scale > 0 or dtype != torch.bfloat16 or cache.page_size != PAGE or dk > 128 or dv > 128 or (dk | dv | ldq) % 8 or ldo % 4 or q_at % 16 or out_at % 8 or data.data_ptr() % 16:
         rc = _lib.on_device(device, L.b200_attn_paged, q_at, ldq, out_at, ldo, hq, B, None, None, seq_lens.data_ptr(), ctypes.byref(desc), ctypes.byref(spec), status)
         _lib.check(rc, "attn_paged")
         return out

@@ -371,3 +371,22 @@ def test_pages_that_do_not_exist_are_left_out_and_told(hq, hkv, dk, chunk, bad):
         for i, n in enumerate(lens):
             want, tol = S.want(q, i, i, [t for t in range(low[i], n) if i not in slots or t // 16 not in gone], 0.2, s, g)
             assert worst(out[i], want, tol) <= 1, (gone, i, worst(out[i], want, tol))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("scale", [0.0, -0.2])
+def test_scales_that_are_not_positive(scale, dtype):
+    """The largest product is not the largest score then: the same results in either type.  scale (q . k) is |scale| (-q . k): the definition is asked that
+    way, because its bound on the sums' error, (dk + 8) 2^-24 scale sum |q k|, is one for scales that are not negative."""
+    from mojo_linuxperiments_b200.ops import shared as SH
+    lens, groups = [300, 257, 256, 0], [([2, 0, 1], 240)]
+    S = Sequences([300, 257, 256, 1], 8, 2, 64, 64, dtype, groups=groups, seed=5)
+    s, g = S.heads_of(4)
+    q, plan = S.rows_of(4), SH.SharedPrefixes(4, DEV)
+    plan.set(groups)
+    out = _run(S, q, lens, plan, scale, s, g)
+    status_ok()
+    assert float(out[3].abs().max()) == 0
+    for i in range(3):
+        want, tol = S.want(-q, i, i, list(range(lens[i])), abs(scale), s, g)
+        assert worst(out[i], want, tol) <= 1, (i, worst(out[i], want, tol))
