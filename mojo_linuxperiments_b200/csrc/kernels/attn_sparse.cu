@@ -605,7 +605,10 @@ extern "C" int b200_attn_paged_sparse(const void* q, long long ldq, void* out, l
   p.q = q; p.ldq = ldq; p.out = out; p.ldo = ldo; p.hq = hq; p.M = M; p.hgroups = (hq / c->kv_heads + 15) / 16;
   p.positions = positions; p.seq_ids = seq_ids; p.seq_lens = seq_lens; p.c = *c; p.s = *s; p.bounds = bounds; p.scores = scores;
   p.top = top; p.first = first; p.last = last; p.splits = splits; p.chosen = chosen; p.status = status;
-  p.list_cap = (((top < c->max_pages ? top : c->max_pages) + splits - 1) / splits + 1 + 3) & ~3;
+  // pages of a row at most: those asked for, of those that it sees
+  int read = top < c->max_pages ? top : c->max_pages;
+  if (s->chunk > 0 && s->chunk / c->page_size + 2 < read) read = s->chunk / c->page_size + 2;
+  p.list_cap = ((read + splits - 1) / splits + 1 + 3) & ~3;
   if (static_cast<long long>(c->kv_heads) * p.hgroups > 65535) return -3;
   if (c->f32) return launch_sparse_any<float>(p, stream);
   if (c->page_size != 16 || c->dk > 128 || c->dv > 128 || c->dk % 8 || c->dv % 8 || ldq % 8 || ldo % 4 || (reinterpret_cast<uintptr_t>(q) & 15) ||

@@ -61,7 +61,8 @@ def attn_paged_sparse(q: torch.Tensor, hq: int, positions: torch.Tensor, seq_ids
     group = hq // kv_heads
     if dk > MAX_HEAD_DIM or dv > MAX_HEAD_DIM or dv == 0 or group * (dk + 127 & ~127) > MAX_QUERIES:
         raise ValueError(f"{hq} heads of {dk} and {dv} over {kv_heads}")
-    if M > MAX_ROWS or min(top, most) > 8 * LIST_PER_CTA:
+    read = min(top, most, spec.chunk // cache.page_size + 2 if spec.chunk > 0 else most)      # pages of a row at most
+    if M > MAX_ROWS or read > 8 * LIST_PER_CTA:
         raise ValueError(f"{M} rows and {top} pages in one call")
     if seq_ids is None and M > seqs:
         raise ValueError(f"{M} rows of {seqs} sequences")
@@ -69,8 +70,7 @@ def attn_paged_sparse(q: torch.Tensor, hq: int, positions: torch.Tensor, seq_ids
     if chosen is not None:
         assert chosen.dtype == torch.int32 and tuple(chosen.shape) == (M, kv_heads, top) and chosen.is_contiguous()
     if splits is None:
-        seen = min(most, spec.chunk // cache.page_size + 2) if spec.chunk > 0 else most
-        splits = pick_sparse_splits(M * kv_heads * ((group + 15) // 16), min(top, seen), clusters_at_once(device.index))
+        splits = pick_sparse_splits(M * kv_heads * ((group + 15) // 16), read, clusters_at_once(device.index))
     scores = torch.empty(M * kv_heads * most, dtype=torch.int32, device=device)
     rc = _lib.on_device(
         device, _lib.lib().b200_attn_paged_sparse, q.data_ptr(), ldq, out.data_ptr(), ldo, hq, M, positions.data_ptr(), _lib.ptr(seq_ids),

@@ -241,3 +241,24 @@ def test_queries_that_are_not_numbers_give_none(hq, hkv, dk, dv, dtype, sink):
     SP.attn_paged_sparse(q, hq, pos, None, S.cache, S.table, _bounds(S), A.attn_spec(0.1, sink=s), out, top=8)
     status_ok()
     assert torch.isnan(out[0, :dv]).all() and torch.isnan(out[1]).all() and torch.isfinite(out[0, dv:]).all() and torch.isfinite(out[2]).all()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_more_pages_than_a_chunk_has(dtype):
+    """Room for all pages of a table of 140,000, which no row ever sees: a row's list is as long as its chunk."""
+    S = Sequences([700, 300], 4, 2, 64, 64, dtype, seed=3)
+    bounds, held = _bounds(S), S.table
+    S.table = torch.full((2, 140000), S.rows[0][0], dtype=torch.int32, device=DEV)
+    S.table[:, :held.shape[1]] = held
+    q = S.rows_of(2)
+    from mojo_linuxperiments_b200.ops import attention as A
+    from mojo_linuxperiments_b200.ops import sparse as SP
+    for chunk in (50, 200):
+        for splits in (None, 1, 8):
+            out = torch.empty((2, 4 * 64), dtype=S.dtype, device=DEV)
+            positions = torch.tensor([699, 298], dtype=torch.int32, device=DEV)
+            SP.attn_paged_sparse(q, 4, positions, None, S.cache, S.table, bounds, A.attn_spec(0.2, chunk=chunk), out, top=140000, splits=splits)
+            status_ok()
+            for i, pos in enumerate((699, 298)):
+                want, tol = S.want(q, i, i, list(range(pos - pos % chunk, pos + 1)), 0.2, None, None)
+                assert worst(out[i], want, tol) <= 1
