@@ -104,7 +104,7 @@ class RuntimeConfig:
     fused_collectives: bool = True      # in-kernel peer-memory collectives; False = NCCL between kernels
     dtype: str = "bfloat16"             # "float32": everything in 32-bit (families that have such a form)
     kv_pool_tokens: int = 0             # tokens all sequences together may hold in the cache; 0: every slot its maximum
-    share_prefix: bool = False          # decoding: keys that forked sequences have in common are read once for all of them
+    share_prefix: bool = False          # decoding: keys that forked sequences have in common are read once for all of them (bf16 heads of up to 128, pages of 16)
     sparse_pages: int = 0               # decoding: pages that a KV head attends to, those of highest score; 0: all
     wait_limit_ms: int = 2000           # bound of every device-side wait
     debug: bool = False

@@ -14,7 +14,7 @@ import torch
 from ..ops import attention as A
 from ..ops import linear as L
 from ..ops.moe import ExpertSum
-from ..ops.shared import attn_decode_shared
+from ..ops.shared import attn_decode_shared, reads_prefixes_once
 from ..ops.sparse import attn_paged_sparse
 from ..parallel.comm import Comm
 from ..utils.trace import op_range
@@ -98,7 +98,7 @@ class Decoder:
                 kv.note_keys(l, *self._spans, max_len)
             v = qkv.view(M, self.hq + 2 * self.hkv, self.cfg.head_dim)[:, self.hq + self.hkv:]
             return A.attn_prefill(q, k_rot, v, cu_seqlens, max_len, scale=self.scale)
-        if kv.bounds[l] is not None or kv.shared is not None:
+        if kv.bounds[l] is not None or (kv.shared is not None and reads_prefixes_once(cache)):
             q = A.rope_kv_write(qkv, positions, self.cos, self.sin, self.hq, self.hkv, cache=cache, page_table=kv.page_table, seq_ids=None,
                                 q_norm_w=W.get("q_norm"), k_norm_w=W.get("k_norm"), eps=self.cfg.eps).view(M, -1)
             out, spec = torch.empty_like(q), A.attn_spec(self.scale)

@@ -12,7 +12,7 @@ from ..ops import attention as A
 from ..ops import dense as D
 from ..ops import latent as LT
 from ..ops import recurrent as R
-from ..ops.shared import attn_decode_shared
+from ..ops.shared import attn_decode_shared, reads_prefixes_once
 from ..ops.sparse import attn_paged_sparse
 from .kvcache import KVState
 from .layered_config import AttentionSpec, LatentSpec, MinGRUSpec
@@ -90,7 +90,7 @@ class Attention:
         spec = A.attn_spec(m.scale, chunk=m.chunk, sink=W["sink"], gate=qkvg[:, g0:g0 + m.heads])
         out = D.rows(qkvg.shape[0], m.heads * m.dv, self.dtype, qkvg.device)
         bounds = c.kv.bounds[run]
-        if c.decode and bounds is None and c.kv.shared is None:
+        if c.decode and bounds is None and (c.kv.shared is None or not reads_prefixes_once(cache)):
             return A.attn_decode_paged(qkvg, m.heads, c.positions, c.kv.seq_lens, self.cos, self.sin, cache, c.kv.page_table, spec, out)
         A.rotary_paged(qkvg, m.heads, c.positions, c.seq_ids, self.cos, self.sin, cache, c.kv.page_table)
         if bounds is not None:

@@ -168,6 +168,11 @@ class SharedPrefixes:
         return cut
 
 
+def reads_prefixes_once(cache: PagedKVCache) -> bool:
+    """Whether the kernels of prefixes take the heads and pages of ``cache``; otherwise sharing changes nothing, and the decode kernel for one sequence is the better one."""
+    return cache.data.dtype == torch.bfloat16 and cache.page_size == PAGE and cache.dk <= 128 and cache.dv <= 128 and (cache.dk | cache.dv) % 8 == 0
+
+
 def attn_decode_shared(q: torch.Tensor, hq: int, seq_lens: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor, shared: SharedPrefixes, spec,
                        out: torch.Tensor, *, splits: int | None = None) -> torch.Tensor:
     """The last token of every slot (row b of q, already rotated, [B, hq dk], row stride free; its key is in the cache) against the first
@@ -190,7 +195,7 @@ def attn_decode_shared(q: torch.Tensor, hq: int, seq_lens: torch.Tensor, cache: 
     on_one_gpu(q, out, data, page_table, seq_lens)
     L, desc, q_at, out_at, status = _lib.lib(), cache.desc(page_table), q.data_ptr(), out.data_ptr(), default_workspace(device).status.data_ptr()
     # (the kernels of prefixes take maxima before they scale)
-    if not spec.scale > 0 or dtype != torch.bfloat16 or cache.page_size != PAGE or dk > 128 or dv > 128 or (dk | dv | ldq) % 8 or ldo % 4 or q_at % 16 or out_at % 8 or data.data_ptr() % 16:
+    if not spec.scale > 0 or not reads_prefixes_once(cache) or ldq % 8 or ldo % 4 or q_at % 16 or out_at % 8 or data.data_ptr() % 16:
         rc = _lib.on_device(device, L.b200_attn_paged, q_at, ldq, out_at, ldo, hq, B, None, None, seq_lens.data_ptr(), ctypes.byref(desc), ctypes.byref(spec), status)
         _lib.check(rc, "attn_paged")
         return out

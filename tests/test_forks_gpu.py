@@ -164,3 +164,21 @@ def test_a_fork_of_everything_and_greedy_decoding():
     eng.release_sequence(2)
     with pytest.raises(ValueError):
         eng.fork_sequence(2, [1])
+
+
+def _wide_heads():
+    from dataclasses import replace
+    cfg = LC.tiny_volonex()
+    return replace(cfg, layers=tuple(replace(x, mixer=replace(x.mixer, dim=200, vdim=136)) for x in cfg.layers))
+
+
+@pytest.mark.parametrize("kind,rt", [("wide", {}), ("volonex32", {}), ("dense", {"page_size": 32})])
+def test_what_no_prefix_kernel_takes_decodes_as_without_the_option(kind, rt, monkeypatch):
+    """Heads above 128, 32 bits, other pages: the same kernels in a step, and the same bits."""
+    monkeypatch.setitem(CONFIGS, "wide", (_wide_heads, "bfloat16"))
+    plain = _engine(kind, **rt)
+    want = _forked(plain)
+    eng = _engine(kind, plain.model.w, share_prefix=True, **rt)
+    got = _forked(eng)
+    assert eng.kernels_per_step == plain.kernels_per_step
+    assert all(torch.equal(x, want[t][s]) for t, logits in enumerate(got) for s, x in logits.items())
