@@ -182,3 +182,100 @@ def test_what_no_prefix_kernel_takes_decodes_as_without_the_option(kind, rt, mon
     got = _forked(eng)
     assert eng.kernels_per_step == plain.kernels_per_step
     assert all(torch.equal(x, want[t][s]) for t, logits in enumerate(got) for s, x in logits.items())
+
+
+def _open_chunks():
+    """Layers that see everything, and one that sees up to seven pages."""
+    from dataclasses import replace
+    cfg = LC.tiny_volonex()
+    return replace(cfg, layers=tuple(replace(x, mixer=replace(x.mixer, chunk=100 if x.mixer.chunk == 24 else None)) for x in cfg.layers))
+
+
+def _select(eng, use_graph):
+    """A prompt of 182 tokens, forks and compaction between the steps; logits per step and slot"""
+    g = torch.Generator().manual_seed(12)
+    prompt, toks = torch.randint(0, eng.cfg.vocab, (182,), generator=g), torch.randint(0, eng.cfg.vocab, (14, SLOTS), generator=g)
+    eng.step([(0, prompt, [181])])
+    eng.fork_sequence(0, [1, 3])
+    out = []
+    for t in range(len(toks)):
+        if t == 6:
+            eng.fork_sequence(1, [2])
+        if t in (3, 9):
+            eng.compact_cache()
+        if t == 11:
+            eng.release_sequence(0)
+        live = [s for s in range(SLOTS) if (s != 2 or t >= 6) and (s != 0 or t < 11)]
+        out += [x[0].clone() for x in eng.step([(s, toks[t][s:s + 1], [0]) for s in live], use_graph=use_graph)]
+    eng.check_status()
+    return out
+
+
+@pytest.mark.parametrize("kind", ["dense", "open", "open32"])
+def test_decoding_attends_to_the_pages_that_the_real_keys_select(kind, monkeypatch):
+    """Four pages of up to thirteen, one of them by score.  Every call of an eager run is held against 64 bits: the bounds that the engine keeps are those of the keys in its
+    cache, through prompts in portions of 24 tokens (16 and 24 are no multiples of one another: portions begin inside pages), decoding, forks and compaction; the pages are
+    those of the largest scores by these keys; the result is the attention over them.  The captured step gives the same bits."""
+    from mojo_linuxperiments_b200.models import decoder, mixers
+    from mojo_linuxperiments_b200.ops.sparse import attn_paged_sparse
+    from paged_cases import HALF_STEP
+    monkeypatch.setitem(CONFIGS, "open", (_open_chunks, "bfloat16"))
+    monkeypatch.setitem(CONFIGS, "open32", (_open_chunks, "float32"))
+    rt = {} if kind == "dense" else {"max_prefill_tokens": 24}
+    graphs = _engine(kind, sparse_pages=4, **rt)
+    want = _select(graphs, True)
+
+    top, first, last, by_score, asked = 4, 1, 2, [0], {}
+    make = mixers.A.attn_spec
+
+    def attn_spec(scale, *, chunk=None, sink=None, gate=None):
+        asked.update(scale=scale, chunk=chunk, sink=sink, gate=gate)
+        return make(scale, chunk=chunk, sink=sink, gate=gate)
+
+    def checked(q, hq, positions, seq_ids, cache, table, bounds, spec, out, *, top, seq_lens):
+        chosen = torch.empty((positions.numel(), cache.kv_heads, top), dtype=torch.int32, device=q.device)
+        attn_paged_sparse(q, hq, positions, seq_ids, cache, table, bounds, spec, out, top=top, seq_lens=seq_lens, chosen=chosen)
+        per, half, dk, dv = hq // cache.kv_heads, HALF_STEP[q.dtype], cache.dk, cache.dv
+        for b, (pos, n) in enumerate(zip(positions.tolist(), seq_lens.tolist())):
+            if n == 0:
+                continue
+            low = pos - pos % asked["chunk"] if asked["chunk"] else 0
+            p0, p1 = low // 16, pos // 16 + 1
+            pages = table[b, p0:p1].long()
+            K, V = cache.keys()[pages].double(), cache.values()[pages].double()              # [pages][kv_heads][16][d]
+            assert torch.equal(bounds[pages[:-1]], torch.stack([K[:-1].amin(2), K[:-1].amax(2)], 2).to(q.dtype))
+            for h in range(cache.kv_heads):
+                x = q[b, :hq * dk].double().view(hq, dk)[h * per:(h + 1) * per]
+                got = [c - p0 for c in chosen[b, h].tolist() if c >= 0]
+                if p1 - p0 <= top:
+                    assert got == list(range(p1 - p0))
+                else:
+                    terms = torch.maximum(x[:, None] * K[:-1, h].amin(1), x[:, None] * K[:-1, h].amax(1))      # of every page but the last
+                    score, off = terms.sum(-1).amax(0).tolist(), 2 * dk * 2.0 ** -24 * float(terms.abs().sum(-1).max())
+                    free = range(first, p1 - p0 - last)
+                    taken = [c for c in got if c in free]
+                    assert len(got) == top and got[0] == 0 and got[-2:] == [p1 - p0 - 2, p1 - p0 - 1] and len(taken) == 1
+                    assert score[taken[0]] >= max(score[c] for c in free) - 2 * off
+                    by_score[0] += taken[0] != free[-1]
+                at = torch.tensor([(c, r) for c in got for r in range(16) if low <= (p0 + c) * 16 + r <= pos], device=q.device)
+                k, v = K[at[:, 0], h, at[:, 1]], V[at[:, 0], h, at[:, 1]]
+                s = x @ k.t() * asked["scale"]
+                off = (dk + 8) * 2.0 ** -24 * float((x.abs() @ k.abs().t() * asked["scale"]).max())
+                if asked["sink"] is not None:
+                    s = torch.cat([s, asked["sink"][h * per:(h + 1) * per].double()[:, None]], 1)
+                w = torch.softmax(s, 1)[:, :len(at)]
+                f = torch.sigmoid(asked["gate"][b, h * per:(h + 1) * per].double())[:, None] if asked["gate"] is not None else 1.0
+                o, a = w @ v * f, w @ v.abs() * f
+                # as in paged_cases: the weights' rounding in the numerator and the denominator, sums and exponentials, the result's rounding
+                tol = half * o.abs() + ((2 * half if q.dtype != torch.float32 else 0.0) + 2 * off + 2.0 ** -18 + len(at) * 2.0 ** -23) * a + 1e-30
+                err = (out[b, :hq * dv].double().view(hq, dv)[h * per:(h + 1) * per] - o).abs()
+                assert bool((err <= tol).all()), (b, h, float((err / tol).max()))
+        return out
+
+    eager = _engine(kind, graphs.model.w, sparse_pages=4, **rt)
+    for m in (decoder, mixers):
+        monkeypatch.setattr(m, "attn_paged_sparse", checked)
+    monkeypatch.setattr(mixers.A, "attn_spec", attn_spec)
+    got = _select(eager, False)
+    assert by_score[0] > 50                        # the page before the last two is not all that is ever taken
+    assert len(got) == len(want) and all(torch.equal(a, b) for a, b in zip(got, want))
