@@ -130,6 +130,8 @@ class Engine:
         if self.kv is not None:
             r["kv_pages"] = {"total": self.kv.num_pages - 1, "in_use": self.kv.pages_in_use(), "high_water": self.kv.pages_high_water,
                              "page_tokens": self.kv.page_size, "shared": len(self.kv._sharers)}
+            if self.kv.shared is not None:       # beside the arena: what its kernels exchange is known at the first step
+                r["shared_prefixes"] = {"groups": len(self.kv.shared.groups), "bytes": self.kv.shared.nbytes()}
         return r
 
     def prefill(self, prompts, use_graph: bool = True) -> torch.Tensor:

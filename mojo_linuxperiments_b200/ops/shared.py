@@ -152,6 +152,10 @@ class SharedPrefixes:
         for cut in self._cuts.values():
             cut.send(self.groups, self.num_seqs)
 
+    def nbytes(self) -> int:
+        """Device bytes of what the calls so far have made: lists of pieces and room for partial results (128 slots, 32 heads of 128 over 8: 42 MiB)."""
+        return sum(cut.plan.nbytes + cut.part.nbytes for cut in self._cuts.values())
+
     def cut_for(self, hq: int, cache: PagedKVCache, room: int, chunk: int = 0, splits: int | None = None) -> _Cut:
         device, per_head = cache.data.device, hq // cache.kv_heads
         if not splits:

@@ -279,3 +279,14 @@ def test_decoding_attends_to_the_pages_that_the_real_keys_select(kind, monkeypat
     got = _select(eager, False)
     assert by_score[0] > 50                        # the page before the last two is not all that is ever taken
     assert len(got) == len(want) and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_what_shared_prefixes_hold_is_reported():
+    eng = _engine("volonex", share_prefix=True)
+    assert eng.memory_report()["shared_prefixes"] == {"groups": 0, "bytes": 0}
+    before = torch.cuda.memory_allocated()
+    _forked(eng)
+    rep, cuts = eng.memory_report()["shared_prefixes"], eng.kv.shared._cuts.values()
+    assert rep["groups"] == len(eng.kv.shared.groups)
+    assert 0 < rep["bytes"] == sum(c.plan.numel() * 4 + c.part.numel() * 4 for c in cuts) <= torch.cuda.memory_allocated() - before
+    assert "shared_prefixes" not in _engine("volonex").memory_report()
