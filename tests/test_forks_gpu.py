@@ -290,3 +290,24 @@ def test_what_shared_prefixes_hold_is_reported():
     assert rep["groups"] == len(eng.kv.shared.groups)
     assert 0 < rep["bytes"] == sum(c.plan.numel() * 4 + c.part.numel() * 4 for c in cuts) <= torch.cuda.memory_allocated() - before
     assert "shared_prefixes" not in _engine("volonex").memory_report()
+
+
+@pytest.mark.parametrize("option", [{}, {"share_prefix": True}])
+@pytest.mark.parametrize("kind", ["volonex", "volonex32", "rakelorn"])
+def test_forked_slots_go_on_with_portions_of_their_own(kind, option, alone):
+    """Behind a common beginning every slot has a portion of several tokens, of its own length, and then decodes: as if each had been run by itself, in the same portions."""
+    weights, _ = alone(kind)
+    one, eng = _engine(kind, weights, max_prefill_tokens=24), _engine(kind, weights, max_prefill_tokens=24, **option)
+    prompt, toks = _tokens(eng.cfg.vocab)
+    own = [(s, prompt[5 * s:5 * s + 7 + 9 * s], [6 + 9 * s]) for s in range(SLOTS)]
+    for s in range(SLOTS):
+        one.step([(s, prompt, [PROMPT - 1])])
+    eng.step([(0, prompt, [PROMPT - 1])])
+    eng.fork_sequence(0, [1, 2, 3])
+    want, got = one.step(own), eng.step(own)
+    assert all(_rel(a, b) < TOL[CONFIGS[kind][1]] / 4 for a, b in zip(got, want))
+    for t in range(6):
+        entries = [(s, toks[t][s:s + 1], [0]) for s in range(SLOTS)]
+        want, got = one.step(entries), eng.step(entries)
+        assert all(_rel(a, b) < TOL[CONFIGS[kind][1]] / (1 if option else 4) for a, b in zip(got, want)), t
+    eng.check_status()
