@@ -358,7 +358,19 @@ def attn_spec(scale: float, *, chunk: int | None = None, sink: torch.Tensor | No
     in the softmax's denominator; ``gate`` [M, hq] (row stride free): logits of a sigmoid on each head's output."""
     if sink is not None:
         assert sink.dtype == torch.float32 and sink.is_contiguous()
-    return _lib.AttnSpecDesc(float(scale), int(chunk or 0), _lib.ptr(sink), _lib.ptr(gate), gate.stride(0) if gate is not None else 0)
+    spec = _lib.AttnSpecDesc(float(scale), int(chunk or 0), _lib.ptr(sink), _lib.ptr(gate), gate.stride(0) if gate is not None else 0)
+    spec.tensors = (sink, gate)            # they live as long as their addresses
+    return spec
+
+
+def check_spec(spec, rows: int, hq: int, q: torch.Tensor) -> None:
+    """Sink and gate of a call are those of ``rows`` rows of ``hq`` heads, on the GPU and of the type of ``q``."""
+    sink, gate = spec.tensors
+    if sink is not None and (sink.numel() < hq or sink.get_device() != q.get_device()):
+        raise ValueError(f"sink of {sink.numel()} for {hq} heads, on {sink.device}")
+    if gate is not None and (gate.dim() != 2 or gate.shape[0] < rows or gate.shape[1] < hq or gate.dtype != q.dtype or (hq > 1 and gate.stride(1) != 1)
+                             or gate.get_device() != q.get_device()):
+        raise ValueError(f"gate {tuple(gate.shape)} {gate.dtype} with strides {gate.stride()} for {rows} rows of {hq} heads of {q.dtype}, on {gate.device}")
 
 
 def rotary_paged(qkv: torch.Tensor, hq: int, positions: torch.Tensor, seq_ids: torch.Tensor | None, cos: torch.Tensor | None,

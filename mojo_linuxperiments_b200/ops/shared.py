@@ -7,7 +7,7 @@ from functools import lru_cache
 import torch
 
 from . import _lib
-from .attention import PAGE, PagedKVCache
+from .attention import PAGE, PagedKVCache, check_spec
 from .pages import on_one_gpu
 from .workspace import default_workspace
 
@@ -197,6 +197,7 @@ def attn_decode_shared(q: torch.Tensor, hq: int, seq_lens: torch.Tensor, cache: 
     if B > seqs or B != shared.num_seqs or shared.longest > room:
         raise ValueError(f"{B} rows, {seqs} sequences of up to {room} tokens, a plan for {shared.num_seqs} with prefixes of up to {shared.longest}")
     on_one_gpu(q, out, data, page_table, seq_lens)
+    check_spec(spec, B, hq, q)
     L, desc, q_at, out_at, status = _lib.lib(), cache.desc(page_table), q.data_ptr(), out.data_ptr(), default_workspace(device).status.data_ptr()
     # (the kernels of prefixes take maxima before they scale)
     if not spec.scale > 0 or not reads_prefixes_once(cache) or ldq % 8 or ldo % 4 or q_at % 16 or out_at % 8 or data.data_ptr() % 16:

@@ -7,7 +7,7 @@ from functools import lru_cache
 import torch
 
 from . import _lib
-from .attention import PagedKVCache
+from .attention import PagedKVCache, check_spec
 from .pages import check_bounds, on_one_gpu
 from .workspace import default_workspace
 
@@ -67,6 +67,7 @@ def attn_paged_sparse(q: torch.Tensor, hq: int, positions: torch.Tensor, seq_ids
     if seq_ids is None and M > seqs:
         raise ValueError(f"{M} rows of {seqs} sequences")
     on_one_gpu(q, out, bounds, page_table, positions, seq_ids, seq_lens, chosen)
+    check_spec(spec, M, hq, q)
     if chosen is not None:
         assert chosen.dtype == torch.int32 and tuple(chosen.shape) == (M, kv_heads, top) and chosen.is_contiguous()
     if splits is None:

@@ -1,4 +1,6 @@
 """What copies of pages, their bounds and the attentions that select or share them refuse, before anything is launched."""
+from types import SimpleNamespace
+
 import pytest
 import torch
 
@@ -134,7 +136,6 @@ def _gpu(t):
 @pytest.fixture
 def launches(monkeypatch):
     """Stands in for the library: what would have been launched"""
-    from types import SimpleNamespace
     calls = []
     for m in (PG, SP, SH):
         monkeypatch.setattr(m._lib, "lib", lambda: SimpleNamespace(b200_page_bounds="page_bounds", b200_attn_paged_sparse="attn_paged_sparse"))
@@ -180,3 +181,44 @@ def test_selections_by_tensors_on_the_host_are_refused(host, launches):
     with pytest.raises(ValueError):
         call()
     assert not launches
+
+
+_SPECS = {"fits": {}, "sink on the host": {"sink": lambda: torch.zeros(4)}, "gate on the host": {"gate": lambda: torch.zeros(3, 4, dtype=torch.bfloat16)},
+          "few sinks": {"sink": lambda: _gpu(torch.zeros(3))}, "few rows": {"gate": lambda: _gpu(torch.zeros(2, 4, dtype=torch.bfloat16))},
+          "few heads": {"gate": lambda: _gpu(torch.zeros(3, 3, dtype=torch.bfloat16))}, "another type": {"gate": lambda: _gpu(torch.zeros(3, 4))},
+          "heads apart": {"gate": lambda: _gpu(torch.zeros(4, 3, dtype=torch.bfloat16).t())}, "one dimension": {"gate": lambda: _gpu(torch.zeros(12, dtype=torch.bfloat16))}}
+
+
+@pytest.mark.parametrize("what", list(_SPECS))
+@pytest.mark.parametrize("op", ["sparse", "shared"])
+def test_sinks_and_gates_that_do_not_fit_are_refused(op, what, launches, monkeypatch):
+    c = _cache()
+    c.data = _gpu(c.data)
+    given = {"sink": lambda: _gpu(torch.zeros(4)), "gate": lambda: _gpu(torch.zeros(3, 9, dtype=torch.bfloat16)[:, :4]), **_SPECS[what]}
+    spec = A.attn_spec(0.1, **{k: f() for k, f in given.items()})
+    q, out, table, n = _gpu(torch.zeros(3, 4 * c.dk, dtype=torch.bfloat16)), _gpu(torch.zeros(3, 4 * c.dv, dtype=torch.bfloat16)), _gpu(_i32(3, 40)), _gpu(_i32(3))
+    monkeypatch.setattr(SH._lib, "lib", lambda: SimpleNamespace(b200_attn_paged_sparse="sparse", b200_attn_decode_shared="shared"))
+    no_plan = torch.zeros(1, dtype=torch.int32)
+    monkeypatch.setattr(SH.SharedPrefixes, "cut_for", lambda *a: SimpleNamespace(plan=no_plan, pieces_at=0, slots_at=0, max_pieces=0, part=no_plan, rows=1,
+                                                                                                    splits=1, sms=1))
+
+    def call():
+        if op == "sparse":
+            SP.attn_paged_sparse(q, 4, n, None, c, table, _gpu(PG.bounds_for(c)), spec, out, top=8, splits=1)
+        else:
+            SH.attn_decode_shared(q, 4, n, c, table, SH.SharedPrefixes(3, "cpu"), spec, out)
+    if what == "fits":
+        call()
+        assert len(launches) == 1
+        return
+    with pytest.raises(ValueError):
+        call()
+    assert not launches
+
+
+def test_sinks_and_gates_live_as_long_as_their_spec():
+    import weakref
+    gate = torch.zeros(3, 4)
+    alive, spec = weakref.ref(gate), A.attn_spec(0.1, gate=gate)
+    del gate
+    assert alive() is not None and spec.gate == alive().data_ptr()
