@@ -69,8 +69,9 @@ def check_bounds(cache: PagedKVCache, bounds: torch.Tensor) -> None:
 def on_one_gpu(*tensors: torch.Tensor | None) -> None:
     """Kernels are given addresses: those of one GPU's memory."""
     index = tensors[0].get_device()
-    if index < 0 or any(t is not None and t.get_device() != index for t in tensors):
-        raise ValueError("tensors on one GPU")
+    for t in tensors:
+        if t is not None and (t.get_device() != index or index < 0):
+            raise ValueError("tensors on one GPU")
 
 
 def page_bounds(cache: PagedKVCache, page_table: torch.Tensor, starts: torch.Tensor, ends: torch.Tensor, seq_ids: torch.Tensor | None, max_tokens: int,
