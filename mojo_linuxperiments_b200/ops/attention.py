@@ -365,12 +365,13 @@ def attn_spec(scale: float, *, chunk: int | None = None, sink: torch.Tensor | No
 
 def check_spec(spec, rows: int, hq: int, q: torch.Tensor) -> None:
     """Sink and gate of a call are those of ``rows`` rows of ``hq`` heads, on the GPU and of the type of ``q``."""
-    sink, gate = spec.tensors
-    if sink is not None and (sink.numel() < hq or sink.get_device() != q.get_device()):
+    (sink, gate), device = spec.tensors, q.get_device()
+    if sink is not None and (sink.numel() < hq or sink.get_device() != device):
         raise ValueError(f"sink of {sink.numel()} for {hq} heads, on {sink.device}")
-    if gate is not None and (gate.dim() != 2 or gate.shape[0] < rows or gate.shape[1] < hq or gate.dtype != q.dtype or (hq > 1 and gate.stride(1) != 1)
-                             or gate.get_device() != q.get_device()):
-        raise ValueError(f"gate {tuple(gate.shape)} {gate.dtype} with strides {gate.stride()} for {rows} rows of {hq} heads of {q.dtype}, on {gate.device}")
+    if gate is not None:
+        given, heads = gate.shape
+        if given < rows or heads < hq or gate.dtype != q.dtype or gate.get_device() != device or (heads > 1 and gate.stride(1) != 1):
+            raise ValueError(f"gate {tuple(gate.shape)} {gate.dtype} with strides {gate.stride()} for {rows} rows of {hq} heads of {q.dtype}, on {gate.device}")
 
 
 def rotary_paged(qkv: torch.Tensor, hq: int, positions: torch.Tensor, seq_ids: torch.Tensor | None, cos: torch.Tensor | None,
