@@ -8,10 +8,10 @@
 // follows them.  The second takes each sequence's own keys (decode_warp.cuh) while the first still runs, joins the pieces of the prefix, adds sink
 // and gate and writes the output; it waits for the first only there.
 //
-// 4 sequences behind 512 tokens (32 heads over 8, rows of 128): 10.3 us, a chain of latencies: start 0.5, plan and queries 2, tiles 2.5, results 2.5, join 2.
-// 32 behind 2,048 tokens with up to 300 of their own: 17 us.  128 behind 32,768 with up to 1,000 of their own: 125 us, 71 for the prefix, then 54 for the own
-// keys, whose CTAs find no place beside the pieces.  (In one kernel's registers beside the pieces: 166 us and more.  Own keys by as many CTAs as there are places,
-// one slot after the other and the joins shared out at the end: 135 us.)
+// 4 sequences behind 512 tokens (32 heads over 8, rows of 128): 11.8 us, a chain of latencies: start 0.5, plan and queries 2, tiles 2.5, results 2.5, join 2, and a cluster
+// of four CTAs per slot and KV head for what may be own keys.  32 behind 2,048 tokens with up to 300 of their own: 17.6 us.  128 behind 32,768 with up to 1,000 of their
+// own: 132 us, 78 for the prefix, then 54 for the own keys, whose CTAs find no place beside the pieces.  (Where that was 125: in one kernel's registers beside the pieces
+// 166 us and more; own keys by as many CTAs as there are places, one slot after the other and the joins shared out at the end, 135 us.)
 #include "ptx.cuh"
 #include "api.h"
 #include "launch.cuh"
@@ -70,9 +70,9 @@ __device__ __forceinline__ void sx_copies_done() { asm volatile("cp.async.wait_a
 // (thread <-> row) and keep O in tensor memory.  Where a group has more than 128 rows the units share the keys, otherwise each has every other tile.  Results are
 // stored with the rows of a tile next to each other, so that a warp's stores and the loads of a slot's heads are whole sectors.
 //
-// A step of both units, 2 x 128 x 128 scores and their products, takes 2.25 us at the 1.5 GHz that this load leaves; the tensor cores, the exponentials and the reads of
-// shared memory would take 1.4 each.  The rest is the way of one unit from its scores to its weights and back, which the other unit covers in part.  Measured on 128
-// sequences behind 32,768 tokens and not kept: scores of 64 keys at a time, two ahead (144 us for 127: MMAs 64 wide read their rows as often as wide ones), two
+// A step of both units, 2 x 128 x 128 scores and their products, takes 2.15 us at the 1.5 GHz that this load leaves, 2.4 to 2.7 where softmaxes are sharp and maxima move
+// on; the tensor cores, the exponentials and the reads of shared memory would take 1.4 each.  The rest is the way of one unit from its scores to its weights and back, which the other unit covers in part.  Measured on 128
+// sequences behind 32,768 tokens, when the step kept took 124 to 136, and not kept: scores of 64 keys at a time, two ahead (144 us for 127: MMAs 64 wide read their rows as often as wide ones), two
 // warpgroups per unit (156 for 136), a quarter or half of the exponentials as polynomials (125, 128 for 125), columns reread in short loops (130 for 125), pages asked for
 // into L2 two or three tiles ahead (135 for 126).
 constexpr int SX_THREADS = 384, SX_BN = 128, SX_PS = 16;
