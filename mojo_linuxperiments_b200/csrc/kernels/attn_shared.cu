@@ -70,11 +70,11 @@ __device__ __forceinline__ void sx_copies_done() { asm volatile("cp.async.wait_a
 // (thread <-> row) and keep O in tensor memory.  Where a group has more than 128 rows the units share the keys, otherwise each has every other tile.  Results are
 // stored with the rows of a tile next to each other, so that a warp's stores and the loads of a slot's heads are whole sectors.
 //
-// A step of both units, 2 x 128 x 128 scores and their products, takes 2.15 us at the 1.5 GHz that this load leaves, 2.4 to 2.7 where softmaxes are sharp and maxima move
-// on; the tensor cores, the exponentials and the reads of shared memory would take 1.4 each.  The rest is the way of one unit from its scores to its weights and back, which the other unit covers in part.  Measured on 128
-// sequences behind 32,768 tokens, when the step kept took 124 to 136, and not kept: scores of 64 keys at a time, two ahead (144 us for 127: MMAs 64 wide read their rows as often as wide ones), two
-// warpgroups per unit (156 for 136), a quarter or half of the exponentials as polynomials (125, 128 for 125), columns reread in short loops (130 for 125), pages asked for
-// into L2 two or three tiles ahead (135 for 126).
+// A step of both units, 2 x 128 x 128 scores and their products, takes 2.15 us at the 1.5 GHz that this load leaves, 2.4 to 2.7 where softmaxes are sharp and maxima
+// move on; the tensor cores, the exponentials and the reads of shared memory would take 1.4 each.  The rest is the way of one unit from its scores to its weights and
+// back, which the other unit covers in part.  Measured on 128 sequences behind 32,768 tokens, when the step kept took 124 to 136, and not kept: scores of 64 keys at a
+// time, two ahead (144 us for 127: MMAs 64 wide read their rows as often as wide ones), two warpgroups per unit (156 for 136), a quarter or half of the exponentials as
+// polynomials (125, 128 for 125), columns reread in short loops (130 for 125), pages asked for into L2 two or three tiles ahead (135 for 126).
 constexpr int SX_THREADS = 384, SX_BN = 128, SX_PS = 16;
 // registers: 384 x 168 at launch, 128 x (72 + 216 + 216) afterwards, which is as many
 constexpr int SX_REGS_FEW = 72, SX_REGS_MANY = 216;

@@ -128,7 +128,7 @@ class SharedPrefixes:
     one group at most; one in none reads its keys alone.
 
     Kept from step to step, like the page table; ``set`` changes it between steps, also under captured calls, which follow it.  It holds the room for
-    partial results as well: calls that may overlap on the GPU (different streams) use different objects."""
+    partial results as well: calls that may overlap on the GPU (different streams) use different objects, and an object is kept until the calls with it have ended."""
 
     def __init__(self, num_seqs: int, device):
         self.num_seqs, self.device = int(num_seqs), torch.device(device)
@@ -181,10 +181,10 @@ def attn_decode_shared(q: torch.Tensor, hq: int, seq_lens: torch.Tensor, cache: 
                        out: torch.Tensor, *, splits: int | None = None) -> torch.Tensor:
     """The last token of every slot (row b of q, already rotated, [B, hq dk], row stride free; its key is in the cache) against the first
     ``seq_lens[b]`` cached tokens of slot b.  Slots of a group of ``shared`` have the same pages in front, which are read once for all of them (bf16 heads of up
-    to 128, pages of 16, a positive scale; otherwise every slot reads its own way through ``attn_paged``); a slot that does not see the prefix up to its end, being shorter or in a later
-    chunk, reads alone.  An empty slot (length 0) gets zeros.
+    to 128, pages of 16, a positive scale; otherwise every slot reads its own way through ``attn_paged``); a slot that does not see the prefix up to its
+    end, being shorter or in a later chunk, reads alone.  An empty slot (length 0) gets zeros.
 
-    ``splits``: CTAs that share a slot's own keys."""
+    ``splits``: CTAs that share a slot's own keys.  The first call for each number of them sends the plan to the device and is not part of a capture."""
     B, dk, dv, kv_heads, data = seq_lens.numel(), cache.dk, cache.dv, cache.kv_heads, cache.data
     (rows, width), (out_rows, out_width), (seqs, pages) = q.shape, out.shape, page_table.shape
     (ldq, q_step), (ldo, out_step), dtype, device = q.stride(), out.stride(), data.dtype, q.device

@@ -40,8 +40,8 @@ def attn_paged_sparse(q: torch.Tensor, hq: int, positions: torch.Tensor, seq_ids
     """Rows of q (already rotated; [M, hq dk], row stride free) against the cached keys of their sequence, as ``attn_paged`` does it, but of every
     KV head only ``top`` pages: the ``first`` pages that the row sees, the ``last`` up to its own (which counts among them), and those others whose
     score is highest, the lower page first where scores are equal.  A page's score is the largest product that any query head of the group could
-    have with a key within the page's ``bounds`` (``page_bounds``; those of the last pages are not read).  A row that sees no more than ``top``
-    pages attends to all.
+    have with a key within the page's ``bounds`` (``page_bounds``; those of the last pages are not read); where these are not finite it counts as the
+    highest.  A row that sees no more than ``top`` pages attends to all.
 
     ``chosen`` int32 [M, kv_heads, top]: receives the pages read (their place in the sequence, ascending, -1 behind them)."""
     M = positions.numel()
